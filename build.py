@@ -112,7 +112,10 @@ def build_gpu(force=False, verbose=False, jobs_n=8):
     hdr = _newest_header_mtime()
     (BUILD / "gpu").mkdir(parents=True, exist_ok=True)
 
-    common = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"--offload-arch={GPU_ARCH}", "-I" + str(CSRC), "-I" + str(rocm / "include")]
+    # No packed fp32 instructions (v_pk_add_f32 and its kin): hipcc forms them out of ordinary scalar code, and some of
+    # their operand forms have given wrong results on this part.  The host pass does not know the feature and says so.
+    no_packed_f32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    common = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"--offload-arch={GPU_ARCH}", *no_packed_f32, "-I" + str(CSRC), "-I" + str(rocm / "include")]
     kernel_flags = common + ["-fno-math-errno", "-ffp-contract=fast", "-fno-gpu-rdc", "-munsafe-fp-atomics", "-Wno-unused-result"]
     torch_flags = common + [
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DHIPBLAS_V2", "-DTORCH_EXTENSION_NAME=_C",
