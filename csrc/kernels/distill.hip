@@ -1,0 +1,460 @@
+// Distillation from a teacher's top logits for gfx950: loss and logits gradient of a student's row against K stored
+// (class, logit) pairs of a teacher, mixed with the cross-entropy of a hard label.
+//
+// No counterpart in the reference, whose only criterion is nn.CrossEntropyLoss (reference min_DDP.py:75,100); it stands
+// beside the fused cross-entropy of softmax_xent.hip.  Per row, with z the C student logits and t the K teacher logits:
+//   p_k  = softmax(t / tau) over the K entries that are there (id in [0, C), t > -inf)
+//   q    = softmax(z / tau),  q1 = softmax(z)                                     over the C classes
+//   loss = (1 - a) tau^2 sum_k p_k (log p_k - log q[id_k])  -  a log q1[y]
+//   dz_j = w { (1 - a) tau ( q_j - sum_{k: id_k = j} p_k )  +  a ( q1_j - [j = y] ) },   w = upstream gradient / #rows
+//
+// One workgroup per row.  The row is read once: every thread keeps its 16-byte vectors packed in registers through the
+// maximum, the two sums of exponentials and the gradient, so a fused call moves exactly one read and one write of the
+// logits (rows too wide for the registers are read again, out of L2 / Infinity Cache).  With one temperature in play (tau = 1, a = 0 or a = 1) there is one
+// exponential per element and pass, otherwise two (DUAL).
+// The K teacher entries are a scatter into the row.  A vector that is about to be stored has to know its entries: LDS
+// holds one bit per vector (a wave's 64 vectors are one 64-bit word, so most waves skip the look-up on a scalar
+// branch) and a chained hash from vector to entries.  Entries of one class are summed beforehand in index order by the
+// first of them, which makes the result independent of the order in which the chains were built.
+// Rows need no alignment: element j of a row sits in vector (j + shift) / V of the 16-byte grid, the vectors at both ends are stored
+// element by element.
+#include <type_traits>
+
+#include "device_utils.h"
+#include "kernels.h"
+
+namespace dpa {
+namespace kernels {
+
+namespace {
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNone = 0x7fffffff;
+enum Mode : int { kForward = 0, kBackward = 1, kFused = 2 };
+
+// Sum / maximum over the threads of a workgroup, in a fixed order.
+template <int NW>
+__device__ __forceinline__ float sum_of_waves(const float* s) {
+  float v = s[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) v += s[w];
+  return v;
+}
+
+__device__ __forceinline__ float teacher_at(const DistillArgs& a, long long i) {
+  if (a.teacher_dtype == kF32) return static_cast<const float*>(a.teacher)[i];
+  const u16 raw = static_cast<const u16*>(a.teacher)[i];
+  return a.teacher_dtype == kBF16 ? BF16::to_f32(raw) : F16::to_f32(raw);
+}
+
+// THREADS x KEEP 16-byte vectors are held in registers (KEEP = 0: none, every pass reads memory).
+template <typename TR, int THREADS, int KEEP, int MODE, bool DUAL, int WAVES_PER_SIMD>
+__global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(DistillArgs a) {
+  using T = typename TR::T;
+  constexpr int V = TR::kVec, NW = THREADS / 64;
+  constexpr bool GRAD = MODE != kForward;
+  static_assert(KEEP == 0 || MODE != kBackward, "the backward reads every vector once");
+  extern __shared__ int s_dyn[];  // ids[K] | p[K] | x[K] | next[K] | head[hash] | bits[2 * words]
+  __shared__ float s_m[NW], s_s[NW], s_s1[NW], s_teacher[2], s_xy;
+  __shared__ int s_arg[NW], s_best;
+  int* const s_id = s_dyn;
+  float* const s_p = reinterpret_cast<float*>(s_dyn + a.K);
+  float* const s_x = s_p + a.K;
+  int* const s_next = s_dyn + 3 * a.K;
+  int* const s_head = s_next + a.K;
+  unsigned* const s_bits = reinterpret_cast<unsigned*>(s_head + a.hash);
+
+  const long long r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int C = static_cast<int>(a.C), ld = static_cast<int>(a.ld);
+  const T* row = static_cast<const T*>(a.logits) + r * a.ld;
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  const char* grid_in = reinterpret_cast<const char*>(row) - shift * sizeof(T);                       // the row's first 16-byte vector
+  char* grid_out = GRAD ? reinterpret_cast<char*>(static_cast<T*>(a.dlogits) + r * a.ld - shift) : nullptr;  // same alignment (checked by the host)
+  const int nvec = (shift + C + V - 1) / V, nvec_ld = (shift + ld + V - 1) / V;
+  const long long target = a.targets ? a.targets[r] : -1;
+  const bool ignored = a.targets && (target == a.ignore_index || target < 0 || target >= C);
+
+  auto store_vec = [&](int k, const float (&d)[V]) {
+    const int j0 = k * V - shift;
+    T* out = reinterpret_cast<T*>(grid_out + 16u * static_cast<unsigned>(k));
+    if (j0 >= 0 && j0 + V <= ld) {
+      store_from_f32<TR, V, true>(out, d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j0 + j >= 0 && j0 + j < ld) out[j] = TR::from_f32(d[j]);
+    }
+  };
+  if (ignored) {
+    if (GRAD) {
+      const float z[V] = {};
+      for (int k = tid; k < nvec_ld; k += THREADS) store_vec(k, z);
+    }
+    if (MODE != kBackward && tid == 0) {
+      a.row_loss[r] = 0.f;
+      a.correct[r] = 0;
+      if (MODE == kForward)
+        for (int i = 0; i < 3; ++i) a.row_stats[3 * r + i] = 0.f;
+    }
+    return;
+  }
+
+  raw16 kept[KEEP > 0 ? KEEP : 1];
+  auto load_vec = [&](int k) { return __builtin_nontemporal_load(reinterpret_cast<const raw16*>(grid_in + 16u * static_cast<unsigned>(k))); };
+  if constexpr (KEEP > 0) {
+#pragma unroll
+    for (int q = 0; q < KEEP; ++q) {
+      const int k = tid + q * THREADS;
+      if (k < nvec) kept[q] = load_vec(k);
+    }
+  }
+  // One pass over the row's vectors: f(k, packed vector).
+  auto each_vec = [&](auto&& f) __attribute__((always_inline)) {
+    if constexpr (KEEP > 0) {
+#pragma unroll
+      for (int q = 0; q < KEEP; ++q) {
+        const int k = tid + q * THREADS;
+        if (k < nvec) f(k, kept[q]);
+        __builtin_amdgcn_sched_barrier(0);  // one vector at a time: interleaved, the expansions of all of them would be live at once
+      }
+      // opaque between the passes, or the compiler keeps the fp32 expansions of one pass for the next and spills
+#pragma unroll
+      for (int q = 0; q < KEEP; ++q) keep_packed(kept[q]);
+    } else {
+      for (int k = tid; k < nvec; k += THREADS) {
+        raw16 v = *reinterpret_cast<const raw16*>(grid_in + 16u * static_cast<unsigned>(k));
+        f(k, v);
+      }
+    }
+  };
+
+  // ---- the teacher's entries: ids, scaled logits, the student's logits at those classes
+  if (GRAD) {
+    for (int i = tid; i < a.hash; i += THREADS) s_head[i] = -1;
+    for (int i = tid; i < a.words * 2; i += THREADS) s_bits[i] = 0u;
+  }
+  for (int k = tid; k < a.K; k += THREADS) {
+    const long long at = r * a.K + k;
+    const long long id = a.ids_64 ? static_cast<const long long*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
+    const bool in = id >= 0 && id < C;
+    const float t = in ? teacher_at(a, at) * a.inv_tau : kNegInf;
+    const bool there = in && t != kNegInf && a.soft_weight != 0.f;  // without a soft term the teacher's values do not matter at all
+    s_id[k] = there ? static_cast<int>(id) : -1;
+    s_p[k] = t;
+    if (MODE != kBackward) s_x[k] = there ? TR::to_f32(row[id]) : 0.f;
+  }
+  if (MODE != kBackward && tid == 0) s_xy = a.targets ? TR::to_f32(row[target]) : 0.f;
+  __syncthreads();
+  if (GRAD) {
+    for (int k = tid; k < a.K; k += THREADS) {
+      const int id = s_id[k];
+      if (id < 0) continue;
+      const int vec = (id + shift) / V;
+      s_next[k] = atomicExch(&s_head[vec & (a.hash - 1)], k);
+      atomicOr(&s_bits[vec >> 5], 1u << (vec & 31));
+    }
+  }
+
+  // ---- row maximum (lowest index among equals)
+  float m, ls, ls1 = 0.f;
+  if (MODE == kBackward) {
+    m = a.row_stats[3 * r];
+    ls = a.row_stats[3 * r + 1];
+    ls1 = a.row_stats[3 * r + 2];
+  } else {
+    m = kNegInf;
+    int arg = kNone;
+    each_vec([&](int k, const raw16& v) __attribute__((always_inline)) {
+      float x[V];
+      raw_to_f32<TR, V>(v, x);
+      const int j0 = k * V - shift;
+      if (j0 >= 0 && j0 + V <= C) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (x[j] > m) { m = x[j]; arg = j0 + j; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j0 + j >= 0 && j0 + j < C && x[j] > m) { m = x[j]; arg = j0 + j; }
+      }
+    });
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float om = __shfl_xor(m, off, 64);
+      const int oa = __shfl_xor(arg, off, 64);
+      if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
+    }
+    if (lane == 0) { s_m[wid] = m; s_arg[wid] = arg; }
+    __syncthreads();
+    m = s_m[0];
+    arg = s_arg[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w)
+      if (s_m[w] > m || (s_m[w] == m && s_arg[w] < arg)) { m = s_m[w]; arg = s_arg[w]; }
+    if (tid == 0) s_best = arg;  // read by the same thread only
+
+    // ---- sums of exponentials at both temperatures
+    float s = 0.f, s1 = 0.f;
+    const float c = a.exp_scale;
+    each_vec([&](int k, const raw16& v) __attribute__((always_inline)) {
+      float x[V];
+      raw_to_f32<TR, V>(v, x);
+      const int j0 = k * V - shift;
+      const bool full = j0 >= 0 && j0 + V <= C;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const bool in = full || (j0 + j >= 0 && j0 + j < C);
+        s += in ? __builtin_amdgcn_exp2f((x[j] - m) * c) : 0.f;
+        if (DUAL) s1 += in ? __builtin_amdgcn_exp2f((x[j] - m) * kLog2e) : 0.f;
+      }
+    });
+    s = wave_sum(s);
+    if (DUAL) s1 = wave_sum(s1);
+    if (lane == 0) { s_s[wid] = s; s_s1[wid] = s1; }
+  }
+  if (MODE == kBackward) __syncthreads();  // the chains are complete
+
+  // ---- one wave turns the teacher's logits into probabilities
+  if (wid == 0) {
+    float tm = kNegInf;
+    int best = kNone;  // first entry with the largest logit
+    for (int k = lane; k < a.K; k += 64)
+      if (s_id[k] >= 0 && !(s_p[k] <= tm)) { tm = s_p[k]; best = k; }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float om = __shfl_xor(tm, off, 64);
+      const int ob = __shfl_xor(best, off, 64);
+      if (om > tm || (om == tm && ob < best)) { tm = om; best = ob; }
+    }
+    const bool some = best != kNone;
+    float z = 0.f;
+    for (int k = lane; k < a.K; k += 64)
+      if (s_id[k] >= 0) z += __builtin_amdgcn_exp2f((s_p[k] - tm) * kLog2e);
+    z = wave_sum(z);
+    const float log_z = logf(z), inv_z = 1.f / z;
+    float b = 0.f;  // sum_k p_k (log p_k - (x_k - m) / tau); with log(sum) added it is the divergence
+    for (int k = lane; k < a.K; k += 64) {
+      if (s_id[k] < 0) continue;
+      const float t = s_p[k] - tm;
+      const float p = __builtin_amdgcn_exp2f(t * kLog2e) * inv_z;
+      if (MODE != kBackward && !(p == 0.f)) b += p * ((t - log_z) - (s_x[k] - m) * a.inv_tau);
+      s_p[k] = p;
+    }
+    b = wave_sum(b);
+    if (GRAD) {
+      // p summed over the entries of one class, kept by the first of them: s_x[k]
+      for (int k = lane; k < a.K; k += 64) {
+        const int id = s_id[k];
+        if (id < 0) continue;
+        bool first = true, alone = true;
+        for (int e = s_head[((id + shift) / V) & (a.hash - 1)]; e >= 0; e = s_next[e])
+          if (e != k && s_id[e] == id) {
+            alone = false;
+            first = first && k < e;
+          }
+        float p = s_p[k];
+        if (!alone && first)
+          for (int e = k + 1; e < a.K; ++e) p += s_id[e] == id ? s_p[e] : 0.f;
+        s_x[k] = first ? p : 0.f;
+      }
+    }
+    if (lane == 0) {
+      s_teacher[0] = some ? 1.f : 0.f;
+      s_teacher[1] = b;
+      if (MODE != kBackward && !a.targets && some) s_best = s_best == s_id[best] ? 1 : 0;  // (agreement with the teacher's first choice)
+      else if (MODE != kBackward) s_best = a.targets && s_best == target ? 1 : 0;
+    }
+  }
+  __syncthreads();
+  const bool some = s_teacher[0] != 0.f;
+  if (MODE != kBackward) {
+    ls = logf(sum_of_waves<NW>(s_s));
+    if (DUAL) ls1 = logf(sum_of_waves<NW>(s_s1));
+    if (tid == 0) {
+      const float soft = some && a.soft_weight != 0.f ? (s_teacher[1] + ls) * a.tau * a.tau * a.soft_weight : 0.f;
+      const float hard = a.hard_weight != 0.f ? ((m - s_xy) + (DUAL ? ls1 : ls)) * a.hard_weight : 0.f;
+      a.row_loss[r] = soft + hard;
+      a.correct[r] = static_cast<unsigned char>(s_best);
+      if (MODE == kForward) {
+        a.row_stats[3 * r] = m;
+        a.row_stats[3 * r + 1] = ls;
+        a.row_stats[3 * r + 2] = ls1;
+      }
+    }
+  }
+  if (!GRAD) return;
+
+  // ---- gradient
+  float w = a.scale[0];
+  if (MODE == kBackward) w *= a.grad_out[a.grad_out_rows ? r : 0];
+  const float cs = w * a.soft_weight * a.tau;       // per unit of q - p
+  const float ch = w * a.hard_weight;               // per unit of q1 - [j = y]
+  // coefficients of the exponentials: with one temperature both terms share it (tau = 1) or one of them is absent
+  const float c0 = DUAL ? (some ? cs : 0.f) : (some ? cs : 0.f) + ch;
+  const float c = a.exp_scale;
+  const int y = a.hard_weight != 0.f ? static_cast<int>(target) : -1;
+  each_vec([&](int k, const raw16& v) __attribute__((always_inline)) {
+    float x[V], d[V];
+    raw_to_f32<TR, V>(v, x);
+    const int j0 = k * V - shift;
+    const bool full = j0 >= 0 && j0 + V <= C;
+    const unsigned long long word = *reinterpret_cast<const unsigned long long*>(s_bits + 2 * (k >> 6));
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      // exp(x - m - log(sum)): the logarithm is scaled with the argument so that one multiply serves both
+      float g = c0 * __builtin_amdgcn_exp2f((x[j] - m) * c - ls * kLog2e);
+      if (DUAL) g += ch * __builtin_amdgcn_exp2f((x[j] - m) * kLog2e - ls1 * kLog2e);
+      if (j0 + j == y) g -= ch;
+      d[j] = full || (j0 + j >= 0 && j0 + j < C) ? g : 0.f;
+    }
+    if (word >> (k & 63) & 1ull) {
+      for (int e = s_head[k & (a.hash - 1)]; e >= 0; e = s_next[e]) {
+        const int at = s_id[e] - j0;
+        if (at < 0 || at >= V) continue;
+        const float p = cs * s_x[e];
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] -= j == at ? p : 0.f;
+      }
+    }
+    store_vec(k, d);
+  });
+  const float zero[V] = {};
+  for (int k = nvec + tid; k < nvec_ld; k += THREADS) store_vec(k, zero);
+}
+
+// metrics = {loss sum, correct, counted rows, loss sum / counted rows}; loss[0] = the requested reduction.  One workgroup,
+// fixed order.
+__global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* __restrict__ row_loss, const unsigned char* __restrict__ correct,
+                                                              const long long* __restrict__ targets, long long N, long long ignore_index,
+                                                              int mean, float* __restrict__ metrics, float* __restrict__ loss) {
+  __shared__ float scratch[16];
+  float l = 0.f, c = 0.f, n = 0.f;
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < N; i += 1024) {
+    l += row_loss[i];
+    c += correct[i] ? 1.f : 0.f;
+    n += !targets || targets[i] != ignore_index ? 1.f : 0.f;
+  }
+  l = block_sum<16>(l, scratch);
+  c = block_sum<16>(c, scratch);
+  n = block_sum<16>(n, scratch);
+  if (threadIdx.x == 0) {
+    metrics[0] = l;
+    metrics[1] = c;
+    metrics[2] = n;
+    metrics[3] = l / fmaxf(n, 1.f);
+    loss[0] = mean ? l / fmaxf(n, 1.f) : l;
+  }
+}
+
+// scale[0] = 1 / max(#rows that count, 1) for a mean, 1 for a sum.
+__global__ __launch_bounds__(1024) void distill_scale_kernel(const long long* __restrict__ targets, long long N, long long ignore_index, int mean,
+                                                             float* __restrict__ scale) {
+  __shared__ float scratch[16];
+  float n = 0.f;
+  if (mean && targets) {
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < N; i += 1024) n += targets[i] != ignore_index ? 1.f : 0.f;
+    n = block_sum<16>(n, scratch);
+  } else {
+    n = static_cast<float>(N);
+  }
+  if (threadIdx.x == 0) scale[0] = mean ? 1.f / fmaxf(n, 1.f) : 1.f;
+}
+
+// x *= g[0] unless g[0] is 1 (the usual loss.backward()), in which case nothing is read or written.
+template <typename TR>
+__global__ __launch_bounds__(256) void distill_apply_upstream_kernel(typename TR::T* x, long long n, const float* __restrict__ g) {
+  const float s = g[0];
+  if (s == 1.f) return;
+  constexpr int V = TR::kVec;
+  const long long nv = (reinterpret_cast<uintptr_t>(x) & 15) == 0 ? n / V : 0, step = static_cast<long long>(gridDim.x) * 256;
+  const long long first = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  for (long long i = first; i < nv; i += step) {
+    float v[V];
+    load_as_f32<TR, V>(x + i * V, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] *= s;
+    store_from_f32<TR, V>(x + i * V, v);
+  }
+  for (long long i = nv * V + first; i < n; i += step) x[i] = TR::from_f32(TR::to_f32(x[i]) * s);
+}
+
+}  // namespace
+
+bool distill_supported(long long C, long long ld, long long K) {
+  return C >= 1 && C <= ld && ld < (1ll << 28) && K >= 1 && K <= kDistillMaxEntries;
+}
+
+void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t stream) {
+  if (args.N <= 0) return;
+  DistillArgs a = args;
+  const bool dual = a.tau != 1.f && a.soft_weight != 0.f && a.hard_weight != 0.f;
+  // one exponential: at the temperature of the term that is there (tau = 1: of both)
+  a.exp_scale = (a.soft_weight != 0.f ? a.inv_tau : 1.f) * kLog2e;
+  a.hash = 64;
+  while (a.hash < a.K) a.hash *= 2;
+  dispatch_dtype(dtype, [&](auto tr) {
+    using TR = decltype(tr);
+    constexpr int V = TR::kVec;
+    const long long nvec = (a.ld + 2 * V - 2) / V;  // worst alignment
+    a.words = static_cast<int>((nvec + 63) / 64);
+    const size_t lds = (static_cast<size_t>(4) * a.K + a.hash + 2 * static_cast<size_t>(a.words)) * 4;
+    const dim3 grid(static_cast<unsigned>(a.N));
+    auto go = [&](auto threads_c, auto keep_c, auto mode_c, auto waves_c) {
+      constexpr int THREADS = decltype(threads_c)::value, KEEP = decltype(keep_c)::value, MODE = decltype(mode_c)::value;
+      constexpr int WAVES = decltype(waves_c)::value;
+      if (dual) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, true, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, false, WAVES>), grid, dim3(THREADS), lds, stream, a);
+    };
+    using std::integral_constant;
+    auto by_size = [&](auto mode_c) {
+      constexpr int MODE = decltype(mode_c)::value;
+      constexpr integral_constant<int, MODE> m{};
+      constexpr integral_constant<int, 4> w4{};
+      constexpr integral_constant<int, 8> w8{};
+      constexpr integral_constant<int, 64> t64{};
+      constexpr integral_constant<int, 256> t256{};
+      constexpr integral_constant<int, 1024> t1024{};
+      constexpr integral_constant<int, 0> none{};
+      if constexpr (MODE == kBackward) {
+        if (nvec <= 64 * 4) go(t64, none, m, w4);
+        else if (nvec <= 256 * 7) go(t256, none, m, w4);
+        else go(t1024, none, m, w8);
+      } else {
+        if (nvec <= 64 * 4) go(t64, integral_constant<int, 4>{}, m, w4);
+        else if (nvec <= 256 * 7) go(t256, integral_constant<int, 7>{}, m, w4);
+        else if (nvec <= 1024 * 7) go(t1024, integral_constant<int, 7>{}, m, w8);
+        else if (nvec <= 1024 * 16) go(t1024, integral_constant<int, 16>{}, m, w4);
+        else go(t1024, none, m, w8);
+      }
+    };
+    if (mode == kForward) by_size(integral_constant<int, kForward>{});
+    else if (mode == kBackward) by_size(integral_constant<int, kBackward>{});
+    else by_size(integral_constant<int, kFused>{});
+  });
+}
+
+void launch_distill_scale(const long long* targets, long long N, long long ignore_index, int mean, float* scale, hipStream_t stream) {
+  hipLaunchKernelGGL(distill_scale_kernel, dim3(1), dim3(1024), 0, stream, targets, N, ignore_index, mean, scale);
+}
+
+void launch_distill_reduce(const float* row_loss, const unsigned char* correct, const long long* targets, long long N, long long ignore_index,
+                           int mean, float* metrics, float* loss, hipStream_t stream) {
+  hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, stream, row_loss, correct, targets, N, ignore_index, mean, metrics, loss);
+}
+
+void launch_distill_apply_upstream(void* x, int dtype, long long n, const float* g, hipStream_t stream) {
+  if (n <= 0) return;
+  dispatch_dtype(dtype, [&](auto tr) {
+    using TR = decltype(tr);
+    const long long blocks = (n / TR::kVec + 255) / 256;
+    hipLaunchKernelGGL((distill_apply_upstream_kernel<TR>), dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 2048 ? 2048 : blocks)), dim3(256), 0,
+                       stream, static_cast<typename TR::T*>(x), n, g);
+  });
+}
+
+}  // namespace kernels
+}  // namespace dpa

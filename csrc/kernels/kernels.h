@@ -93,6 +93,44 @@ void launch_xent_fused(void* logits, int dtype, const long long* targets, long l
                        long long ld, long long ignore_index, int mean, float* grad_scale,
                        float* row_loss, unsigned char* correct, hipStream_t stream);
 
+// ------------------------------------------------------------------ distillation from a teacher's top logits
+// logits [N, ld] (first C columns are classes); ids [N, K] int64 / int32 and teacher [N, K] fp32 / bf16 / fp16: the teacher's
+// entries, an id outside [0, C) or a logit of -inf means "no entry".  targets [N] int64 or nullptr (then every row counts).
+//   row loss = soft_weight tau^2 KL(p || softmax(z / tau)) + hard_weight CE(z, target), 0 for ignored rows
+// mode 0: row losses, correct flags, row_stats[3 r ..] = {max z, log sum at tau, log sum at 1} (dual) | {max, log sum, 0}
+// mode 1: dlogits from row_stats, scaled by scale[0] * grad_out[grad_out_rows ? r : 0]
+// mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits
+// dlogits [N, ld]: columns [C, ld) are written as zero; its address must equal that of logits modulo 16.
+constexpr int kDistillMaxEntries = 1024;
+struct DistillArgs {
+  const void* logits;
+  void* dlogits;
+  const void* ids;
+  const void* teacher;
+  const long long* targets;
+  long long N, C, ld, ignore_index;
+  int K, ids_64, teacher_dtype;
+  float tau, inv_tau, soft_weight, hard_weight;
+  float* row_loss;
+  float* row_stats;
+  unsigned char* correct;
+  const float* scale;
+  const float* grad_out;
+  int grad_out_rows;
+  // set by the launcher
+  float exp_scale;
+  int hash, words;
+};
+bool distill_supported(long long C, long long ld, long long K);
+void launch_distill(const DistillArgs& a, int dtype, int mode, hipStream_t stream);
+// scale[0] = 1 / max(#targets != ignore_index, 1) for a mean (N rows without targets), 1 for a sum.
+void launch_distill_scale(const long long* targets, long long N, long long ignore_index, int mean, float* scale, hipStream_t stream);
+// metrics[0] = sum of row losses, [1] = correct rows, [2] = rows that count, [3] = mean; loss[0] = mean or sum.
+void launch_distill_reduce(const float* row_loss, const unsigned char* correct, const long long* targets, long long N, long long ignore_index,
+                           int mean, float* metrics, float* loss, hipStream_t stream);
+// x[0 .. n) *= g[0]; x is left untouched when g[0] is 1.
+void launch_distill_apply_upstream(void* x, int dtype, long long n, const float* g, hipStream_t stream);
+
 // ------------------------------------------------------------------ dense layers
 enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2 };
 

@@ -291,6 +291,105 @@ std::tuple<Tensor, Tensor> xent_fused(Tensor logits, Tensor targets, int64_t n_c
   return {correct, metrics};
 }
 
+// ------------------------------------------------------------------ distillation from a teacher's top logits
+kernels::DistillArgs distill_args(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const c10::optional<Tensor>& targets,
+                                  int64_t n_classes, int64_t ignore_index, double temperature, double hard_weight, const char* who) {
+  check_gpu(logits, "logits");
+  check_gpu(ids, "teacher_ids");
+  check_gpu(teacher, "teacher_logits");
+  TORCH_CHECK(logits.dim() == 2, who, ": logits must be [N, C]");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16 == 0, who, ": logits must start on a 16-byte boundary");
+  const int64_t N = logits.size(0), ld = logits.size(1);
+  const int64_t C = n_classes > 0 ? n_classes : ld;
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == N && ids.sizes() == teacher.sizes(), who, ": teacher_ids and teacher_logits must both be [N, K]");
+  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, who, ": teacher_ids must be int64 or int32");
+  TORCH_CHECK(ids.get_device() == logits.get_device() && teacher.get_device() == logits.get_device(), who, ": tensors on different devices");
+  TORCH_CHECK(kernels::distill_supported(C, ld, ids.size(1)), who, ": needs 1 <= n_classes <= width and 1 .. ", kernels::kDistillMaxEntries,
+              " teacher entries (got ", C, ", ", ld, ", ", ids.size(1), ")");
+  TORCH_CHECK(N < (1ll << 31), who, ": too many rows");
+  TORCH_CHECK(temperature > 0.0 && hard_weight >= 0.0 && hard_weight <= 1.0, who, ": needs temperature > 0 and 0 <= hard_weight <= 1");
+  kernels::DistillArgs a{};
+  if (targets.has_value() && targets->defined()) {
+    check_gpu(*targets, "targets");
+    TORCH_CHECK(targets->dim() == 1 && targets->size(0) == N && targets->scalar_type() == at::kLong && targets->get_device() == logits.get_device(),
+                who, ": targets must be int64 [N] on the logits' device");
+    a.targets = reinterpret_cast<const long long*>(targets->data_ptr<int64_t>());
+  }
+  TORCH_CHECK(a.targets != nullptr || hard_weight == 0.0, who, ": a hard term needs targets");
+  a.logits = logits.data_ptr();
+  a.ids = ids.data_ptr();
+  a.teacher = teacher.data_ptr();
+  a.N = N; a.C = C; a.ld = ld; a.ignore_index = ignore_index;
+  a.K = static_cast<int>(ids.size(1));
+  a.ids_64 = ids.scalar_type() == at::kLong;
+  a.teacher_dtype = kdtype(teacher);
+  a.tau = static_cast<float>(temperature);
+  a.inv_tau = static_cast<float>(1.0 / temperature);
+  a.soft_weight = static_cast<float>(1.0 - hard_weight);
+  a.hard_weight = static_cast<float>(hard_weight);
+  return a;
+}
+
+// Returns (loss [], row_loss [N], correct [N], metrics [4], scale [1], row_stats [N, 3] or undefined, dlogits or undefined).
+// gradient: "none" (row_stats are kept for distill_backward), "new" (dlogits for a unit upstream gradient in a fresh
+// tensor) or "inplace" (the same, over the logits).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> distill_forward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets,
+                                                                                   int64_t n_classes, int64_t ignore_index, double temperature,
+                                                                                   double hard_weight, bool mean, const std::string& gradient) {
+  TORCH_CHECK(gradient == "none" || gradient == "new" || gradient == "inplace", "distill_forward: gradient must be none, new or inplace");
+  kernels::DistillArgs a = distill_args(logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, "distill_forward");
+  DevGuard g(logits);
+  hipStream_t s = stream_of(logits);
+  auto fopt = logits.options().dtype(at::kFloat);
+  Tensor loss = at::empty({}, fopt), row_loss = at::empty({a.N}, fopt), metrics = at::empty({4}, fopt), scale = at::empty({1}, fopt), stats, dlogits;
+  Tensor correct = at::empty({a.N}, logits.options().dtype(at::kBool));
+  a.row_loss = row_loss.data_ptr<float>();
+  a.correct = reinterpret_cast<unsigned char*>(correct.data_ptr<bool>());
+  a.scale = scale.data_ptr<float>();
+  if (gradient == "none") {
+    stats = at::empty({a.N, 3}, fopt);
+    a.row_stats = stats.data_ptr<float>();
+  } else {
+    dlogits = gradient == "inplace" ? logits : at::empty_like(logits);
+    a.dlogits = dlogits.data_ptr();
+  }
+  kernels::launch_distill_scale(a.targets, a.N, ignore_index, mean ? 1 : 0, scale.data_ptr<float>(), s);
+  kernels::launch_distill(a, kdtype(logits), gradient == "none" ? 0 : 2, s);
+  kernels::launch_distill_reduce(a.row_loss, a.correct, a.targets, a.N, ignore_index, mean ? 1 : 0, metrics.data_ptr<float>(), loss.data_ptr<float>(), s);
+  return {loss, row_loss, correct, metrics, scale, stats, dlogits};
+}
+
+// dlogits from the statistics of a "none" forward.  grad_out: one value, or one per row.
+Tensor distill_backward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets, Tensor row_stats, Tensor scale, Tensor grad_out,
+                        int64_t n_classes, int64_t ignore_index, double temperature, double hard_weight) {
+  kernels::DistillArgs a = distill_args(logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, "distill_backward");
+  check_gpu(row_stats, "row_stats");
+  check_gpu(scale, "scale");
+  check_gpu(grad_out, "grad_out");
+  TORCH_CHECK(row_stats.scalar_type() == at::kFloat && row_stats.numel() == 3 * a.N && scale.scalar_type() == at::kFloat && scale.numel() == 1,
+              "distill_backward: row_stats [N, 3] and scale [1] must be float32");
+  TORCH_CHECK(grad_out.scalar_type() == at::kFloat && (grad_out.dim() <= 1) && (grad_out.numel() == 1 || grad_out.numel() == a.N),
+              "distill_backward: grad_out must be one float32 value or one per row");
+  DevGuard g(logits);
+  Tensor dlogits = at::empty_like(logits);
+  a.dlogits = dlogits.data_ptr();
+  a.row_stats = row_stats.data_ptr<float>();
+  a.scale = scale.data_ptr<float>();
+  a.grad_out = grad_out.data_ptr<float>();
+  a.grad_out_rows = grad_out.dim() == 1 ? 1 : 0;
+  kernels::launch_distill(a, kdtype(logits), 1, stream_of(logits));
+  return dlogits;
+}
+
+// x *= g (float32 scalar on the device); nothing is moved when g is 1.
+void distill_apply_upstream(Tensor x, Tensor g) {
+  check_gpu(x, "x");
+  check_gpu(g, "g");
+  TORCH_CHECK(g.scalar_type() == at::kFloat && g.numel() == 1 && g.get_device() == x.get_device(), "distill_apply_upstream: g must be a float32 scalar");
+  DevGuard guard(x);
+  kernels::launch_distill_apply_upstream(x.data_ptr(), kdtype(x), x.numel(), g.data_ptr<float>(), stream_of(x));
+}
+
 // ------------------------------------------------------------------ batch normalisation (training mode, channels last)
 // x: [R, C] (the channels-last activation flattened over batch and space).  Returns (y, mean, rstd, scale | shift).
 // running_mean / running_var are updated in place when given.
@@ -1006,6 +1105,13 @@ void init_ops(py::module_& m) {
     return kernels::gemm_bf16_split_k(a);
   }, "contraction ranges the bf16 GEMM would use for an [M,K]x[K,N] product (1 = single pass)");
   m.def("xent_fused", &xent_fused, py::arg("logits"), py::arg("targets"), py::arg("n_classes"), py::arg("ignore_index"), py::arg("mean"));
+  m.def("distill_forward", &distill_forward, py::arg("logits"), py::arg("teacher_ids"), py::arg("teacher_logits"), py::arg("targets"),
+        py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"), py::arg("hard_weight"), py::arg("mean"), py::arg("gradient") = "none");
+  m.def("distill_backward", &distill_backward, py::arg("logits"), py::arg("teacher_ids"), py::arg("teacher_logits"), py::arg("targets"),
+        py::arg("row_stats"), py::arg("scale"), py::arg("grad_out"), py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"),
+        py::arg("hard_weight"));
+  m.def("distill_apply_upstream", &distill_apply_upstream, py::arg("x"), py::arg("g"));
+  m.attr("DISTILL_MAX_ENTRIES") = kernels::kDistillMaxEntries;
   m.def("dgrad_act_backward", &dgrad_act_backward, py::arg("dout"), py::arg("weight"), py::arg("aux"), py::arg("act"), py::arg("want_colsum"));
   m.def("dgrad_act_backward_supported", &dgrad_act_backward_supported);
   m.def("attention_supported", [](int64_t T, int64_t hd, int64_t rs) { return kernels::attention_supported(T, hd, rs); });

@@ -1,0 +1,398 @@
+"""Distillation from a teacher's top logits: loss, by-products and gradients against float64, refusals, streams, graphs."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from distributed_pytorch_amd.ops import TopKDistillation, projection_topk_distillation, topk_distillation
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+NEG = float("-inf")
+
+
+def make(N, C, K, dtype=torch.float32, device="cpu", width=None, seed=0, pad_rows=True):
+    """Logits [N, width], K distinct entries a row in no order, targets with some rows ignored."""
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn(N, width or C, generator=g) * 3 - 20).to(dtype)  # an offset, as real vocabularies have
+    ids = torch.stack([torch.randperm(C, generator=g)[:K] for _ in range(N)])
+    teacher = torch.randn(N, K, generator=g) * 2
+    targets = torch.randint(0, C, (N,), generator=g)
+    if pad_rows and N > 2:
+        targets[1] = -100
+        ids[2, K // 2:] = -1
+    return logits.to(device), ids.to(device), teacher.to(device), targets.to(device)
+
+
+def reference(logits, ids, teacher, targets, tau=1.0, a=0.0, C=None, ignore_index=-100):
+    """Row losses and mean-loss gradient in float64, entry by entry from the definition."""
+    C = C or logits.shape[1]
+    N = logits.shape[0]
+    z = logits.detach().double().cpu()
+    out, grad = torch.zeros(N, dtype=torch.float64), torch.zeros_like(z)
+    live = [targets is None or 0 <= int(targets[r]) < C for r in range(N)]
+    n = max(1, N if targets is None else int((targets != ignore_index).sum()))
+    for r in range(N):
+        if not live[r]:
+            grad[r] = 0
+            continue
+        x = z[r, :C]
+        q, q1 = torch.softmax(x / tau, 0), torch.softmax(x, 0)
+        there = [(int(i), float(t)) for i, t in zip(ids[r].cpu(), teacher[r].double().cpu()) if 0 <= int(i) < C and float(t) != NEG]
+        if there and a < 1:
+            p = torch.softmax(torch.tensor([t for _, t in there], dtype=torch.float64) / tau, 0)
+            log_q = torch.log_softmax(x / tau, 0)
+            out[r] += (1 - a) * tau ** 2 * sum(float(pk * (pk.log() - log_q[i])) for (i, _), pk in zip(there, p) if pk > 0)
+            grad[r, :C] += (1 - a) * tau * q
+            for (i, _), pk in zip(there, p):
+                grad[r, i] -= (1 - a) * tau * pk
+        if a > 0:
+            y = int(targets[r])
+            out[r] -= a * float(torch.log_softmax(x, 0)[y])
+            grad[r, :C] += a * q1
+            grad[r, y] -= a
+    return out, grad, n
+
+
+def check(logits, ids, teacher, targets, tau, a, C=None, seed_grad=None):
+    C = C or logits.shape[1]
+    x = logits.detach().clone().requires_grad_()
+    r = topk_distillation(x, ids, teacher, targets, tau, a, n_classes=C)
+    rows, grad, n = reference(logits, ids, teacher, targets, tau, a, C)
+    # float32 arithmetic: an exponent off by 2^-23 of its size (below 64 here), sums of positive terms, a few roundings
+    near = 64 * 2.0 ** -23
+    size = max(1.0, tau ** 2) * (1 + float(rows.abs().max()) / max(1.0, tau ** 2))
+    assert abs(float(r.loss.detach()) - float(rows.sum() / n)) <= near * size
+    up = 1.0
+    if seed_grad is not None:
+        up = seed_grad
+    (r.loss * up).backward()
+    half = torch.finfo(logits.dtype).eps / 2
+    atol = near * max(tau, 1.0) * up / n + (2.0 ** -25 if logits.dtype == torch.float16 else 0.0)
+    rtol = half * (1.01 if up == 1.0 else 2.02)  # another upstream gradient: rounded once more
+    torch.testing.assert_close(x.grad.double().cpu(), grad * up / n, rtol=rtol, atol=atol)
+    assert torch.equal(x.grad[:, C:], torch.zeros_like(x.grad[:, C:]))
+    m = r.metrics.cpu()
+    live = torch.ones(len(rows), dtype=torch.bool) if targets is None else (targets.cpu() != -100)
+    best = logits[:, :C].float().argmax(1).cpu()
+    # equal maxima: the lowest index
+    best = torch.tensor([int((logits[i, :C] == logits[i, b]).nonzero()[0]) if live[i] else -1 for i, b in enumerate(best.tolist())])
+    if targets is not None:
+        assert torch.equal(r.correct.cpu(), (best == targets.cpu()) & live)
+    assert m[1] == r.correct.sum().cpu() and m[2] == live.sum()
+    return x.grad
+
+
+# ------------------------------------------------------------------------------------------------ CPU
+@pytest.mark.parametrize("tau,a", [(1.0, 0.0), (2.0, 0.5), (0.5, 1.0), (4.0, 0.1)])
+def test_composed_matches_the_definition(tau, a):
+    logits, ids, teacher, targets = make(6, 40, 7)
+    check(logits, ids, teacher, targets, tau, a, C=37)
+
+
+def test_composed_gradient_against_differences():
+    logits, ids, teacher, targets = make(5, 23, 6, dtype=torch.float64)
+    f = lambda z: topk_distillation(z, ids, teacher.double(), targets, 3.0, 0.3, n_classes=20).loss  # noqa: E731
+    ids.clamp_(max=19)
+    targets.clamp_(max=19)
+    assert torch.autograd.gradcheck(f, logits.requires_grad_())
+
+
+def test_rows_that_count_for_nothing():
+    logits, ids, teacher, targets = make(4, 11, 3)
+    logits[1] = float("nan")          # ignored row
+    ids[2] = -1                       # no entries: the soft term is 0
+    teacher[3] = NEG
+    x = logits.requires_grad_()
+    r = topk_distillation(x, ids, teacher, targets, 2.0, 0.0, reduction="none")
+    assert r.loss.tolist()[1:] == [0.0, 0.0, 0.0] and r.loss[0] > 0
+    r.loss.sum().backward()
+    assert torch.equal(x.grad[1:], torch.zeros(3, 11)) and bool(x.grad[0].abs().sum() > 0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals(device):
+    logits, ids, teacher, targets = make(4, 11, 3, device=device)
+    bad = [
+        (dict(temperature=0.0), ValueError), (dict(temperature=-1.0), ValueError), (dict(temperature=float("nan")), ValueError),
+        (dict(temperature=float("inf")), ValueError), (dict(hard_weight=1.5, targets=targets), ValueError), (dict(hard_weight=0.5), ValueError),
+        (dict(reduction="avg"), ValueError), (dict(n_classes=12), ValueError), (dict(n_classes=0), ValueError),
+        (dict(targets=targets[:3]), ValueError), (dict(targets=targets.int()), ValueError),
+        (dict(targets=targets.clamp(min=0) + 11, check_targets=True), IndexError),
+    ]
+    for kw, err in bad:
+        with pytest.raises(err):
+            topk_distillation(logits, ids, teacher, **kw)
+    with pytest.raises(ValueError):
+        topk_distillation(logits, ids[:3], teacher[:3])
+    with pytest.raises(ValueError):
+        topk_distillation(logits, ids, teacher[:, :2])
+    with pytest.raises(ValueError):
+        topk_distillation(logits, ids[:, :0], teacher[:, :0])
+    with pytest.raises(ValueError):
+        topk_distillation(logits, ids.float(), teacher)
+    with pytest.raises(ValueError):
+        topk_distillation(logits, ids, teacher.long())
+    with pytest.raises(ValueError):
+        topk_distillation(logits.reshape(2, 2, 11), ids, teacher)
+    with pytest.raises(IndexError):
+        topk_distillation(logits, ids + 11, teacher, check_targets=True)
+    w = torch.randn(11, 8, device=device)
+    with pytest.raises(ValueError):
+        projection_topk_distillation(torch.randn(4, 8, device=device), w, ids, teacher, reduction="none")
+
+
+def test_module_and_projection_on_the_cpu():
+    logits, ids, teacher, targets = make(6, 30, 4)
+    crit = TopKDistillation(2.0, 0.25)
+    loss = crit(logits.view(2, 3, 30), ids.view(2, 3, 4), teacher.view(2, 3, 4), targets.view(2, 3))
+    rows, _, n = reference(logits, ids, teacher, targets, 2.0, 0.25)
+    assert abs(float(loss) - float(rows.sum() / n)) < 1e-4 and crit.last_metrics[2] == n and crit.last_correct.shape == (6,)
+    w = torch.randn(30, 5, requires_grad=True)
+    x = torch.randn(2, 3, 5, requires_grad=True)
+    r = projection_topk_distillation(x, w, ids.view(2, 3, 4), teacher.view(2, 3, 4), targets.view(2, 3), 2.0, 0.25)
+    s = topk_distillation(F.linear(x, w).view(6, 30), ids, teacher, targets, 2.0, 0.25)
+    assert torch.equal(r.loss, s.loss)
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+# widths on both sides of every kernel's limit, odd ones (rows that start anywhere), one class
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("C,K", [(1, 1), (7, 3), (64, 5), (1000, 64), (1003, 64), (2041, 9), (2049, 100), (4099, 33), (7170, 64), (14343, 65),
+                                 (50257, 64), (57345, 7), (65543, 128), (131083, 1024)])
+def test_against_float64(C, K, dtype):
+    logits, ids, teacher, targets = make(5, C, K, dtype, DEV, seed=C)
+    check(logits, ids, teacher, targets, 2.0, 0.25)
+    check(logits, ids, teacher, None, 1.0, 0.0)
+
+
+@gpu
+@pytest.mark.parametrize("tau,a", [(1.0, 0.0), (1.0, 0.5), (1.0, 1.0), (3.0, 0.0), (3.0, 1.0), (0.25, 0.5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_weights_and_temperatures(tau, a, dtype):
+    logits, ids, teacher, targets = make(7, 5000, 17, dtype, DEV)
+    check(logits, ids, teacher, targets, tau, a)
+    check(logits, ids, teacher, targets, tau, a, seed_grad=0.375)
+
+
+@gpu
+@pytest.mark.parametrize("C,width", [(50257, 50304), (1000, 1024), (1001, 1021)])
+def test_padding_columns_may_hold_anything(C, width):
+    logits, ids, teacher, targets = make(6, C, 12, torch.bfloat16, DEV, width=width)
+    logits[0, C:] = float("nan")
+    logits[3, C:] = float("inf")
+    logits[4, C:] = 100.0
+    check(logits, ids, teacher, targets, 2.0, 0.5, C=C)
+
+
+@gpu
+def test_rows_without_entries_and_ignored_rows():
+    logits, ids, teacher, targets = make(8, 999, 10, torch.float32, DEV)
+    logits[1] = float("nan")           # targets[1] is ignore_index
+    ids[0] = -1
+    teacher[3] = NEG
+    ids[4, ::2] = 999                  # beyond the classes: absent
+    teacher[4, ::2] = float("nan")     # the value of an absent entry does not matter
+    teacher[5, 1:] = NEG
+    targets[6] = 5000                  # out of range: like an ignored row, but counted
+    check(logits, ids, teacher, targets, 2.0, 0.5)
+    check(logits, ids, teacher, targets, 2.0, 0.0)
+    targets.fill_(-100)                # nothing counts: loss 0, no gradient
+    logits.fill_(float("nan"))
+    x = logits.requires_grad_()
+    r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5)
+    r.loss.backward()
+    assert float(r.loss) == 0.0 and torch.equal(x.grad, torch.zeros_like(x.grad)) and r.metrics.tolist() == [0, 0, 0, 0]
+
+
+@gpu
+def test_non_finite_values_stay_in_their_row():
+    logits, ids, teacher, targets = make(4, 700, 5, torch.float32, DEV, pad_rows=False)
+    logits[1, 3] = float("nan")
+    teacher[2, 0] = float("nan")
+    logits[3, 5:300] = NEG             # masked classes of a row that is fine otherwise
+    ids[3] = torch.tensor([0, 1, 2, 300, 301], device=DEV)
+    targets[3] = 400
+    x = logits.clone().requires_grad_()
+    r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5, reduction="none")
+    r.loss[[0, 3]].sum().backward()
+    rows, grad, _ = reference(logits[[0, 3]], ids[[0, 3]], teacher[[0, 3]], targets[[0, 3]], 2.0, 0.5)
+    assert torch.isnan(r.loss[1]) and torch.isnan(r.loss[2])
+    torch.testing.assert_close(r.loss[[0, 3]].double().cpu(), rows, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(x.grad[[0, 3]].double().cpu(), grad, rtol=1e-6, atol=2e-5)
+
+
+@gpu
+@pytest.mark.parametrize("C", [9, 3000, 60001])
+def test_entries_of_one_class_add_up(C):
+    logits, ids, teacher, targets = make(4, C, 9, torch.float32, DEV, pad_rows=False)
+    ids[0] = 8 if C > 9 else 3                     # all of them
+    ids[1, ::2] = ids[1, 0].item()
+    ids[2] = torch.tensor([0, 1, 2, 3, 0, 1, 2, 3, 4], device=DEV)  # neighbours in one vector
+    a = check(logits, ids, teacher, targets, 2.0, 0.5)
+    for _ in range(3):
+        assert torch.equal(a, check(logits, ids, teacher, targets, 2.0, 0.5))
+    many = torch.randint(0, min(C, 40), (4, 1024), device=DEV)
+    t = torch.randn(4, 1024, device=DEV)
+    b = check(logits, many, t, targets, 1.5, 0.0)
+    assert torch.equal(b, check(logits, many, t, targets, 1.5, 0.0))
+
+
+@gpu
+def test_equal_maxima_count_for_the_lowest_class():
+    logits = torch.zeros(3, 5001, device=DEV, dtype=torch.bfloat16)
+    logits[1, 17] = logits[1, 4000] = 3.0
+    ids = torch.tensor([[0, 1], [4000, 17], [7, 0]], device=DEV)
+    teacher = torch.zeros(3, 2, device=DEV)
+    targets = torch.tensor([0, 17, 1], device=DEV)
+    assert topk_distillation(logits, ids, teacher, targets).correct.tolist() == [True, True, False]
+    assert topk_distillation(logits, ids, teacher).correct.tolist() == [True, False, False]
+
+
+@gpu
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("t_dtype", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+def test_types_and_strides_of_the_teacher(ids_dtype, t_dtype):
+    logits, ids, teacher, targets = make(6, 3001, 20, torch.bfloat16, DEV)
+    ids = ids.to(ids_dtype).t().contiguous().t()
+    check(logits, ids, teacher.to(t_dtype).t().contiguous().t(), targets, 2.0, 0.5)
+
+
+@gpu
+def test_logits_of_any_stride_and_offset():
+    base, ids, teacher, targets = make(6, 3001, 20, torch.bfloat16, DEV)
+    flat = torch.empty(6 * 3001 + 3, dtype=base.dtype, device=DEV)
+    flat[3:] = base.reshape(-1)
+    want = check(base, ids, teacher, targets, 2.0, 0.5)
+    for view in (flat[3:].view(6, 3001), base.t().contiguous().t(), torch.cat([base, base], 1)[:, :3001]):
+        x = view.detach().requires_grad_()
+        topk_distillation(x, ids, teacher, targets, 2.0, 0.5).loss.backward()
+        assert torch.equal(x.grad, want)
+
+
+@gpu
+def test_reductions_and_a_second_backward():
+    logits, ids, teacher, targets = make(9, 5003, 20, torch.float32, DEV)
+    rows, grad, n = reference(logits, ids, teacher, targets, 2.0, 0.5)
+    x = logits.clone().requires_grad_()
+    up = torch.rand(9, device=DEV) + 0.5
+    r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5, reduction="none")
+    torch.testing.assert_close(r.loss.double().cpu(), rows, rtol=1e-5, atol=1e-5)
+    (g,) = torch.autograd.grad(r.loss, x, up)
+    torch.testing.assert_close(g.double().cpu(), grad * up.double().cpu().unsqueeze(1), rtol=1e-6, atol=2e-5)
+    for reduction, k in (("sum", 1), ("mean", n)):
+        r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5, reduction=reduction)
+        first = torch.autograd.grad(r.loss * 3, x, retain_graph=True)[0]
+        second = torch.autograd.grad(r.loss, x, retain_graph=True)[0]
+        third = torch.autograd.grad(r.loss, x)[0]
+        torch.testing.assert_close(first.double().cpu(), grad * 3 / k, rtol=1e-6, atol=5e-5 / k)
+        torch.testing.assert_close(second.double().cpu(), grad / k, rtol=1e-6, atol=2e-5 / k)
+        assert torch.equal(second, third)
+    with torch.no_grad():
+        quiet = topk_distillation(logits, ids, teacher, targets, 2.0, 0.5)
+    assert torch.equal(quiet.loss, r.loss.detach())
+
+
+@gpu
+def test_empty_batch_and_one_row():
+    for N in (0, 1):
+        x = torch.randn(N, 70, device=DEV, requires_grad=True)
+        r = topk_distillation(x, torch.zeros(N, 2, dtype=torch.long, device=DEV), torch.zeros(N, 2, device=DEV))
+        r.loss.backward()
+        assert x.grad.shape == (N, 70) and torch.isfinite(r.loss)
+
+
+@gpu
+@pytest.mark.parametrize("N,C,width,K_in", [(64, 1000, 1024, 96), (257, 5003, 5008, 64), (3, 131, 136, 40), (40, 70, 72, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_projection_against_float64(N, C, width, K_in, dtype):
+    _, ids, teacher, targets = make(N, C, 11, dtype, DEV)
+    x = torch.randn(N, K_in, device=DEV).to(dtype)
+    w = (torch.randn(width, K_in, device=DEV) / math.sqrt(K_in)).to(dtype)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    r = projection_topk_distillation(xs, ws, ids, teacher, targets, 2.0, 0.5, n_classes=C)
+    (r.loss * 0.5).backward()
+    half = torch.finfo(dtype).eps / 2
+    logits = (x.double() @ w.double().t())
+    rows, grad, n = reference(logits, ids, teacher, targets, 2.0, 0.5, C)
+    grad = grad.to(DEV) * 0.5 / n
+    # logits off by half a step of their own size move a row's loss by at most tau (1 - a) + a times twice that
+    zmax = float(logits.abs().max())
+    slack = half * zmax * 2 * 1.5 + 1e-4 * (1 if dtype == torch.float32 else 0) + 1e-5
+    assert abs(float(r.loss.detach()) - float(rows.sum() / n)) <= slack
+    # dlogits: the probabilities move by a factor exp(2 half zmax), and the result is rounded; then one product and two roundings
+    factor = math.expm1(2 * half * zmax) + 3 * half + 2e-5
+    z = logits[:, :C]
+    q = grad.abs() + 0.5 / n * F.pad(torch.softmax(z / 2, 1) + 0.5 * torch.softmax(z, 1), (0, width - C))  # every positive part of dlogits
+    for got, want, bound in ((xs.grad, grad @ w.double(), q @ w.double().abs()), (ws.grad, grad.t() @ x.double(), q.t() @ x.double().abs())):
+        err = (got.double() - want).abs()
+        assert bool((err <= factor * bound + half * want.abs() + 1e-9).all())
+    assert torch.equal(ws.grad[C:], torch.zeros_like(ws.grad[C:]))
+
+
+@gpu
+def test_gradient_against_differences():
+    logits, ids, teacher, targets = make(3, 900, 8, torch.float32, DEV, pad_rows=False)
+    x = logits.clone().requires_grad_()
+    topk_distillation(x, ids, teacher, targets, 3.0, 0.3).loss.backward()
+    # central differences of the float64 loss: exact to h^2
+    h = 1e-4
+    for r, j in ((0, int(ids[0, 0])), (1, int(targets[1])), (2, int(ids[2, 5])), (0, 3)):
+        at = []
+        for s in (h, -h):
+            z = logits.double()
+            z[r, j] += s
+            rows, _, n = reference(z, ids, teacher, targets, 3.0, 0.3)
+            at.append(float(rows.sum() / n))
+        assert abs((at[0] - at[1]) / (2 * h) - float(x.grad[r, j])) < 2e-6
+
+
+@gpu
+def test_other_stream_and_two_calls_at_once():
+    a = make(64, 20011, 30, torch.bfloat16, DEV, seed=1)
+    b = make(64, 20011, 30, torch.bfloat16, DEV, seed=2)
+
+    def grad(t):
+        x = t[0].detach().requires_grad_()
+        (g,) = torch.autograd.grad(topk_distillation(x, t[1], t[2], t[3], 2.0, 0.5).loss, x)
+        return g
+
+    want = [grad(a), grad(b)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            ga = grad(a)
+        with torch.cuda.stream(s2):
+            gb = grad(b)
+        torch.cuda.synchronize()
+        assert torch.equal(ga, want[0]) and torch.equal(gb, want[1])
+
+
+@gpu
+def test_captured_and_replayed():
+    logits, ids, teacher, targets = make(32, 5003, 30, torch.bfloat16, DEV)
+    x = logits.clone().requires_grad_()
+
+    def step():
+        r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5)
+        (g,) = torch.autograd.grad(r.loss, x)
+        return r.loss, g
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, g = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(logits * (1 + 0.1 * k))
+        graph.replay()
+        torch.cuda.synchronize()
+        want_loss, want_g = step()
+        assert torch.equal(loss, want_loss) and torch.equal(g, want_g)
