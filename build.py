@@ -134,7 +134,9 @@ def build_gpu(force=False, verbose=False, jobs_n=8):
     # -amdgpu-mfma-vgpr-form: the one-wave-per-SIMD forward kernel has a 512-register budget, with which the
     # compiler would give every matrix instruction an AGPR destination and copy the score accumulators to
     # ordinary registers for the softmax; the file's other kernels (256-register budget) already get this form.
-    per_file = {"attention.hip": ["-fno-honor-nans", "-fno-slp-vectorize", "-mllvm", "-amdgpu-mfma-vgpr-form"]}
+    # window_attention.hip: the same reasons.
+    attention_flags = ["-fno-honor-nans", "-fno-slp-vectorize", "-mllvm", "-amdgpu-mfma-vgpr-form"]
+    per_file = {"attention.hip": attention_flags, "window_attention.hip": attention_flags}
     objs, cmds = [], []
     draw_asm = None
     for s in kernels:

@@ -305,5 +305,31 @@ void launch_attention_bwd(const void* q, const void* k, const void* v, const voi
 // bias_partial: nullptr, or [B*T/128][3*H*64] fp32 receiving the column sums of dq | dk | dv per block
 // of 128 positions (summed over the first index they give the bias gradient of the q|k|v projection).
 
+// ------------------------------------------------------------------ causal attention with a sliding window and sinks
+// qkv: element (b, t, j) of the packed q | k | v projection at qkv[b * batch_stride + t * row_stride + j], j < (H + 2 KV) D: H query heads, KV
+// key heads, KV value heads of D = 64 or 128; 16-byte aligned, strides in multiples of 8.  o, d_o: [B, T, H, D] contiguous, dqkv:
+// [B, T, H + 2 KV, D] contiguous.  lens: [B] int32 or nullptr.  lse2 (log2 of the softmax denominators) and delta: [B, H, T] fp32; lse2 may be
+// nullptr in a forward without a backward.  window >= 1, 0 <= sinks; both at most T.
+struct WindowAttnArgs {
+  const void* qkv;
+  void* o;
+  const void* d_o;
+  void* dqkv;
+  const int* lens;
+  float* lse2;
+  float* delta;
+  float* partial;   // window_attention_partial_floats() floats
+  long long row_stride, batch_stride;
+  int B, T, H, KV, D, window, sinks;
+  float scale;      // > 0
+  int compute_units, pieces;
+  float scale_log2; // set by the launcher
+};
+bool window_attention_supported(long long B, long long T, long long H, long long KV, long long D, long long row_stride, int dtype);
+int window_attention_pieces(const WindowAttnArgs& a);  // workgroups of the dK/dV kernel: a.pieces
+long long window_attention_partial_floats(const WindowAttnArgs& a);
+void launch_window_attention_fwd(const WindowAttnArgs& a, int dtype, hipStream_t stream);
+void launch_window_attention_bwd(const WindowAttnArgs& a, int dtype, hipStream_t stream);
+
 }  // namespace kernels
 }  // namespace dpa

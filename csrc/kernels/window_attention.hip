@@ -1,0 +1,885 @@
+// Causal attention with a sliding window and sinks for gfx950, forward and backward: bf16 / fp16, head size 64 or 128,
+// key / value heads shared by groups of query heads, any sequence length, padded batches.
+//
+// Not an op of the reference (its model is two linear layers, reference min_DDP.py:41-49); it stands beside the causal
+// attention of attention.hip.  Query i of a sequence of `len` positions sees key j when
+//     j <= i  and  (i - j < window  or  j < sinks)
+//   s_ij = c q_i k_j,  p_ij = exp(s_ij - lse_i),  o_i = sum_j p_ij v_j
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i v_j - delta_i),  delta_i = do_i o_i,  dq_i = c sum_j ds_ij k_j,  dk_j = c sum_i ds_ij q_i
+// (dk, dv summed over the query heads of a group).
+//
+// Layout of the work: a workgroup is four waves of 32 rows each -- queries in the forward and dQ kernels, keys in the
+// dK/dV kernel -- and walks only the 64-row tiles of the other operand that the window or the sinks can reach; a wave
+// skips the tiles that miss its own 32 rows, and only tiles that straddle a border of the mask pay for the comparisons.  The
+// products run transposed (S^T = K Q^T), so a query's softmax statistics are scalars of its lane and the probabilities leave the
+// accumulators as the operand of the next product without changing lanes; the other operand of that product comes
+// from the row-major tile through the transposing LDS read.  Tiles travel global -> LDS by DMA through a ring, requested one or two
+// tiles ahead.  The tile image is one for both kinds of reads: 16-byte chunk c of row r sits at chunk c ^ swz(r), which
+// puts the 16 rows of a row-wise read on 16 different 16-byte bank groups and the 8 rows of a transposing read on 8
+// different 32-byte groups.
+// Rows at and beyond a sequence's length are never read: source rows are clamped to the last valid one, what they
+// would contribute is masked, and their outputs and gradients are written as zero.
+//
+// dK/dV: blocks of 128 keys cost unlike amounts -- a block with sinks meets every later query of every head of its group, the
+// others only a window of them -- so the list of (key block, head, query tile) units is cut into equal pieces, one per
+// workgroup slot of the chip.  A block inside one piece is written directly; a block that is cut leaves fp32 partial
+// sums, which a last kernel adds up in order: no atomics, the same result every time.
+#include <type_traits>
+
+#include "device_utils.h"
+#include "kernels.h"
+
+namespace dpa {
+namespace kernels {
+
+namespace {
+
+constexpr int kRows = 128;     // rows per workgroup
+constexpr int kTile = 64;      // rows per LDS tile
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2;
+using lptr_t = __attribute__((address_space(3))) void*;
+
+template <typename TR>
+__device__ __forceinline__ f32x4 mfma(const s16x8& a, const s16x8& b, const f32x4& c) {
+  if constexpr (std::is_same<TR, F16>::value) {
+    typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  } else {
+    typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+}
+
+template <typename TR>
+__device__ __forceinline__ s16x8 pack8(const f32x4& a, const f32x4& b) {
+  u16x8 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r[e] = TR::from_f32(a[e]);
+    r[4 + e] = TR::from_f32(b[e]);
+  }
+  return __builtin_bit_cast(s16x8, r);
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile image of [rows][D] 16-bit elements.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  return D == 64 ? (((r >> 1) & 3) << 1 | ((r >> 3) & 1)) : ((r & 7) << 1 | ((r >> 3) & 1));
+}
+template <int D>
+__device__ __forceinline__ int tile_off(int r, int c) { return r * (2 * D) + ((c ^ swz<D>(r)) << 4); }
+
+// Matrix operand fragment out of a tile: lane holds row 16 t + (lane & 15), d = 32 kk + 8 (lane >> 4) ..
+template <int D>
+__device__ __forceinline__ s16x8 row_frag(const char* tile, int t, int kk, int lane) {
+  return *reinterpret_cast<const s16x8*>(tile + tile_off<D>(16 * t + (lane & 15), 4 * kk + (lane >> 4)));
+}
+// Transposed fragment: lane holds d = 16 td + (lane & 15); its eight k-slots are rows base + 4 g + 0..3 and base + 16 + 4 g + 0..3
+// (g = lane >> 4), the rows that a 16x16 accumulator pair keeps in that lane group's registers.
+template <int D>
+__device__ __forceinline__ s16x8 tr_frag(const char* tile, int base, int td, int lane) {
+  const int g = lane >> 4, i = lane & 15, qq = i >> 2, pp = i & 3;
+  const int c = 2 * td + (pp >> 1), sub = (pp & 1) << 3, r = base + 4 * g + qq;
+  using lds_ptr = __attribute__((address_space(3))) s16x4*;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<D>(r, c) + sub));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_off<D>(r + 16, c) + sub));
+  return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+__device__ __forceinline__ float groups_max(float x) {  // over the four 16-lane groups of a wave
+  const unsigned xi = __float_as_uint(x);
+  const u32x2 a = __builtin_amdgcn_permlane32_swap(xi, xi, false, false);
+  const float m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const unsigned mi = __float_as_uint(m);
+  const u32x2 b = __builtin_amdgcn_permlane16_swap(mi, mi, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+  const unsigned xi = __float_as_uint(x);
+  const u32x2 a = __builtin_amdgcn_permlane32_swap(xi, xi, false, false);
+  const float s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const unsigned si = __float_as_uint(s);
+  const u32x2 b = __builtin_amdgcn_permlane16_swap(si, si, false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// At most N of this wave's vector-memory operations (DMA included) outstanding, visible to the compiler's own bookkeeping.
+template <int N>
+__device__ __forceinline__ void wait_vmem_at_most() {
+  static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+__device__ __forceinline__ const char* uniform_ptr(const void* p) {
+  const unsigned long long v = reinterpret_cast<unsigned long long>(p);
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
+  const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v >> 32));
+  return reinterpret_cast<const char*>((static_cast<unsigned long long>(hi) << 32) | lo);
+}
+// 64 x 16 (64 x 4) bytes global -> LDS: lane l's piece lands at lds + 16 l (4 l).  As assembly, because the compiler would put
+// every transposing read behind ALL the DMA it knows of; the kernels order DMA and reads by counted waits and barriers.
+__device__ __forceinline__ void dma_16B(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma_4B(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const char* p) {
+  return __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<uintptr_t>((lptr_t)p)));
+}
+
+// One wave's share of a tile's requests: D / 16 pieces of 1 KiB of one operand, starting at piece `piece0`.
+template <int D>
+struct TileSource {
+  static constexpr int kPieces = D / 16;
+  static constexpr int kPieceRows = 512 / D;   // rows of 2 D bytes per 1 KiB
+  unsigned off[kPieces];
+  unsigned pitch;   // bytes between rows
+  int row[kPieces], chunk[kPieces];
+  __device__ __forceinline__ void init(long long stride, int piece0, int lane) {
+    pitch = static_cast<unsigned>(stride) * 2u;
+    constexpr int kLanesPerRow = 64 / kPieceRows;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      row[i] = (piece0 + i) * kPieceRows + lane / kLanesPerRow;
+      chunk[i] = ((lane % kLanesPerRow) ^ swz<D>(row[i])) * 16;
+      off[i] = static_cast<unsigned>(row[i]) * pitch + static_cast<unsigned>(chunk[i]);
+    }
+  }
+  // `first`: the tile's first row; only `valid` (>= 1) of its rows may be read, the others repeat the last of those.
+  __device__ __forceinline__ void request(const u16* first, int valid, unsigned lds) const {
+    const char* base = uniform_ptr(first);
+    if (valid >= kTile) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) dma_16B(base, off[i], lds + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = row[i] < valid ? row[i] : valid - 1;
+        dma_16B(base, static_cast<unsigned>(r) * pitch + static_cast<unsigned>(chunk[i]), lds + i * 1024);
+      }
+    }
+  }
+};
+
+template <int D>
+constexpr int kTileBytes = kTile * D * 2;
+template <int D>
+constexpr int kStages = D == 64 ? 3 : 2;  // two workgroups of D = 128 tiles per CU
+template <int D>
+constexpr int kStripPitch = 2 * D + 16;
+template <int D>
+constexpr int kStripBytes = 32 * kStripPitch<D>;
+
+// The wave's 32 rows leave through an LDS strip of its own, whole rows per store instruction.  acc[st][td]: row 16 st + (lane & 15), d = 16 td + 4 g + e.
+// Rows at or beyond `len` become zero, rows at or beyond `T` are not written.  row0: the wave's first row.
+template <typename TR, int D>
+__device__ __forceinline__ void store_rows(char* strip, const f32x4 (&acc)[2][D / 16], const float (&scale)[2], u16* out, long long stride, int row0, int len,
+                                           int T, int lane) {
+  const int g = lane >> 4, li = lane & 15;
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    const bool live = row0 + 16 * st + li < len;
+#pragma unroll
+    for (int td = 0; td < D / 16; ++td) {
+      u16x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = live ? TR::from_f32(acc[st][td][e] * scale[st]) : static_cast<u16>(0);
+      *reinterpret_cast<u16x4*>(strip + (16 * st + li) * kStripPitch<D> + (16 * td + 4 * g) * 2) = w;
+    }
+  }
+  // a wave reads back only its own writes; the LDS serves one wave's requests in order
+  constexpr int kPerRow = D / 8, kRowsPerStore = 64 / kPerRow;
+#pragma unroll
+  for (int it = 0; it < 32 / kRowsPerStore; ++it) {
+    const int r = it * kRowsPerStore + lane / kPerRow, ch = lane % kPerRow;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(strip + r * kStripPitch<D> + ch * 16);
+    if (row0 + r < T) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out + static_cast<long long>(row0 + r) * stride + ch * 8));
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void zero_rows(u16* out, long long stride, int row0, int T) {
+  constexpr int kPerRow = D / 8;
+  for (int i = threadIdx.x; i < kRows * kPerRow; i += kThreads) {
+    const int r = row0 + i / kPerRow;
+    if (r < T) *reinterpret_cast<u32x4*>(out + static_cast<long long>(r) * stride + (i % kPerRow) * 8) = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// Workgroup id -> position in an order whose neighbours share an XCD (and so its L2).
+__device__ __forceinline__ int xcd_order(int id, int n) {
+  const int q = n >> 3, r = n & 7, x = id & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+}
+
+__device__ __forceinline__ int length_of(const WindowAttnArgs& p, int b) {
+  if (!p.lens) return p.T;
+  const int n = p.lens[b];
+  return n < 0 ? 0 : n > p.T ? p.T : n;
+}
+
+// Key tiles that a block of queries q0 .. q0 + 127 can see: the first `sink_tiles` tiles, then tiles first .. last.
+struct KeyTiles {
+  int sink_tiles, first, count;
+  __device__ __forceinline__ KeyTiles(const WindowAttnArgs& p, int q0, int len) {
+    const int lo = q0 - p.window + 1, hi = q0 + kRows - 1 < len - 1 ? q0 + kRows - 1 : len - 1;
+    first = (lo > 0 ? lo : 0) / kTile;
+    const int s = (p.sinks + kTile - 1) / kTile;
+    sink_tiles = s < first ? s : first;
+    count = sink_tiles + hi / kTile - first + 1;
+  }
+  __device__ __forceinline__ int key0(int it) const { return (it < sink_tiles ? it : first + it - sink_tiles) * kTile; }
+  // Rows of the tile that the block may see at all: the tiles in front of the window hold sinks only.
+  __device__ __forceinline__ int valid(const WindowAttnArgs& p, int it, int len) const {
+    return (it < sink_tiles && p.sinks < len ? p.sinks : len) - key0(it);
+  }
+};
+
+// What a wave of 32 queries from qw has to do with the 64 keys from key0.
+__device__ __forceinline__ bool wave_sees(const WindowAttnArgs& p, int qw, int key0) {
+  return key0 <= qw + 31 && (key0 + kTile - 1 > qw - p.window || key0 < p.sinks);
+}
+__device__ __forceinline__ bool needs_mask(const WindowAttnArgs& p, int qw, int key0) {
+  return key0 + kTile - 1 > qw || !(key0 > qw + 31 - p.window || key0 + kTile - 1 < p.sinks);
+}
+
+// ---------------------------------------------------------------------------------------------------- forward
+// Online softmax over raw scores with the scale in the exponent's FMA; the running maximum (log2 domain) only moves when a score
+// exceeds it by more than kDefer, so probabilities stay below 2^kDefer and the rescale of the output is rare.  Row sums come out of
+// the matrix pipe (ones times P), of exactly the rounded values that multiply V.
+constexpr float kDefer = 8.f;
+constexpr float kLowest = -1e30f;  // a start below every score that keeps exp2(-inf - m) at zero where a query sees nothing yet
+
+template <typename TR, int D, bool MASK>
+__device__ __forceinline__ void fwd_tile(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], f32x4 (&o)[2][D / 16],
+                                         float (&m)[2], f32x4 (&lsum)[2], int key0, int qw, int lane) {
+  const int g = lane >> 4, li = lane & 15;
+  const float c = p.scale_log2;
+  f32x4 s[2][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) s[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      const s16x8 kf = row_frag<D>(ks, t, kk, lane);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
+    }
+  }
+  s16x8 pf[2][2];
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    if (MASK) {  // register (t, e) is key key0 + 4 g + 16 t + e
+      const int rel = qw + 16 * st + li - key0 - 4 * g, sink = p.sinks - key0 - 4 * g;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 16 * t + e;
+          if (j > rel || (j <= rel - p.window && j >= sink)) s[st][t][e] = kNegInf;
+        }
+    }
+    float mx = s[st][0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[st][i >> 2][i & 3]);
+    mx *= c;  // c > 0
+    if (__any(mx > m[st] + kDefer)) {
+      const float mg = groups_max(mx);
+      const float m_new = mg > m[st] + kDefer ? mg : m[st];
+      const float alpha = __builtin_amdgcn_exp2f(m[st] - m_new);
+      m[st] = m_new;
+#pragma unroll
+      for (int td = 0; td < D / 16; ++td)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[st][td][e] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lsum[st][e] *= alpha;
+    }
+    const float nm = -m[st];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[st][t][e] = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, nm));
+#pragma unroll
+    for (int sk = 0; sk < 2; ++sk) pf[st][sk] = pack8<TR>(s[st][2 * sk], s[st][2 * sk + 1]);
+  }
+  const short one = std::is_same<TR, F16>::value ? 0x3C00 : 0x3F80;
+  const s16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+  for (int sk = 0; sk < 2; ++sk)
+#pragma unroll
+    for (int st = 0; st < 2; ++st) lsum[st] = mfma<TR>(ones, pf[st][sk], lsum[st]);
+#pragma unroll
+  for (int td = 0; td < D / 16; ++td)
+#pragma unroll
+    for (int sk = 0; sk < 2; ++sk) {
+      const s16x8 vf = tr_frag<D>(vs, 32 * sk, td, lane);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) o[st][td] = mfma<TR>(vf, pf[st][sk], o[st][td]);
+    }
+}
+
+// Workgroup -> (batch, query head, query block): the heads of a group next to each other, then the blocks, the long ones first.
+__device__ __forceinline__ void query_item(const WindowAttnArgs& p, int& b, int& h, int& qb) {
+  const int G = p.H / p.KV, nqb = (p.T + kRows - 1) / kRows;
+  const int v = xcd_order(blockIdx.x, gridDim.x);
+  const int per_kv = nqb * G, bk = v / per_kv, rest = v - bk * per_kv;
+  b = bk / p.KV;
+  h = (bk - b * p.KV) * G + rest % G;
+  qb = nqb - 1 - rest / G;
+}
+
+template <typename TR, int D>
+__global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stages][K | V], then the output strips
+  constexpr int S = kStages<D>, TB = kTileBytes<D>, NP = TileSource<D>::kPieces;
+  int b, h, qb;
+  query_item(p, b, h, qb);
+  const int q0 = qb * kRows, len = length_of(p, b);
+  const long long o_stride = static_cast<long long>(p.H) * D;
+  u16* out = static_cast<u16*>(p.o) + static_cast<long long>(b) * p.T * o_stride + static_cast<long long>(h) * D;
+  if (q0 >= len) {
+    zero_rows<D>(out, o_stride, q0, p.T);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, li = lane & 15, qw = q0 + wid * 32;
+  const u16* base = static_cast<const u16*>(p.qkv) + static_cast<long long>(b) * p.batch_stride;
+  const u16* Q = base + static_cast<long long>(h) * D;
+  const int kv = h / (p.H / p.KV);
+  const bool moves_v = wid >= 2;
+  const u16* src = base + static_cast<long long>(p.H + kv + (moves_v ? p.KV : 0)) * D;
+  const KeyTiles tiles(p, q0, len);
+  TileSource<D> ts;
+  ts.init(p.row_stride, (wid & 1) * NP, lane);
+  const unsigned dst = lds_address(smem) + (moves_v ? TB : 0) + (wid & 1) * NP * 1024;
+  auto request = [&](int it, int stage) {
+    const int k0 = tiles.key0(it);
+    ts.request(src + static_cast<long long>(k0) * p.row_stride, tiles.valid(p, it, len), dst + stage * 2 * TB);
+  };
+  request(0, 0);
+  if (S > 2 && tiles.count > 1) request(1, 1);
+  s16x8 qf[2][D / 32];
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    const int qi = qw + 16 * st + li < len ? qw + 16 * st + li : len - 1;
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) qf[st][kk] = *reinterpret_cast<const s16x8*>(Q + static_cast<long long>(qi) * p.row_stride + 32 * kk + 8 * g);
+  }
+  f32x4 o[2][D / 16], lsum[2];
+  float m[2] = {kLowest, kLowest};
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    lsum[st] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int td = 0; td < D / 16; ++td) o[st][td] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  wait_vmem_at_most<0>();
+  int stage = 0;
+  for (int it = 0; it < tiles.count; ++it) {
+    if (S > 2 && it + 1 < tiles.count) wait_vmem_at_most<NP>();  // this wave's pieces of the tile have landed
+    else wait_vmem_at_most<0>();
+    __syncthreads();  // everybody's have; nobody still reads the stage that is requested next
+    if (it + S - 1 < tiles.count) request(it + S - 1, stage == 0 ? S - 1 : stage - 1);
+    const char* ks = smem + stage * 2 * TB;
+    const int key0 = tiles.key0(it);
+    if (wave_sees(p, qw, key0)) {
+      if (needs_mask(p, qw, key0)) fwd_tile<TR, D, true>(p, ks, ks + TB, qf, o, m, lsum, key0, qw, lane);
+      else fwd_tile<TR, D, false>(p, ks, ks + TB, qf, o, m, lsum, key0, qw, lane);
+    }
+    stage = stage + 1 == S ? 0 : stage + 1;
+  }
+  float inv[2];
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    const float l = lsum[st][0];  // every accumulator row holds the sum for this lane's query
+    inv[st] = 1.f / l;
+    const int qi = qw + 16 * st + li;
+    if (p.lse2 && g == 0 && qi < len) p.lse2[(static_cast<long long>(b) * p.H + h) * p.T + qi] = m[st] + log2f(l);
+  }
+  __syncthreads();  // tile stages -> output strips
+  store_rows<TR, D>(smem + wid * kStripBytes<D>, o, inv, out, o_stride, qw, len, p.T, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------- backward: dQ
+template <typename TR, int D, bool MASK>
+__device__ __forceinline__ void dq_tile(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], const s16x8 (&dof)[2][D / 32],
+                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const float (&delta)[2], int key0, int qw, int lane) {
+  const int g = lane >> 4, li = lane & 15;
+  const float c = p.scale_log2;
+  s16x8 dsf[2][2];
+  // two 16-key tiles at a time: one operand of the next product
+#pragma unroll
+  for (int sk = 0; sk < 2; ++sk) {
+    f32x4 s[2][2], dp[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int st = 0; st < 2; ++st) s[st][t] = dp[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk) {
+        const s16x8 kf = row_frag<D>(ks, 2 * sk + t, kk, lane), vf = row_frag<D>(vs, 2 * sk + t, kk, lane);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
+          dp[st][t] = mfma<TR>(vf, dof[st][kk], dp[st][t]);
+        }
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const int rel = qw + 16 * st + li - key0 - 4 * g - 32 * sk, sink = p.sinks - key0 - 4 * g - 32 * sk;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 16 * t + e;
+          const float pe = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, -lse2[st]));
+          const float ds = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
+          s[st][t][e] = MASK && (j > rel || (j <= rel - p.window && j >= sink)) ? 0.f : ds;
+        }
+      dsf[st][sk] = pack8<TR>(s[st][0], s[st][1]);
+    }
+  }
+#pragma unroll
+  for (int td = 0; td < D / 16; ++td)
+#pragma unroll
+    for (int sk = 0; sk < 2; ++sk) {
+      const s16x8 kt = tr_frag<D>(ks, 32 * sk, td, lane);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) dq[st][td] = mfma<TR>(kt, dsf[st][sk], dq[st][td]);
+    }
+}
+
+template <typename TR, int D>
+__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int S = kStages<D>, TB = kTileBytes<D>, NP = TileSource<D>::kPieces;
+  int b, h, qb;
+  query_item(p, b, h, qb);
+  const int q0 = qb * kRows, len = length_of(p, b);
+  const long long g_stride = static_cast<long long>(p.H + 2 * p.KV) * D, o_stride = static_cast<long long>(p.H) * D;
+  u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(h) * D;
+  if (q0 >= len) {
+    zero_rows<D>(out, g_stride, q0, p.T);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, li = lane & 15, qw = q0 + wid * 32;
+  const u16* base = static_cast<const u16*>(p.qkv) + static_cast<long long>(b) * p.batch_stride;
+  const u16* Q = base + static_cast<long long>(h) * D;
+  const int kv = h / (p.H / p.KV);
+  const bool moves_v = wid >= 2;
+  const u16* src = base + static_cast<long long>(p.H + kv + (moves_v ? p.KV : 0)) * D;
+  const KeyTiles tiles(p, q0, len);
+  TileSource<D> ts;
+  ts.init(p.row_stride, (wid & 1) * NP, lane);
+  const unsigned dst = lds_address(smem) + (moves_v ? TB : 0) + (wid & 1) * NP * 1024;
+  auto request = [&](int it, int stage) {
+    const int k0 = tiles.key0(it);
+    ts.request(src + static_cast<long long>(k0) * p.row_stride, tiles.valid(p, it, len), dst + stage * 2 * TB);
+  };
+  request(0, 0);
+  if (S > 2 && tiles.count > 1) request(1, 1);
+  const long long ho = static_cast<long long>(b) * p.T * o_stride + static_cast<long long>(h) * D;
+  const u16* O = static_cast<const u16*>(p.o) + ho;
+  const u16* DO = static_cast<const u16*>(p.d_o) + ho;
+  const long long stat = (static_cast<long long>(b) * p.H + h) * p.T;
+  s16x8 qf[2][D / 32], dof[2][D / 32];
+  float lse2[2], delta[2];
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    const bool live = qw + 16 * st + li < len;
+    const long long qi = live ? qw + 16 * st + li : len - 1;
+    float part = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      qf[st][kk] = *reinterpret_cast<const s16x8*>(Q + qi * p.row_stride + 32 * kk + 8 * g);
+      dof[st][kk] = *reinterpret_cast<const s16x8*>(DO + qi * o_stride + 32 * kk + 8 * g);
+      const s16x8 of = *reinterpret_cast<const s16x8*>(O + qi * o_stride + 32 * kk + 8 * g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part = fmaf(TR::to_f32(static_cast<u16>(dof[st][kk][j])), TR::to_f32(static_cast<u16>(of[j])), part);
+    }
+    lse2[st] = p.lse2[stat + qi];
+    delta[st] = groups_sum(part);  // the four lane groups hold D / 4 values each
+    if (g == 0 && live) p.delta[stat + qi] = delta[st];
+  }
+  f32x4 dq[2][D / 16];
+#pragma unroll
+  for (int st = 0; st < 2; ++st)
+#pragma unroll
+    for (int td = 0; td < D / 16; ++td) dq[st][td] = f32x4{0.f, 0.f, 0.f, 0.f};
+  wait_vmem_at_most<0>();
+  int stage = 0;
+  for (int it = 0; it < tiles.count; ++it) {
+    if (S > 2 && it + 1 < tiles.count) wait_vmem_at_most<NP>();
+    else wait_vmem_at_most<0>();
+    __syncthreads();
+    if (it + S - 1 < tiles.count) request(it + S - 1, stage == 0 ? S - 1 : stage - 1);
+    const char* ks = smem + stage * 2 * TB;
+    const int key0 = tiles.key0(it);
+    if (wave_sees(p, qw, key0)) {
+      if (needs_mask(p, qw, key0)) dq_tile<TR, D, true>(p, ks, ks + TB, qf, dof, dq, lse2, delta, key0, qw, lane);
+      else dq_tile<TR, D, false>(p, ks, ks + TB, qf, dof, dq, lse2, delta, key0, qw, lane);
+    }
+    stage = stage + 1 == S ? 0 : stage + 1;
+  }
+  __syncthreads();
+  const float by_scale[2] = {p.scale, p.scale};
+  store_rows<TR, D>(smem + wid * kStripBytes<D>, dq, by_scale, out, g_stride, qw, len, p.T, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------- backward: dK, dV
+// Units of one (batch, key / value head): key block kb (128 keys) meets the query tiles (64 queries) 2 kb .. 2 kb + tiles(kb) - 1 of each
+// of the G heads of its group; its units are numbered head by head.
+struct Units {
+  int T, window, sinks, G, n_tiles, n_blocks;
+  int by_window;   // query tiles that a window reaches from a block, its own two among them
+  int sink_blocks;
+  __host__ __device__ Units(int T_, int window_, int sinks_, int G_) : T(T_), window(window_), sinks(sinks_), G(G_) {
+    n_tiles = (T + kTile - 1) / kTile;
+    n_blocks = (T + kRows - 1) / kRows;
+    by_window = static_cast<int>((static_cast<long long>(kRows) + window - 2) / kTile) + 1;
+    sink_blocks = (sinks + kRows - 1) / kRows;
+    if (sink_blocks > n_blocks) sink_blocks = n_blocks;
+  }
+  __host__ __device__ int tiles(int kb) const {
+    const int left = n_tiles - 2 * kb;
+    return kb < sink_blocks || left < by_window ? left : by_window;
+  }
+  __host__ __device__ long long before(int kb) const {  // units of the blocks in front of kb
+    const long long s = kb < sink_blocks ? kb : sink_blocks, w = kb - s;
+    long long n = s * n_tiles - s * (s - 1);
+    if (w > 0) {
+      // blocks s .. kb - 1: by_window tiles each until fewer are left, from block `cut` on
+      long long cut = n_tiles - by_window >= 0 ? (n_tiles - by_window) / 2 + 1 : 0;
+      cut = cut < s ? s : cut > kb ? kb : cut;
+      n += (cut - s) * by_window;
+      n += (kb - cut) * n_tiles - (static_cast<long long>(kb) * (kb - 1) - cut * (cut - 1));
+    }
+    return n * G;
+  }
+  __host__ __device__ long long all() const { return before(n_blocks); }
+  __host__ __device__ int block_of(long long u) const {  // the block that unit u belongs to
+    int lo = 0, hi = n_blocks - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before(mid) <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+
+template <int D>
+constexpr int kDkdvStageBytes = 2 * kTileBytes<D> + 2 * kTile * 4;  // Q | dO | lse2 | delta
+constexpr int kDkdvStages = 3;
+
+template <typename TR, int D, bool MASK>
+__device__ __forceinline__ void dkdv_tile(const WindowAttnArgs& p, const char* qs_, const char* dos_, const char* stats, const s16x8 (&kf)[2][D / 32],
+                                          const s16x8 (&vf)[2][D / 32], f32x4 (&dk)[2][D / 16], f32x4 (&dv)[2][D / 16], int half, int q0, int kw,
+                                          int len, int lane) {
+  // the 32 queries from q0, rows 32 half .. of the stage's tiles, against the wave's 32 keys from kw
+  const int g = lane >> 4, li = lane & 15;
+  const float c = p.scale_log2;
+  f32x4 l2[2], dl[2];  // register (qs, e): query q0 + 16 qs + 4 g + e
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    l2[qs] = *reinterpret_cast<const f32x4*>(stats + (32 * half + 16 * qs + 4 * g) * 4);
+    dl[qs] = *reinterpret_cast<const f32x4*>(stats + (kTile + 32 * half + 16 * qs + 4 * g) * 4);
+  }
+  f32x4 s[2][2], dp[2][2];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) s[kt][qs] = dp[kt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk) {
+      const s16x8 qr = row_frag<D>(qs_, 2 * half + qs, kk, lane), dr = row_frag<D>(dos_, 2 * half + qs, kk, lane);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        s[kt][qs] = mfma<TR>(qr, kf[kt][kk], s[kt][qs]);
+        dp[kt][qs] = mfma<TR>(dr, vf[kt][kk], dp[kt][qs]);
+      }
+    }
+  }
+  s16x8 pB[2], dsB[2];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const int key = kw + 16 * kt + li, rel = key - q0 - 4 * g;   // register (qs, e) is query index 16 qs + e against rel
+    const int far = key < p.sinks ? 0x7fffffff : rel + p.window;  // first index beyond the window
+    const int end = len - q0 - 4 * g;                             // first index beyond the sequence
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * qs + e;
+        float pe = __builtin_amdgcn_exp2f(fmaf(s[kt][qs][e], c, -l2[qs][e]));
+        float ds = pe * (dp[kt][qs][e] - dl[qs][e]);
+        if (MASK && (i < rel || i >= far || i >= end)) pe = ds = 0.f;
+        s[kt][qs][e] = pe;
+        dp[kt][qs][e] = ds;
+      }
+    pB[kt] = pack8<TR>(s[kt][0], s[kt][1]);
+    dsB[kt] = pack8<TR>(dp[kt][0], dp[kt][1]);
+  }
+#pragma unroll
+  for (int td = 0; td < D / 16; ++td) {
+    const s16x8 dot = tr_frag<D>(dos_, 32 * half, td, lane), qt = tr_frag<D>(qs_, 32 * half, td, lane);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      dv[kt][td] = mfma<TR>(dot, pB[kt], dv[kt][td]);
+      dk[kt][td] = mfma<TR>(qt, dsB[kt], dk[kt][td]);
+    }
+  }
+}
+
+// fp32 partial sums of a cut block: [slot][wave][dk | dv][kt][td][lane] of four values.
+template <int D>
+constexpr long long kPartialFloats = 2LL * kRows * D;
+
+__device__ __forceinline__ long long piece_start(const WindowAttnArgs& p, long long total, int w) { return total * w / p.pieces; }
+
+template <typename TR, int D>
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(WindowAttnArgs p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stages][Q | dO | lse2 | delta], then the output strips
+  constexpr int S = kDkdvStages, TB = kTileBytes<D>, SB = kDkdvStageBytes<D>, NP = TileSource<D>::kPieces;
+  const int G = p.H / p.KV;
+  const Units units(p.T, p.window, p.sinks, G);
+  const long long per_head = units.all(), total = per_head * p.KV * p.B;
+  const int piece = xcd_order(blockIdx.x, p.pieces);
+  long long u = piece_start(p, total, piece);
+  const long long u_end = piece_start(p, total, piece + 1);
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, li = lane & 15;
+  const long long o_stride = static_cast<long long>(p.H) * D, g_stride = static_cast<long long>(p.H + 2 * p.KV) * D;
+  const bool moves_do = wid >= 2, moves_stat = (wid & 1) == 0;
+  TileSource<D> ts;
+  ts.init(moves_do ? o_stride : p.row_stride, (wid & 1) * NP, lane);
+  const unsigned lds0 = lds_address(smem);
+  const unsigned dst = lds0 + (moves_do ? TB : 0) + (wid & 1) * NP * 1024;
+  const unsigned stat_dst = lds0 + 2 * TB + (moves_do ? kTile * 4 : 0);
+
+  while (u < u_end) {
+    const long long bk = u / per_head, in_head = u - bk * per_head;
+    const int b = static_cast<int>(bk / p.KV), kv = static_cast<int>(bk - static_cast<long long>(b) * p.KV);
+    const int kb = units.block_of(in_head);
+    const long long start = bk * per_head + units.before(kb);
+    const int n = units.tiles(kb);                              // query tiles per head, at full length
+    const long long stop = start + static_cast<long long>(n) * G;
+    const long long upto = stop < u_end ? stop : u_end;
+    const int len = length_of(p, b), k0 = kb * kRows, kw = k0 + wid * 32;
+    const int first_qt = 2 * kb;
+    int ne = (len + kTile - 1) / kTile - first_qt;              // query tiles that hold anything
+    ne = ne < 0 ? 0 : ne < n ? ne : n;
+    // this piece's part of the block: units ua .. ub - 1 of it, of which those with a tile index below ne are walked
+    const int ua = static_cast<int>(u - start), ub = static_cast<int>(upto - start);
+    auto walked = [&](int x) { const int q = x / n, r = x - q * n; return q * ne + (r < ne ? r : ne); };
+    const int steps = walked(ub) - walked(ua);
+    int rg = ua / n, rt = ua - rg * n;                          // request cursor: head of the group, tile
+    if (rt >= ne) { rt = 0; ++rg; }
+    int ct = rt;                                                // tile being multiplied
+    const u16* base = static_cast<const u16*>(p.qkv) + static_cast<long long>(b) * p.batch_stride;
+    auto request = [&](int stage) {
+      const int row = (first_qt + rt) * kTile, h = kv * G + rg;
+      const u16* src = moves_do ? static_cast<const u16*>(p.d_o) + (static_cast<long long>(b) * p.T + row) * o_stride + static_cast<long long>(h) * D
+                                : base + static_cast<long long>(row) * p.row_stride + static_cast<long long>(h) * D;
+      ts.request(src, len - row, dst + stage * SB);
+      if (moves_stat) {
+        const float* st = (moves_do ? p.delta : p.lse2) + (static_cast<long long>(b) * p.H + h) * p.T + row;
+        const int i = lane < len - row ? lane : len - row - 1;
+        dma_4B(uniform_ptr(st), static_cast<unsigned>(i) * 4u, stat_dst + stage * SB);
+      }
+      if (++rt == ne) { rt = 0; ++rg; }
+    };
+    f32x4 dk[2][D / 16], dv[2][D / 16];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int td = 0; td < D / 16; ++td) dk[kt][td] = dv[kt][td] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (steps > 0) {
+      __syncthreads();  // the previous block's output strips (same memory) have been read back
+      request(0);
+      if (steps > 1) request(1);
+      s16x8 kf[2][D / 32], vf[2][D / 32];
+      const u16* K = base + static_cast<long long>(p.H + kv) * D;
+      const u16* V = K + static_cast<long long>(p.KV) * D;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const long long key = kw + 16 * kt + li < len ? kw + 16 * kt + li : len - 1;
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {
+          kf[kt][kk] = *reinterpret_cast<const s16x8*>(K + key * p.row_stride + 32 * kk + 8 * g);
+          vf[kt][kk] = *reinterpret_cast<const s16x8*>(V + key * p.row_stride + 32 * kk + 8 * g);
+        }
+      }
+      wait_vmem_at_most<0>();
+      int stage = 0;
+      for (int it = 0; it < steps; ++it) {
+        if (it + 1 < steps) {
+          if (moves_stat) wait_vmem_at_most<NP + 1>();
+          else wait_vmem_at_most<NP>();
+        } else {
+          wait_vmem_at_most<0>();
+        }
+        __syncthreads();
+        if (it + 2 < steps) request(stage == 0 ? 2 : stage - 1);
+        const char* qs = smem + stage * SB;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int q0 = (first_qt + ct) * kTile + 32 * half;
+          // the half precedes all of the wave's keys, lies behind the window of the last one and no sink is among them, or behind the sequence
+          const bool skip = q0 + 31 < kw || (q0 >= kw + 31 + p.window && kw >= p.sinks) || q0 >= len;
+          if (!skip) {
+            const bool clear = q0 >= kw + 31 && (q0 + 31 < kw + p.window || kw + 31 < p.sinks) && q0 + 31 < len;
+            if (clear) dkdv_tile<TR, D, false>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
+            else dkdv_tile<TR, D, true>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
+          }
+        }
+        if (++ct == ne) ct = 0;
+        stage = stage + 1 == S ? 0 : stage + 1;
+      }
+    }
+    if (u == start && upto == stop) {
+      __syncthreads();  // tile stages -> output strips
+      u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(p.H + kv) * D;
+      const float by_scale[2] = {p.scale, p.scale}, one[2] = {1.f, 1.f};
+      store_rows<TR, D>(smem + wid * kStripBytes<D>, dk, by_scale, out, g_stride, kw, len, p.T, lane);
+      store_rows<TR, D>(smem + wid * kStripBytes<D>, dv, one, out + static_cast<long long>(p.KV) * D, g_stride, kw, len, p.T, lane);
+    } else {
+      // slot 0: the block began in an earlier piece; slot 1: it began here
+      f32x4* ws = reinterpret_cast<f32x4*>(p.partial + (2LL * piece + (u == start ? 1 : 0)) * kPartialFloats<D>) + wid * (4 * (D / 16) * 64) + lane;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int td = 0; td < D / 16; ++td) {
+          ws[(kt * (D / 16) + td) * 64] = dk[kt][td];
+          ws[((2 + kt) * (D / 16) + td) * 64] = dv[kt][td];
+        }
+    }
+    u = upto;
+  }
+}
+
+// Adds up the partial sums of the block that piece `blockIdx.x` begins in the middle of, if it is the first such piece.
+template <typename TR, int D>
+__global__ __launch_bounds__(kThreads, 2) void window_join_kernel(WindowAttnArgs p) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int G = p.H / p.KV;
+  const Units units(p.T, p.window, p.sinks, G);
+  const long long per_head = units.all(), total = per_head * p.KV * p.B;
+  const int w = blockIdx.x + 1;
+  const long long s = piece_start(p, total, w);
+  const long long bk = s / per_head;
+  const int b = static_cast<int>(bk / p.KV), kv = static_cast<int>(bk - static_cast<long long>(b) * p.KV);
+  const int kb = units.block_of(s - bk * per_head);
+  const long long start = bk * per_head + units.before(kb), stop = start + static_cast<long long>(units.tiles(kb)) * G;
+  if (s == start || s == total || piece_start(p, total, w - 1) > start) return;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int len = length_of(p, b), kw = kb * kRows + wid * 32;
+  f32x4 dk[2][D / 16], dv[2][D / 16];
+  auto add = [&](int piece, int slot, bool first) {
+    const f32x4* ws = reinterpret_cast<const f32x4*>(p.partial + (2LL * piece + slot) * kPartialFloats<D>) + wid * (4 * (D / 16) * 64) + lane;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int td = 0; td < D / 16; ++td) {
+        const f32x4 a = ws[(kt * (D / 16) + td) * 64], c = ws[((2 + kt) * (D / 16) + td) * 64];
+        dk[kt][td] = first ? a : dk[kt][td] + a;
+        dv[kt][td] = first ? c : dv[kt][td] + c;
+      }
+  };
+  add(w - 1, 1, true);
+  for (int piece = w; piece < p.pieces && piece_start(p, total, piece) < stop; ++piece)
+    if (piece_start(p, total, piece + 1) > piece_start(p, total, piece)) add(piece, 0, false);
+  const long long g_stride = static_cast<long long>(p.H + 2 * p.KV) * D;
+  u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(p.H + kv) * D;
+  const float by_scale[2] = {p.scale, p.scale}, one[2] = {1.f, 1.f};
+  store_rows<TR, D>(smem + wid * kStripBytes<D>, dk, by_scale, out, g_stride, kw, len, p.T, lane);
+  store_rows<TR, D>(smem + wid * kStripBytes<D>, dv, one, out + static_cast<long long>(p.KV) * D, g_stride, kw, len, p.T, lane);
+}
+
+// More than 64 KiB of dynamic LDS has to be asked for.
+template <typename Kernel>
+void allow_lds(Kernel k, int bytes) {
+  if (bytes > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <int D>
+constexpr int kQueryLds = kStages<D> * 2 * kTileBytes<D> > 4 * kStripBytes<D> ? kStages<D> * 2 * kTileBytes<D> : 4 * kStripBytes<D>;
+template <int D>
+constexpr int kDkdvLds = kDkdvStages * kDkdvStageBytes<D> > 4 * kStripBytes<D> ? kDkdvStages * kDkdvStageBytes<D> : 4 * kStripBytes<D>;
+
+template <typename F>
+void dispatch(int dtype, int D, F&& f) {
+  if (dtype == kBF16) {
+    if (D == 64) f(BF16{}, std::integral_constant<int, 64>{});
+    else f(BF16{}, std::integral_constant<int, 128>{});
+  } else {
+    if (D == 64) f(F16{}, std::integral_constant<int, 64>{});
+    else f(F16{}, std::integral_constant<int, 128>{});
+  }
+}
+
+long long query_items(const WindowAttnArgs& a) { return static_cast<long long>(a.B) * a.H * ((a.T + kRows - 1) / kRows); }
+
+}  // namespace
+
+bool window_attention_supported(long long B, long long T, long long H, long long KV, long long D, long long row_stride, int dtype) {
+  if (!(dtype == kBF16 || dtype == kF16) || !(D == 64 || D == 128)) return false;
+  if (B < 0 || T < 0 || H < 1 || KV < 1 || H % KV != 0) return false;
+  if (T > (1ll << 30) || row_stride % 8 != 0 || row_stride >= (1ll << 24) || (H + 2 * KV) * D >= (1ll << 24)) return false;  // a tile's byte offsets are 32-bit
+  return B * H * ((T + kRows - 1) / kRows) < (1ll << 31);
+}
+
+// One piece per workgroup that the chip holds at once, and none of less than four units.
+int window_attention_pieces(const WindowAttnArgs& a) {
+  const Units units(a.T, a.window, a.sinks, a.H / a.KV);
+  const long long total = units.all() * a.KV * a.B;
+  long long n = a.compute_units * (a.D == 64 ? 2 : 1);
+  if (n > (total + 3) / 4) n = (total + 3) / 4;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+long long window_attention_partial_floats(const WindowAttnArgs& a) { return a.pieces > 1 ? 2LL * a.pieces * 2 * kRows * a.D : 0; }
+
+void launch_window_attention_fwd(const WindowAttnArgs& args, int dtype, hipStream_t stream) {
+  WindowAttnArgs a = args;
+  if (a.B == 0 || a.T == 0) return;
+  a.scale_log2 = a.scale * kLog2e;
+  const dim3 grid(static_cast<unsigned>(query_items(a)));
+  dispatch(dtype, a.D, [&](auto tr, auto d) {
+    constexpr int D = decltype(d)::value;
+    auto k = window_fwd_kernel<decltype(tr), D>;
+    allow_lds(k, kQueryLds<D>);
+    hipLaunchKernelGGL(k, grid, dim3(kThreads), kQueryLds<D>, stream, a);
+  });
+}
+
+void launch_window_attention_bwd(const WindowAttnArgs& args, int dtype, hipStream_t stream) {
+  WindowAttnArgs a = args;
+  if (a.B == 0 || a.T == 0) return;
+  a.scale_log2 = a.scale * kLog2e;
+  const dim3 grid(static_cast<unsigned>(query_items(a)));
+  dispatch(dtype, a.D, [&](auto tr, auto d) {
+    constexpr int D = decltype(d)::value;
+    using TR = decltype(tr);
+    auto dq = window_dq_kernel<TR, D>;
+    auto dkdv = window_dkdv_kernel<TR, D>;
+    auto join = window_join_kernel<TR, D>;
+    allow_lds(dq, kQueryLds<D>);
+    allow_lds(dkdv, kDkdvLds<D>);
+    hipLaunchKernelGGL(dq, grid, dim3(kThreads), kQueryLds<D>, stream, a);
+    hipLaunchKernelGGL(dkdv, dim3(static_cast<unsigned>(a.pieces)), dim3(kThreads), kDkdvLds<D>, stream, a);
+    if (a.pieces > 1) hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(a.pieces - 1)), dim3(kThreads), 4 * kStripBytes<D>, stream, a);
+  });
+}
+
+}  // namespace kernels
+}  // namespace dpa

@@ -4,6 +4,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <atomic>
 #include <tuple>
 
 #include "kernels/kernels.h"
@@ -1044,6 +1046,97 @@ std::tuple<Tensor, Tensor> attention_backward(Tensor d_o, Tensor qkv, Tensor o, 
   return {dqkv, dbias};
 }
 
+// ------------------------------------------------------------------ attention with a sliding window and sinks
+int compute_units_of(const Tensor& t) {
+  static std::atomic<int> known[64];
+  const int d = t.get_device();
+  int n = d < 64 ? known[d].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    TORCH_CHECK(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d) == hipSuccess && n > 0, "cannot read the device's compute units");
+    if (d < 64) known[d].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+kernels::WindowAttnArgs window_args(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, int64_t window, int64_t sinks, double scale,
+                                    const c10::optional<Tensor>& lens, const char* who) {
+  TORCH_CHECK(qkv.defined() && qkv.is_cuda() && qkv.dim() == 3, who, ": qkv must be a GPU tensor [B, T, (H + 2 KV) * D]");
+  TORCH_CHECK(n_head >= 1 && n_kv_head >= 1 && n_head % n_kv_head == 0, who, ": the query heads must be a multiple of the key / value heads");
+  const int64_t B = qkv.size(0), T = qkv.size(1), W = qkv.size(2), heads = n_head + 2 * n_kv_head;
+  TORCH_CHECK(W % heads == 0, who, ": the last dimension must be (n_head + 2 * n_kv_head) * head_dim");
+  const int64_t D = W / heads;
+  const bool one_row = T <= 1, one_batch = B <= 1;  // strides of dimensions of one entry mean nothing
+  const int64_t rs = one_row ? W : qkv.stride(1), bs = one_batch ? 0 : qkv.stride(0);
+  TORCH_CHECK(qkv.stride(2) == 1 && rs >= 0 && bs >= 0 && bs % 8 == 0 && reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0, who,
+              ": qkv needs contiguous rows on 16-byte boundaries");
+  TORCH_CHECK(kernels::window_attention_supported(B, T, n_head, n_kv_head, D, rs, kdtype(qkv)), who, ": needs bf16 / fp16 and head size 64 or 128 (got ",
+              qkv.scalar_type(), ", ", D, ")");
+  TORCH_CHECK(window >= 1 && sinks >= 0 && scale > 0.0, who, ": needs window >= 1, sinks >= 0 and a positive scale");
+  kernels::WindowAttnArgs a{};
+  if (lens.has_value() && lens->defined()) {
+    check_gpu(*lens, "seq_lens");
+    TORCH_CHECK(lens->scalar_type() == at::kInt && lens->dim() == 1 && lens->size(0) == B && lens->get_device() == qkv.get_device(), who,
+                ": seq_lens must be int32 [B] on the device of qkv");
+    a.lens = lens->data_ptr<int>();
+  }
+  a.qkv = qkv.data_ptr();
+  a.row_stride = rs;
+  a.batch_stride = bs;
+  a.B = static_cast<int>(B); a.T = static_cast<int>(T); a.H = static_cast<int>(n_head); a.KV = static_cast<int>(n_kv_head); a.D = static_cast<int>(D);
+  a.window = static_cast<int>(std::min<int64_t>(window, std::max<int64_t>(T, 1)));
+  a.sinks = static_cast<int>(std::min<int64_t>(sinks, T));
+  a.scale = static_cast<float>(scale);
+  return a;
+}
+
+// Returns (o [B, T, H * D], lse2 [B, H, T] or undefined).
+std::tuple<Tensor, Tensor> window_attention_forward(Tensor qkv, int64_t n_head, int64_t n_kv_head, int64_t window, int64_t sinks, double scale,
+                                                    c10::optional<Tensor> lens, bool want_stats) {
+  kernels::WindowAttnArgs a = window_args(qkv, n_head, n_kv_head, window, sinks, scale, lens, "window_attention_forward");
+  DevGuard guard(qkv);
+  Tensor o = at::empty({a.B, a.T, static_cast<int64_t>(a.H) * a.D}, qkv.options()), lse2;
+  if (want_stats) {
+    lse2 = at::empty({a.B, a.H, a.T}, qkv.options().dtype(at::kFloat));
+    a.lse2 = lse2.data_ptr<float>();
+  }
+  a.o = o.data_ptr();
+  kernels::launch_window_attention_fwd(a, kdtype(qkv), stream_of(qkv));
+  return {o, lse2};
+}
+
+// dqkv [B, T, (H + 2 KV) * D] from the forward's inputs and outputs and d_o [B, T, H * D].
+Tensor window_attention_backward(Tensor d_o, Tensor qkv, Tensor o, Tensor lse2, int64_t n_head, int64_t n_kv_head, int64_t window, int64_t sinks,
+                                 double scale, c10::optional<Tensor> lens) {
+  kernels::WindowAttnArgs a = window_args(qkv, n_head, n_kv_head, window, sinks, scale, lens, "window_attention_backward");
+  check_gpu(d_o, "d_o");
+  check_gpu(o, "o");
+  check_gpu(lse2, "lse2");
+  TORCH_CHECK(o.dim() == 3 && o.size(0) == a.B && o.size(1) == a.T && o.size(2) == static_cast<int64_t>(a.H) * a.D && d_o.sizes() == o.sizes() &&
+                  o.scalar_type() == qkv.scalar_type() && d_o.scalar_type() == qkv.scalar_type() && o.get_device() == qkv.get_device() &&
+                  d_o.get_device() == qkv.get_device() && reinterpret_cast<uintptr_t>(d_o.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
+              "window_attention_backward: o and d_o must be [B, T, H * D] like the forward's output");
+  TORCH_CHECK(lse2.scalar_type() == at::kFloat && lse2.numel() == static_cast<int64_t>(a.B) * a.H * a.T && lse2.get_device() == qkv.get_device(),
+              "window_attention_backward: lse2 must be float32 [B, H, T]");
+  DevGuard guard(qkv);
+  Tensor dqkv = at::empty({a.B, a.T, qkv.size(2)}, qkv.options());
+  Tensor delta = at::empty_like(lse2);
+  a.o = o.data_ptr();
+  a.d_o = d_o.data_ptr();
+  a.dqkv = dqkv.data_ptr();
+  a.lse2 = lse2.data_ptr<float>();
+  a.delta = delta.data_ptr<float>();
+  a.compute_units = compute_units_of(qkv);
+  a.pieces = kernels::window_attention_pieces(a);
+  Tensor partial;
+  if (const long long n = kernels::window_attention_partial_floats(a)) {
+    partial = at::empty({n}, lse2.options());
+    a.partial = partial.data_ptr<float>();
+  }
+  kernels::launch_window_attention_bwd(a, kdtype(qkv), stream_of(qkv));
+  return dqkv;
+}
+
 bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
 bool embedding_ok(const Tensor& idx, const Tensor& wte, const Tensor& wpe, int64_t T) {
@@ -1115,6 +1208,13 @@ void init_ops(py::module_& m) {
   m.def("dgrad_act_backward", &dgrad_act_backward, py::arg("dout"), py::arg("weight"), py::arg("aux"), py::arg("act"), py::arg("want_colsum"));
   m.def("dgrad_act_backward_supported", &dgrad_act_backward_supported);
   m.def("attention_supported", [](int64_t T, int64_t hd, int64_t rs) { return kernels::attention_supported(T, hd, rs); });
+  m.def("window_attention_supported", [](int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t row_stride, const std::string& dtype) {
+    return kernels::window_attention_supported(B, T, H, KV, D, row_stride, dtype == "bfloat16" ? kernels::kBF16 : dtype == "float16" ? kernels::kF16 : kernels::kF32);
+  });
+  m.def("window_attention_forward", &window_attention_forward, py::arg("qkv"), py::arg("n_head"), py::arg("n_kv_head"), py::arg("window"),
+        py::arg("sinks"), py::arg("scale"), py::arg("seq_lens") = py::none(), py::arg("want_stats") = true);
+  m.def("window_attention_backward", &window_attention_backward, py::arg("d_o"), py::arg("qkv"), py::arg("o"), py::arg("lse2"), py::arg("n_head"),
+        py::arg("n_kv_head"), py::arg("window"), py::arg("sinks"), py::arg("scale"), py::arg("seq_lens") = py::none());
   m.def("multi_copy_scale", &multi_copy_scale, py::arg("srcs"), py::arg("dsts"), py::arg("scale") = 1.0);
   m.def("scale_inplace", &scale_inplace);
   m.def("adamw_tick", &adamw_tick);

@@ -8,3 +8,4 @@ from .cross_entropy import SoftmaxCrossEntropy, softmax_cross_entropy  # noqa: F
 from .layernorm import LayerNorm  # noqa: F401
 from .linear import Linear, linear_bias_act  # noqa: F401
 from .rank1_mlp import rank1_mlp  # noqa: F401
+from .window_attention import window_attention_qkvpacked  # noqa: F401
