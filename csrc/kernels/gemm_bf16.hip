@@ -1281,26 +1281,23 @@ bool gemm_bf16_supported(const GemmArgs& a) {
   return tiles < (1ll << 31);
 }
 
-// Tile counters of the streaming (several tiles per workgroup) launches: a small ring of 16-byte slots
-// in the code object's own memory, one per launch in flight, zeroed on the launch's stream.
-__device__ unsigned g_tile_counters[256 * 8];  // one set of eight (a counter per XCD segment) per launch in flight
+// Compute units of the current device.
+int compute_units() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 0;
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
-struct StreamingSetup {
-  unsigned* counters = nullptr;
-  int cus = 0;
-  unsigned next_slot = 0;
-};
-StreamingSetup& streaming_setup() {
-  static StreamingSetup s = [] {
-    StreamingSetup t;
-    void* addr = nullptr;
-    if (hipGetSymbolAddress(&addr, HIP_SYMBOL(g_tile_counters)) == hipSuccess) t.counters = static_cast<unsigned*>(addr);
-    int dev = 0;
-    hipDeviceProp_t prop;
-    if (hipGetDevice(&dev) == hipSuccess && hipGetDeviceProperties(&prop, dev) == hipSuccess) t.cus = prop.multiProcessorCount;
-    return t;
-  }();
-  return s;
+// Zeroes the tile counters of a streaming launch (a kernel, because a captured memory-set node has given wrong results on
+// replays after the first).
+__global__ void clear_tile_counters_kernel(unsigned* counters) {
+  if (threadIdx.x < kTileCounters) counters[threadIdx.x] = 0u;
 }
 
 // Several tiles per workgroup pay off when a tile is short (few k-steps): the cold start and the
@@ -1315,8 +1312,8 @@ bool use_streaming(const GemmArgs& a, long long tiles, bool split) {
   // training step; the workgroups then wait for their aux tiles and stores together instead of being relaunched.)
   if (split || a.aux_mode != kActNone) return false;
   const long long nk = a.K / BK2;
-  const StreamingSetup& s = streaming_setup();
-  return s.counters != nullptr && s.cus > 0 && nk >= 3 && nk <= kStreamingMaxKSteps && tiles >= 3ll * s.cus;
+  const int cus = compute_units();
+  return cus >= 8 && nk >= 3 && nk <= kStreamingMaxKSteps && tiles >= 3ll * cus;
 }
 
 bool gemm_bf16_conv_supported(const GemmArgs& a) {
@@ -1352,6 +1349,11 @@ void ensure_gelu_tables(hipStream_t stream) {
   done.fetch_or(bit, std::memory_order_release);
 }
 
+bool gemm_bf16_wants_tile_counters(const GemmArgs& a) {
+  if (a.split_k > 1 || a.conv_mode == 2 || !use_large_tile(a)) return false;
+  return use_streaming(a, ((a.M + BM2 - 1) / BM2) * ((a.N + BN2 - 1) / BN2), false);
+}
+
 void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream) {
   if (a.act == kActGelu || a.aux_mode == kActGelu) ensure_gelu_tables(stream);
   const bool split = (a.split_k > 1 || a.conv_mode == 2) && a.workspace != nullptr;
@@ -1364,11 +1366,10 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream) {
     const long long tiles = static_cast<long long>(tm2) * tn2;
     unsigned* counter = nullptr;
     unsigned grid_x = static_cast<unsigned>(tiles);
-    if (use_streaming(a, tiles, split)) {
-      StreamingSetup& s = streaming_setup();
-      counter = s.counters + 8 * (s.next_slot++ & 255u);
-      (void)hipMemsetAsync(counter, 0, 32, stream);
-      grid_x = static_cast<unsigned>(s.cus) & ~7u;  // the same number of workgroups on every XCD
+    if (a.tile_counters != nullptr && use_streaming(a, tiles, split)) {
+      counter = a.tile_counters;
+      hipLaunchKernelGGL(clear_tile_counters_kernel, dim3(1), dim3(64), 0, stream, counter);
+      grid_x = static_cast<unsigned>(compute_units()) & ~7u;  // the same number of workgroups on every XCD
 #ifdef GEMM_GRID_OVERRIDE  // experiment (tools/kernel_harness): fewer workgroups than CUs
       grid_x = GEMM_GRID_OVERRIDE;
 #endif

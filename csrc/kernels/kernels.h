@@ -159,6 +159,9 @@ struct GemmArgs {
   // gemm_bf16_split_k(); zero / nullptr means a single pass.
   float* workspace;
   int split_k;
+  // kTileCounters values of device memory that belong to this launch alone until it has run (the bf16 kernel that walks several
+  // tiles per workgroup draws tile ids from them; see gemm_bf16_wants_tile_counters).  nullptr: one tile per workgroup.
+  unsigned* tile_counters;
   // Activation-backward epilogue (bf16, 256x256-tile kernel, M and N multiples of 256, no bias /
   // act / pre_act / beta): C = (alpha*acc) * act'(aux) with aux [M,N] at leading dimension ldc --
   // the pre-activation for GELU (aux_mode = kActGelu), the activation output for ReLU
@@ -181,6 +184,8 @@ struct GemmArgs {
 // Number of contraction ranges worth using for this product (1 = do not split): > 1 when the
 // output has too few 256x256 tiles to occupy the chip but a long contraction (weight gradients).
 int gemm_bf16_split_k(const GemmArgs& a);
+constexpr int kTileCounters = 8;
+bool gemm_bf16_wants_tile_counters(const GemmArgs& a);
 bool gemm_bf16_act_backward_supported(const GemmArgs& a);
 bool gemm_f32_supported(const GemmArgs& a);
 void launch_gemm_f32(const GemmArgs& a, hipStream_t stream);

@@ -526,6 +526,15 @@ bool gemm_path_ok(const kernels::GemmArgs& a, int dt) {
                              : (dt == kernels::kBF16 ? kernels::gemm_bf16_supported(a) : (dt == kernels::kF16 ? kernels::gemm_f16_supported(a) : false));
 }
 
+// Device memory for the tile ids of a bf16 launch that walks several tiles per workgroup.  From the caching allocator, so that it is the
+// launch's own on whatever stream, device or graph capture it runs in; hold it until the launch has been made.
+Tensor tile_counters_for(kernels::GemmArgs& a, const Tensor& like) {
+  if (!kernels::gemm_bf16_wants_tile_counters(a)) return Tensor();
+  Tensor t = at::empty({kernels::kTileCounters}, like.options().dtype(at::kInt));
+  a.tile_counters = reinterpret_cast<unsigned*>(t.data_ptr<int>());
+  return t;
+}
+
 // `like` supplies the device for the split-K workspace (fp32 partials, caching allocator).
 void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& like) {
   if (dt == kernels::kF32) {
@@ -545,7 +554,9 @@ void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& l
     kernels::launch_gemm_bf16(b, s);
     return;
   }
-  kernels::launch_gemm_bf16(a, s);
+  kernels::GemmArgs b = a;
+  const Tensor counters = tile_counters_for(b, like);
+  kernels::launch_gemm_bf16(b, s);
 }
 
 // Whether the MFMA GEMMs take C[M,N] = op(A) op(B)^T with contiguous operands in the given layouts.
@@ -845,6 +856,7 @@ Tensor conv3x3_forward(Tensor xpad, Tensor w, int64_t B, int64_t H, int64_t W) {
   a.conv_mode = 1; a.conv_B = static_cast<int>(B); a.conv_H = static_cast<int>(H); a.conv_W = static_cast<int>(W); a.conv_C = static_cast<int>(g.C);
   TORCH_CHECK(kernels::gemm_bf16_conv_supported(a), "conv3x3_forward: unsupported geometry B=", B, " H=", H, " W=", W, " C=", g.C, " N=", N);
   DevGuard guard(xpad);
+  const Tensor counters = tile_counters_for(a, xpad);
   kernels::launch_gemm_bf16(a, stream_of(xpad));
   return y;
 }

@@ -45,6 +45,7 @@ int main(int argc, char** argv) {
   hipMalloc(&times, kTimeBytes); hipMemset(times, 0, kTimeBytes);
   a.colsum_partial = reinterpret_cast<float*>(times);
 #endif
+  hipMalloc(&a.tile_counters, dpa::kernels::kTileCounters * sizeof(unsigned));
   hipEvent_t e0, e1; hipEventCreate(&e0); hipEventCreate(&e1);
   for (int i = 0; i < 3; ++i) dpa::kernels::launch_gemm_bf16(a, 0);
   float ms;

@@ -136,7 +136,10 @@ static int check_one(long long M, long long N, long long K, int ak, int bk, int 
   return (bad || nondet) ? 1 : 0;
 }
 
-static double time_fn(const GemmArgs& a, int which, int iters) {
+static double time_fn(GemmArgs a, int which, int iters) {
+  static unsigned* counters = nullptr;
+  if (!counters) CK(hipMalloc(&counters, dpa::kernels::kTileCounters * sizeof(unsigned)));
+  a.tile_counters = counters;
   hipEvent_t e0, e1; CK(hipEventCreate(&e0)); CK(hipEventCreate(&e1));
   CK(hipEventRecord(e0));
   for (int i = 0; i < iters; ++i) {
