@@ -90,6 +90,92 @@ __device__ __forceinline__ void store_tile_bf16(const GemmArgs& p, const f32x4& 
   }
 }
 
+// Gated pair of projections (GemmArgs::gate).  The gate's and the up projection's rows of the weight are interleaved 16 by 16
+// on their way into a tile: row v of the product's N dimension is row (v >> 5) * 16 + (v & 15) of the gate (bit 4 of v clear) or of the
+// up projection (set).  Neighbouring accumulator tiles of a wave then hold g and u of the same elements in the same registers, and the
+// product of the two needs no exchange between lanes.
+__device__ __forceinline__ long long gate_row(long long v) { return ((v >> 5) << 4) + (v & 15); }
+
+// h and (when wanted) g | u of four consecutive columns col .. col + 3 of one row, out of accumulators that hold no bias yet.
+template <typename TR, int ACT>
+__device__ __forceinline__ void store_gate_fwd(const GemmArgs& p, const f32x4& ag, const f32x4& au, long long row, long long col) {
+  const long long H = p.gate_H;
+  if (row >= p.M || col >= H) return;
+  u16* C = static_cast<u16*>(p.C) + row * p.ldc;
+  u16* P = p.pre_act ? static_cast<u16*>(p.pre_act) + row * 2 * H : nullptr;
+  const u16* bias = static_cast<const u16*>(p.bias);
+  u16x4 h, gr, ur;
+  const int n = H - col < 4 ? static_cast<int>(H - col) : 4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float g = ag[e], u = au[e];
+    if (bias && e < n) {
+      g += TR::to_f32(bias[col + e]);
+      u += TR::to_f32(bias[H + col + e]);
+    }
+    h[e] = TR::from_f32(gate_value<ACT>(g) * u);
+    gr[e] = TR::from_f32(g);
+    ur[e] = TR::from_f32(u);
+  }
+  if (n == 4 && (H & 3) == 0 && (p.ldc & 3) == 0) {  // (outputs start on 16-byte boundaries)
+    *reinterpret_cast<u16x4*>(C + col) = h;
+    if (P) {
+      *reinterpret_cast<u16x4*>(P + col) = gr;
+      *reinterpret_cast<u16x4*>(P + H + col) = ur;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= n) break;
+      C[col + e] = h[e];
+      if (P) {
+        P[col + e] = gr[e];
+        P[H + col + e] = ur[e];
+      }
+    }
+  }
+}
+
+// dg | du of four consecutive columns of one row from their dh.
+template <typename TR, int ACT>
+__device__ __forceinline__ void store_gate_bwd(const GemmArgs& p, const f32x4& dh, long long row, long long col) {
+  const long long H = p.gate_H;
+  if (row >= p.M || col >= H) return;
+  const u16* GU = static_cast<const u16*>(p.aux) + row * 2 * H + col;
+  u16* C = static_cast<u16*>(p.C) + row * p.ldc + col;
+  const int n = H - col < 4 ? static_cast<int>(H - col) : 4;
+  const bool whole = n == 4 && (H & 3) == 0;
+  u16x4 g4, u4, dg, du;
+  if (whole) {
+    g4 = *reinterpret_cast<const u16x4*>(GU);
+    u4 = *reinterpret_cast<const u16x4*>(GU + H);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g4[e] = e < n ? GU[e] : static_cast<u16>(0);
+      u4[e] = e < n ? GU[H + e] : static_cast<u16>(0);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float value, slope;
+    gate_value_and_slope<ACT>(TR::to_f32(g4[e]), value, slope);
+    dg[e] = TR::from_f32(dh[e] * TR::to_f32(u4[e]) * slope);
+    du[e] = TR::from_f32(dh[e] * value);
+  }
+  if (whole) {
+    *reinterpret_cast<u16x4*>(C) = dg;
+    *reinterpret_cast<u16x4*>(C + H) = du;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= n) break;
+      C[e] = dg[e];
+      C[H + e] = du[e];
+    }
+  }
+}
+
 // Byte offset of 16-byte chunk c (8 k-values) of `row` in the swizzled [128][64] image.
 __device__ __forceinline__ int kmajor_off(int row, int c) { return row * 128 + ((c ^ ((row >> 1) & 7)) << 4); }
 // Byte offset of 16-byte chunk c (8 rows) of contraction index k in the swizzled [64][128] image.
@@ -99,14 +185,31 @@ __device__ __forceinline__ int rmajor_off(int k, int c) { return k * 256 + ((c ^
 // address, leading dimension and contiguous extent are multiples of 8 elements): one 16-byte load per piece.
 // Otherwise (odd extents, leading dimensions or base addresses) the piece is gathered element by element with a
 // bounds check each -- the tail path that lets every shape run here; it costs load instructions, not correctness.
-template <bool KMAJOR, bool ALIGNED>
+// PAIRED: the rows are the interleaved ones of a gated pair of R rows each (see gate_row).
+template <bool KMAJOR, bool ALIGNED, bool PAIRED = false>
 __device__ __forceinline__ void load_tile(const u16* __restrict__ base, long long ld, long long r0, long long R, long long k0,
                                           long long K, u32x4 (&regs)[4]) {
+  static_assert(!PAIRED || KMAJOR, "a gated pair is stored with the contraction index contiguous");
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int id = threadIdx.x + i * kThreads;
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (KMAJOR) {
+    if (PAIRED) {
+      const long long vr = r0 + (id >> 3), h = gate_row(vr), k = k0 + ((id & 7) << 3);
+      if (h < R && k < K) {
+        const u16* src = base + (h + (vr & 16 ? R : 0)) * ld + k;
+        if (ALIGNED) {
+          v = *reinterpret_cast<const u32x4*>(src);
+        } else {
+          const int n = K - k < 8 ? static_cast<int>(K - k) : 8;
+          unsigned short e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = j < n ? src[j] : static_cast<unsigned short>(0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = static_cast<unsigned>(e[2 * j]) | (static_cast<unsigned>(e[2 * j + 1]) << 16);
+        }
+      }
+    } else if (KMAJOR) {
       const long long row = r0 + (id >> 3), k = k0 + ((id & 7) << 3);
       if (ALIGNED) {
         if (row < R && k < K) v = *reinterpret_cast<const u32x4*>(base + row * ld + k);
@@ -168,7 +271,8 @@ __device__ __forceinline__ bf16x8 read_frag(const char* lds, int tile_row0, int 
 }
 
 // TR = BF16 or F16: the two 16-bit types share everything but the MFMA opcode and the epilogue's conversions.
-template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED, typename TR>
+// GATE / GACT: GemmArgs::gate with its activation.
+template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED, typename TR, int GATE = 0, int GACT = kActNone>
 __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(16))) char smem_bf16[];
 
@@ -193,7 +297,8 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
   u32x4 ra[4], rb[4];
   const long long nk = (p.K + BK - 1) / BK;
   load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, 0, p.K, ra);
-  load_tile<B_KMAJOR, ALIGNED>(B, p.ldb, n0, p.N, 0, p.K, rb);
+  const long long b_rows = GATE == 1 ? p.gate_H : p.N;
+  load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, 0, p.K, rb);
   store_tile<A_KMAJOR>(smem_bf16, ra);
   store_tile<B_KMAJOR>(smem_bf16 + kTileBytes, rb);
   __syncthreads();
@@ -203,7 +308,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
     const bool more = kt + 1 < nk;
     if (more) {
       load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, (kt + 1) * BK, p.K, ra);
-      load_tile<B_KMAJOR, ALIGNED>(B, p.ldb, n0, p.N, (kt + 1) * BK, p.K, rb);
+      load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, (kt + 1) * BK, p.K, rb);
     }
     const char* as = smem_bf16 + cur * 2 * kTileBytes;
     const char* bs = as + kTileBytes;
@@ -236,11 +341,20 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
   }
 
   // Epilogue (operands were swapped in the MFMA: see store_tile_bf16).
+  if constexpr (GATE == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        store_gate_fwd<TR, GACT>(p, acc[i][2 * j], acc[i][2 * j + 1], m0 + wm + 16 * i + (lane & 15), gate_row(n0 + wn + 32 * j) + 4 * (lane >> 4));
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      store_tile_bf16<TR>(p, acc[i][j], m0 + wm + 16 * i + (lane & 15), n0 + wn + 16 * j + 4 * (lane >> 4));
+      if constexpr (GATE == 2) store_gate_bwd<TR, GACT>(p, acc[i][j], m0 + wm + 16 * i + (lane & 15), n0 + wn + 16 * j + 4 * (lane >> 4));
+      else store_tile_bf16<TR>(p, acc[i][j], m0 + wm + 16 * i + (lane & 15), n0 + wn + 16 * j + 4 * (lane >> 4));
 }
 
 // =====================================================================================
@@ -366,6 +480,24 @@ __device__ __forceinline__ void dma_offsets(long long ld, long long r0, long lon
         rel = rel < lim ? rel : lim;
         off[h][i] = static_cast<unsigned>(k) * ld2 + rel * 2u;
       }
+    }
+}
+// The same for the interleaved rows of a gated pair (see gate_row): tile-relative row v is row h of the gate or of the up projection, which
+// begins gate_H rows further.
+__device__ __forceinline__ void dma_offsets_gate(const GemmArgs& p, long long n0, int wid, int lane, unsigned (&off)[2][2]) {
+  const unsigned ld2 = static_cast<unsigned>(p.ldb) * 2u, up = static_cast<unsigned>(p.gate_H) * ld2;
+  const long long room = p.gate_H - (n0 >> 1) - 1;
+  const unsigned lim = static_cast<unsigned>(room < 127 ? room : 127);
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lr = (wid * 2 + i) * 8 + (lane >> 3);
+      const int c = (lane & 7) ^ ((lr >> 1) & 7);
+      const unsigned rel = static_cast<unsigned>((lr / 32) * 64 + h * 32 + lr % 32);
+      unsigned row = (rel >> 5) * 16u + (rel & 15u);
+      row = row < lim ? row : lim;
+      off[h][i] = row * ld2 + (rel & 16u ? up : 0u) + static_cast<unsigned>(c * 16);
     }
 }
 // Base of the tile for k-step starting at k0 (wave-uniform).
@@ -537,11 +669,14 @@ constexpr int kStreamingMaxKSteps = 64;  // beyond K = 4096 a tile is long enoug
 // 2 = operand B is that view for the weight gradient (split-K TN layout).  See GemmArgs::conv_mode.
 // ACTBWD: the activation-backward epilogue (GemmArgs::aux); an instantiation of its own, so that the plain products do
 // not carry its code and registers (as a run-time branch it cost the NT forward kernel 8 spilled registers).
-template <bool A_KMAJOR, bool B_KMAJOR, bool SPLIT, int CONV = 0, bool ACTBWD = false>
+// GATE / GACT: GemmArgs::gate with its activation (1: interleaved B rows and a product epilogue, streaming like the plain kernel; 2: an
+// epilogue like the activation-backward one, with two tensors in and two out).
+template <bool A_KMAJOR, bool B_KMAJOR, bool SPLIT, int CONV = 0, bool ACTBWD = false, int GATE = 0, int GACT = kActNone>
 __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p, int tiles_m, int tiles_n, int k_iters, unsigned* tile_counter) {
   static_assert(CONV == 0 || (CONV == 1 && A_KMAJOR && B_KMAJOR && !SPLIT) || (CONV == 2 && !A_KMAJOR && !B_KMAJOR && SPLIT),
                 "convolution views exist for the NT forward product and the split-K TN weight gradient");
   static_assert(!ACTBWD || (!SPLIT && CONV == 0), "the activation-backward epilogue belongs to the plain single-pass product");
+  static_assert(GATE == 0 || (!SPLIT && CONV == 0 && !ACTBWD && A_KMAJOR && B_KMAJOR == (GATE == 1)), "gated pairs: NT forward, NN backward");
   extern __shared__ __attribute__((aligned(16))) char smem2[];  // [2 k-steps][B0 | A0 | B1 | A1][GELU table][staging][control]
   DPA_STAMP(0);
   DPA_STAMP_REAL(4);
@@ -587,7 +722,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
   const int wr = wid >> 2, wc = wid & 3;
   const int wm = wr * 128, wn = wc * 64;
   const unsigned lds_base = static_cast<unsigned>(reinterpret_cast<uintptr_t>((lptr_t)smem2));
-  if (!SPLIT && (ACTBWD ? p.aux_mode == kActGelu : p.act == kActGelu)) {
+  if (!SPLIT && GATE == 0 && (ACTBWD ? p.aux_mode == kActGelu : p.act == kActGelu)) {
     // backward epilogue: GELU'(x); forward epilogue: Phi(x), so that GELU(x) = x * table[x].  15 pieces of 1 KiB, two
     // per wave: older than every operand request, so the prologue's counted wait and barrier publish them as well.
     const char* src = reinterpret_cast<const char*>(g_gelu_tables[ACTBWD ? 1 : 0]);
@@ -642,6 +777,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
     if constexpr (CONV == 1) dma_offsets_conv_a(p, rm0, wid, l, off_a);
     else dma_offsets<A_KMAJOR, 64>(p.lda, rm0, p.M, wid, l, off_a);
     if constexpr (CONV == 2) dma_offsets_conv_b(p, rn0, wid, l, off_b);
+    else if constexpr (GATE == 1) dma_offsets_gate(p, rn0, wid, l, off_b);
     else dma_offsets<B_KMAJOR, 32>(p.ldb, rn0, p.N, wid, l, off_b);
   };
   // CONV == 1: the A base does not depend on the tile; it walks 128 bytes per k-step through the 3*C contiguous
@@ -663,7 +799,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       // k-step kt0 of X, shifted up by the (W + 3) rows that dma_offsets_conv_b adds back per column
       r_bptr = uniform_ptr(reinterpret_cast<const char*>(B + (kt0 * BK2 - (p.conv_W + 3)) * p.conv_C));
     } else {
-      r_bptr = uniform_ptr(dma_base<B_KMAJOR>(B, p.ldb, rn0, kt0 * BK2));
+      r_bptr = uniform_ptr(dma_base<B_KMAJOR>(B, p.ldb, GATE == 1 ? rn0 >> 1 : rn0, kt0 * BK2));
     }
   };
   // Requests the next half-tile of the stream; `which` runs B0 A0 B1 A1 B0 ... by construction of the callers.
@@ -738,12 +874,13 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
   // so its latency hides behind that step's MFMAs; the second half follows once the operand buffers are
   // dead.  LDS position (lane & 7) of row (lane >> 3) receives chunk (lane & 7) ^ (lane >> 3) of the row
   // (XOR on the source address), which spreads the accumulator-layout reads of the epilogue over the banks.
-  constexpr bool act_bwd = ACTBWD;
+  constexpr bool act_bwd = ACTBWD || GATE == 2;  // (an epilogue that takes the operand buffers over)
   long long m0, n0;  // origin of the tile being multiplied
-  auto aux_request = [&](int half, int buf) __attribute__((always_inline)) {
+  bool whole_tile = true;  // GATE == 2: the tile lies inside the matrix
+  auto aux_request = [&](int half, int buf, long long col = 0) __attribute__((always_inline)) {
     const int al = fresh_lane();
     const unsigned aux_off = static_cast<unsigned>(((al >> 3) * p.ldc + (((al & 7) ^ (al >> 3)) << 3)) * 2);
-    const char* src = uniform_ptr(reinterpret_cast<const char*>(static_cast<const u16*>(p.aux) + (m0 + wm + 64 * half) * p.ldc + n0 + wn));
+    const char* src = uniform_ptr(reinterpret_cast<const char*>(static_cast<const u16*>(p.aux) + (m0 + wm + 64 * half) * p.ldc + n0 + wn + col));
     const unsigned dst0 = lds_base + buf * 2 * kTileBytes2 + wid * 8192;
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
@@ -761,11 +898,12 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
   // in flight, so that wait (and the barrier behind it) publishes them like an operand tile.
   auto bias_request = [&](long long bn0) __attribute__((always_inline)) {
     if (wid != 0) return;
-    const char* base = uniform_ptr(reinterpret_cast<const char*>(static_cast<const u16*>(p.bias) + bn0));
+    const char* base = uniform_ptr(reinterpret_cast<const char*>(static_cast<const u16*>(p.bias) + (GATE == 1 ? bn0 >> 1 : bn0)));
     const unsigned voff = static_cast<unsigned>(fresh_lane() * 4);
     const unsigned dst = lds_base + kBiasOff;
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(base), "s"(dst) : "memory");
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(base + 256), "s"(dst + 256) : "memory");
+    const char* second = GATE == 1 ? uniform_ptr(base + p.gate_H * 2) : base + 256;  // the up projection's 128 values / the next 128 columns
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(second), "s"(dst + 256) : "memory");
   };
 
   // One k-step = four phases; each phase is {fragment reads + one half-tile request | barrier | 16 MFMAs |
@@ -806,8 +944,9 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       tile_origin(nxt, bm0, bn0);
       if (bn0 + BN2 <= p.N) bias_request(bn0);
     }
-    if (LAST && act_bwd) aux_request(0, c_buf ^ 1);
-    else if (FIRST ? !a1_ahead : (!LAST || r_valid)) request(A1);
+    if (LAST && act_bwd) {
+      if (GATE != 2 || whole_tile) aux_request(0, c_buf ^ 1);
+    } else if (FIRST ? !a1_ahead : (!LAST || r_valid)) request(A1);
     if (PENULT) {
       if (nxt < ntiles) set_cursor(nxt);
       else r_valid = false;
@@ -833,7 +972,9 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
     // phase 4
     if (!(PENULT || LAST) || r_valid) {
       request(B1);
-      if (FIRST && a1_ahead && ahead_stores == 16) asm volatile("s_waitcnt vmcnt(22)" ::: "memory");
+      if (GATE == 1 && FIRST && a1_ahead && ahead_stores == 8) asm volatile("s_waitcnt vmcnt(14)" ::: "memory");
+      else if (GATE == 1 && FIRST && a1_ahead && ahead_stores == 24) asm volatile("s_waitcnt vmcnt(30)" ::: "memory");
+      else if (FIRST && a1_ahead && ahead_stores == 16) asm volatile("s_waitcnt vmcnt(22)" ::: "memory");
       else if (FIRST && a1_ahead && ahead_stores == 32) asm volatile("s_waitcnt vmcnt(38)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
     } else if (!(LAST && act_bwd)) {
@@ -901,6 +1042,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
     tile_origin(cur, m0, n0);
     // Full interior tiles of a plain product leave through the LDS-staged epilogue below (with the bias
     // already in the accumulators); everything else through the element-wise one.
+    if (GATE == 2) whole_tile = m0 + BM2 <= p.M && n0 + BN2 <= p.N;
     const bool staged = !SPLIT && p.beta == 0.f && p.alpha == 1.f && m0 + BM2 <= p.M && n0 + BN2 <= p.N && (p.ldc & 7) == 0 &&
                         ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.pre_act)) & 15) == 0;
     if (staged && p.bias != nullptr) {
@@ -908,7 +1050,8 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       const int bias_lane = fresh_lane();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u16x4 raw = *(lds_u16x4_cptr)(lds_base + kBiasOff + (wn + 16 * j + 4 * (bias_lane >> 4)) * 2);
+        const int at = GATE == 1 ? (j & 1) * 128 + (wn >> 1) + 16 * (j >> 1) : wn + 16 * j;
+        const u16x4 raw = *(lds_u16x4_cptr)(lds_base + kBiasOff + (at + 4 * (bias_lane >> 4)) * 2);
         f32x4 b;
 #pragma unroll
         for (int e = 0; e < 4; ++e) b[e] = BF16::to_f32(raw[e]);
@@ -966,7 +1109,213 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
     // reads) and writes 8 rows x 128 contiguous bytes per store instruction.  Bias and activation are
     // applied in registers first.  The strips lie outside the operand buffers, which already receive the
     // next tile.
-    if (staged && act_bwd) {
+    if constexpr (GATE == 2) {
+      if (!whole_tile) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            store_gate_bwd<BF16, GACT>(p, acc[i][j], m0 + wm + 16 * i + (lane & 15), n0 + wn + 16 * j + 4 * (lane >> 4));
+            __builtin_amdgcn_sched_barrier(0);  // or the loads of all 32 pieces come first and spill
+          }
+        return;
+      }
+      // Both inputs of the epilogue arrive like the aux tile of the activation-backward one below: this wave's 128 x 64 piece in halves of 64
+      // rows, g into the buffer that the last k-step left idle (requested during that step), u into the other one once everybody is done
+      // with it.  A lane replaces g and u under its accumulators by dg and du, and whole 128-byte row pieces leave.  An image's second
+      // half is requested as soon as the first half's results are in registers, ahead of their stores.
+      phase_barrier();  // every wave has finished reading the operand buffers
+      const int last = c_buf ^ 1, idle = c_buf;
+      char* const img_g = smem2 + idle * 2 * kTileBytes2 + wid * 8192;
+      char* const img_u = smem2 + last * 2 * kTileBytes2 + wid * 8192;
+      const long long H = p.gate_H;
+      aux_request(0, last, H);
+      const int el = fresh_lane();
+      const int r = el & 15, g = el >> 4;
+      float cg[4][4] = {}, cu[4][4] = {};  // this lane's sums over its rows (bias gradient)
+      auto process = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ii = 0; ii < 4; ++ii) {
+          int cell[4];
+          u16x4 gx[4], ux[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            cell[j] = (16 * ii + r) * 128 + (((2 * j + (g >> 1)) ^ (r & 7)) << 4) + 8 * (g & 1);
+            gx[j] = *reinterpret_cast<const u16x4*>(img_g + cell[j]);
+            ux[j] = *reinterpret_cast<const u16x4*>(img_u + cell[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4& a = acc[4 * half + ii][j];
+            u16x4 dg, du;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float value, slope;
+              gate_value_and_slope<GACT>(BF16::to_f32(gx[j][e]), value, slope);
+              dg[e] = BF16::from_f32(a[e] * BF16::to_f32(ux[j][e]) * slope);
+              du[e] = BF16::from_f32(a[e] * value);
+              cg[j][e] += BF16::to_f32(dg[e]);
+              cu[j][e] += BF16::to_f32(du[e]);
+            }
+            *reinterpret_cast<u16x4*>(img_g + cell[j]) = dg;  // same lane, same cell
+            *reinterpret_cast<u16x4*>(img_u + cell[j]) = du;
+          }
+          // The sums are taken here, not behind the branch that uses them: sunk there, every value added up stays live and spills.
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(cg[j][e]), "+v"(cu[j][e]));
+          __builtin_amdgcn_sched_barrier(0);  // one row of cells at a time: interleaved, the four rows' values do not fit the registers
+        }
+      };
+      // One image's 64 rows into registers; its refill (`next`) is requested ahead of the stores.
+      auto drain = [&](const char* img, int half, long long col, auto next) __attribute__((always_inline)) {
+        u32x4 v[8];
+#pragma unroll
+        for (int it = 0; it < 8; ++it) v[it] = *reinterpret_cast<const u32x4*>(img + (8 * it + (el >> 3)) * 128 + (el & 7) * 16);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        next();
+        u16* out = static_cast<u16*>(p.C) + (m0 + wm + 64 * half + (el >> 3)) * p.ldc + n0 + wn + ((el & 7) ^ (el >> 3)) * 8 + col;
+#pragma unroll
+        for (int it = 0; it < 8; ++it) __builtin_nontemporal_store(v[it], reinterpret_cast<u32x4*>(out + static_cast<long long>(8 * it) * p.ldc));
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      process(0);
+      drain(img_g, 0, 0, [&]() __attribute__((always_inline)) { aux_request(1, idle); });
+      drain(img_u, 0, H, [&]() __attribute__((always_inline)) { aux_request(1, last, H); });
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // everything but the stores behind the last request
+      process(1);
+      drain(img_g, 1, 0, []() {});
+      drain(img_u, 1, H, []() {});
+      if (p.colsum_partial != nullptr) {
+        auto rot = [](float v, auto n_c) __attribute__((always_inline)) {
+          constexpr int ctrl = 0x120 + decltype(n_c)::value;  // row_ror:n
+          return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, false));
+        };
+        auto total = [&](float v) __attribute__((always_inline)) {
+          v += rot(v, std::integral_constant<int, 8>{});
+          v += rot(v, std::integral_constant<int, 4>{});
+          v += rot(v, std::integral_constant<int, 2>{});
+          return v + rot(v, std::integral_constant<int, 1>{});
+        };
+        float* dst = p.colsum_partial + (2 * (m0 / BM2) + wr) * 2 * H + n0 + wn + 4 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4 og, ou;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            og[e] = total(cg[j][e]);
+            ou[e] = total(cu[j][e]);
+          }
+          if (r == 0) {
+            *reinterpret_cast<f32x4*>(dst + 16 * j) = og;
+            *reinterpret_cast<f32x4*>(dst + 16 * j + H) = ou;
+          }
+        }
+      }
+      return;
+    }
+    if constexpr (GATE == 1) {
+      if (!staged) {
+        ahead_stores = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            store_gate_fwd<BF16, GACT>(p, acc[i][2 * j], acc[i][2 * j + 1], m0 + wm + 16 * i + (lane & 15), gate_row(n0 + wn + 32 * j) + 4 * (lane >> 4));
+      } else {
+        // The wave's 128 x 32 outputs (and 128 x 32 of g and of u) leave through its 2 KiB strip like the plain epilogue's below: a pass writes 16
+        // rows of 128 bytes -- g | u of 16 rows, or h of 32 rows side by side -- and reads them back as 16-byte pieces of 64-byte row
+        // segments.  Row r of the strip swaps the halves of its chunks for r >= 8.
+        using lds_u16x4_ptr = __attribute__((address_space(3))) u16x4*;
+        using lds_u32x4_ptr = const __attribute__((address_space(3))) u32x4*;
+        const int l = fresh_lane();
+        const int r = l & 15, g = l >> 4;
+        const unsigned mine = lds_base + kStageOff + wid * 2048;
+        const unsigned wr_addr = mine + r * 128 + 8 * ((g & 1) ^ (r >> 3));
+        const unsigned rd_addr = mine + (l >> 3) * 128 + (l & 7) * 16;
+        const int chunk = (l & 7) ^ (l >> 3);  // of the row piece this lane reads back
+        const long long H = p.gate_H, col = (n0 >> 1) + (wn >> 1) + (chunk & 3) * 8, row = m0 + wm + (l >> 3);
+        u16* const h_out = static_cast<u16*>(p.C) + (row + (chunk >> 2) * 16) * p.ldc + col;
+        u16* const p_out = p.pre_act ? static_cast<u16*>(p.pre_act) + row * 2 * H + col + (chunk >> 2) * H : nullptr;
+        auto put = [&](int c2, const u16x4& o) __attribute__((always_inline)) {  // 16-column group c2 (0 .. 3) of the strip's rows
+          *(lds_u16x4_ptr)(wr_addr + (((2 * c2 + (g >> 1)) ^ (r & 7)) << 4)) = o;
+        };
+        auto pre_pass = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            u16x4 o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = BF16::from_f32(acc[i][j][e]);
+            put((j & 1) * 2 + (j >> 1), o);
+          }
+        };
+        auto h_pass = [&](int i) __attribute__((always_inline)) {  // rows of tiles 2 i and 2 i + 1
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              u16x4 o;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[e] = BF16::from_f32(gate_value<GACT>(acc[2 * i + t][2 * j][e]) * acc[2 * i + t][2 * j + 1][e]);
+              put(2 * t + j, o);
+            }
+        };
+        auto read_rows = [&](u32x4 (&v)[2]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int it = 0; it < 2; ++it) v[it] = *(lds_u32x4_ptr)(rd_addr + it * 1024);
+        };
+        auto store = [&](u16* out, long long pitch, const u32x4 (&v)[2]) __attribute__((always_inline)) {
+          __builtin_nontemporal_store(v[0], reinterpret_cast<u32x4*>(out));
+          __builtin_nontemporal_store(u32x4{v[1][2], v[1][3], v[1][0], v[1][1]}, reinterpret_cast<u32x4*>(out + 8 * pitch));
+        };
+        u32x4 v[2][2];
+        if (p_out) {
+          // passes: g | u of tile 2 i, of tile 2 i + 1, h of both
+          auto write = [&](auto q_c) __attribute__((always_inline)) {
+            constexpr int q = decltype(q_c)::value;
+            if constexpr (q % 3 == 2) h_pass(q / 3);
+            else pre_pass(2 * (q / 3) + q % 3);
+          };
+          auto emit = [&](auto q_c) __attribute__((always_inline)) {
+            constexpr int q = decltype(q_c)::value;
+            if constexpr (q + 1 < 12) {
+              write(std::integral_constant<int, q + 1>{});
+              read_rows(v[(q + 1) & 1]);
+            }
+            if constexpr (q % 3 == 2) store(h_out + static_cast<long long>(32 * (q / 3)) * p.ldc, p.ldc, v[q & 1]);
+            else store(p_out + static_cast<long long>(16 * (2 * (q / 3) + q % 3)) * 2 * H, 2 * H, v[q & 1]);
+          };
+          write(std::integral_constant<int, 0>{});
+          read_rows(v[0]);
+          emit(std::integral_constant<int, 0>{});
+          emit(std::integral_constant<int, 1>{});
+          emit(std::integral_constant<int, 2>{});
+          emit(std::integral_constant<int, 3>{});
+          emit(std::integral_constant<int, 4>{});
+          emit(std::integral_constant<int, 5>{});
+          emit(std::integral_constant<int, 6>{});
+          emit(std::integral_constant<int, 7>{});
+          emit(std::integral_constant<int, 8>{});
+          emit(std::integral_constant<int, 9>{});
+          emit(std::integral_constant<int, 10>{});
+          emit(std::integral_constant<int, 11>{});
+        } else {
+          h_pass(0);
+          read_rows(v[0]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i + 1 < 4) {
+              h_pass(i + 1);
+              read_rows(v[(i + 1) & 1]);
+            }
+            store(h_out + static_cast<long long>(32 * i) * p.ldc, p.ldc, v[i & 1]);
+          }
+        }
+        ahead_stores = p_out ? 24 : 8;
+      }
+    } else if (staged && act_bwd) {
       // Activation-backward epilogue: C = (alpha*acc) * act'(aux).  Each lane picks the aux values
       // that sit under its accumulators out of the DMA image, writes the result back into the same
       // cells, and the rows then leave as 8 rows x 128 contiguous bytes per store instruction -- so
@@ -1073,7 +1422,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       DPA_TILE_TIME(1);
       return;
     }
-    if (staged) {
+    if (GATE == 0 && staged) {
       using lds_u16x4_ptr = __attribute__((address_space(3))) u16x4*;
       using lds_u32x4_ptr = const __attribute__((address_space(3))) u32x4*;
       const int l = fresh_lane();  // the epilogue's lane constants are derived here, not kept from the top of the kernel
@@ -1173,7 +1522,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       else if (p.act == kActRelu) emit_all(std::integral_constant<int, kActRelu>{});
       else emit_all(std::integral_constant<int, kActNone>{});
       ahead_stores = p.pre_act ? 32 : 16;
-    } else {
+    } else if (GATE == 0) {
       ahead_stores = 0;  // ragged tile: an unknown number of stores, the next wait covers them all
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -1310,7 +1659,7 @@ bool use_streaming(const GemmArgs& a, long long tiles, bool split) {
   // well -- next tile's id drawn during the k-steps, its first two k-steps requested from inside the epilogue as the
   // buffers fall free -- was built and measured: 2152 -> 2120 us standalone on 393216 x 3072 x 768, nothing in the
   // training step; the workgroups then wait for their aux tiles and stores together instead of being relaunched.)
-  if (split || a.aux_mode != kActNone) return false;
+  if (split || a.aux_mode != kActNone || a.gate == 2) return false;
   const long long nk = a.K / BK2;
   const int cus = compute_units();
   return cus >= 8 && nk >= 3 && nk <= kStreamingMaxKSteps && tiles >= 3ll * cus;
@@ -1349,8 +1698,80 @@ void ensure_gelu_tables(hipStream_t stream) {
   done.fetch_or(bit, std::memory_order_release);
 }
 
+// The 256x256 kernel's gated forms: 16-byte row pieces of both halves of g | u, 32-bit byte offsets from a tile's first gate row to its last
+// row of the up projection.
+static bool gate_large(const GemmArgs& a, int dtype) {
+  if (dtype != kBF16 || !use_large_tile(a) || a.gate_H % 8 != 0 || a.ldc % 8 != 0 || !aligned16(a.C)) return false;
+  if (a.gate == 1) return (a.gate_H + 128) * a.ldb * 2 < (1ll << 32) && aligned16(a.pre_act) && reinterpret_cast<uintptr_t>(a.bias) % 4 == 0;
+  return aligned16(a.aux);
+}
+
+bool gemm_gate_supported(const GemmArgs& a, int dtype) {
+  if (dtype != kBF16 && dtype != kF16) return false;
+  if (a.act != kActRelu && a.act != kActGelu && a.act != kActSilu) return false;
+  if (a.gate_H <= 0 || a.gate_H >= (1ll << 30)) return false;
+  // 8-byte accesses of the epilogues where H is a multiple of 4
+  if (reinterpret_cast<uintptr_t>(a.C) % 8 || reinterpret_cast<uintptr_t>(a.pre_act) % 8 || reinterpret_cast<uintptr_t>(a.aux) % 8) return false;
+  if (a.gate == 1) return a.a_kmajor && a.b_kmajor && a.N == 2 * a.gate_H && a.ldc == a.gate_H && gemm_bf16_supported(a);
+  return a.gate == 2 && a.a_kmajor && !a.b_kmajor && a.N == a.gate_H && a.ldc == 2 * a.gate_H && a.aux != nullptr && gemm_bf16_supported(a);
+}
+
+long long gemm_gate_colsum_rows(const GemmArgs& a, int dtype) {
+  return a.gate == 2 && gate_large(a, dtype) && a.M % BM2 == 0 && a.N % BN2 == 0 ? 2 * (a.M / BM2) : 0;
+}
+
+void launch_gemm_gate(const GemmArgs& a, int dtype, hipStream_t stream) {
+  auto with_act = [&](auto&& f) {
+    if (a.act == kActSilu) f(std::integral_constant<int, kActSilu>{});
+    else if (a.act == kActGelu) f(std::integral_constant<int, kActGelu>{});
+    else f(std::integral_constant<int, kActRelu>{});
+  };
+  if (gate_large(a, dtype)) {
+    const int tm = static_cast<int>((a.M + BM2 - 1) / BM2), tn = static_cast<int>((a.N + BN2 - 1) / BN2);
+    const long long tiles = static_cast<long long>(tm) * tn;
+    unsigned* counter = nullptr;
+    unsigned grid = static_cast<unsigned>(tiles);
+    if (a.tile_counters != nullptr && use_streaming(a, tiles, false)) {
+      counter = a.tile_counters;
+      hipLaunchKernelGGL(clear_tile_counters_kernel, dim3(1), dim3(64), 0, stream, counter);
+      grid = static_cast<unsigned>(compute_units()) & ~7u;
+    }
+    with_act([&](auto act_c) {
+      constexpr int ACT = decltype(act_c)::value;
+      auto go = [&](auto kernel) {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes2);
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads2), kLdsBytes2, stream, a, tm, tn, static_cast<int>(a.K / BK2), counter);
+      };
+      if (a.gate == 1) go(gemm_bf16_8ph_kernel<true, true, false, 0, false, 1, ACT>);
+      else go(gemm_bf16_8ph_kernel<true, false, false, 0, false, 2, ACT>);
+    });
+    return;
+  }
+  // a paired tile of 128 rows holds 64 of either half
+  const int tiles_m = static_cast<int>((a.M + BM - 1) / BM);
+  const int tiles_n = static_cast<int>(a.gate == 1 ? (a.gate_H + 63) / 64 : (a.N + BN - 1) / BN);
+  const dim3 grid(static_cast<unsigned>(tiles_m) * static_cast<unsigned>(tiles_n));
+  const bool vec = gemm_bf16_vector_aligned(a);
+  with_act([&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    auto typed = [&](auto tr) {
+      using TR = decltype(tr);
+      auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 4 * kTileBytes, stream, a, tiles_m, tiles_n); };
+      if (a.gate == 1) {
+        if (vec) go(gemm_bf16_kernel<true, true, true, TR, 1, ACT>);
+        else go(gemm_bf16_kernel<true, true, false, TR, 1, ACT>);
+      } else {
+        if (vec) go(gemm_bf16_kernel<true, false, true, TR, 2, ACT>);
+        else go(gemm_bf16_kernel<true, false, false, TR, 2, ACT>);
+      }
+    };
+    if (dtype == kF16) typed(F16{});
+    else typed(BF16{});
+  });
+}
+
 bool gemm_bf16_wants_tile_counters(const GemmArgs& a) {
-  if (a.split_k > 1 || a.conv_mode == 2 || !use_large_tile(a)) return false;
+  if (a.split_k > 1 || a.conv_mode == 2 || (a.gate == 0 ? !use_large_tile(a) : !gate_large(a, kBF16))) return false;
   return use_streaming(a, ((a.M + BM2 - 1) / BM2) * ((a.N + BN2 - 1) / BN2), false);
 }
 

@@ -132,7 +132,7 @@ void launch_distill_reduce(const float* row_loss, const unsigned char* correct, 
 void launch_distill_apply_upstream(void* x, int dtype, long long n, const float* g, hipStream_t stream);
 
 // ------------------------------------------------------------------ dense layers
-enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2 };
+enum Act : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };  // (SiLU: as a gate only)
 
 // C[M,N] = act(A * B^T + bias) style products on the matrix cores.  Layout flags say which
 // dimension of each operand is contiguous:  a_kmajor: A is [M,K] row-major (K contiguous),
@@ -180,6 +180,13 @@ struct GemmArgs {
   //     channel c.  B points to X row 0; (W + 3) rows before and after it must be readable zeros.  N = 9*C, ldb = C.
   int conv_mode;
   int conv_B, conv_H, conv_W, conv_C;
+  // Gated pair of projections (bf16 / fp16; act = kActSilu, kActGelu or kActRelu):
+  //   gate 1 (forward, NT layout): B = W [2 H, K], the gate's rows before the up projection's; C = act(g) * u with g | u = A B^T + bias,
+  //     [M, H] at ldc; pre_act, when given, receives g | u as [M, 2 H].  N = 2 H is what the product computes.
+  //   gate 2 (backward, NN layout): dh = A B with B = W_out [K, H]; aux = g | u [M, 2 H]; C receives dh u act'(g) | dh act(g), [M, 2 H] at
+  //     ldc = 2 H.  N = H.  colsum_partial, when given (gemm_gate_colsum_rows() rows of 2 H), receives sums over the rows of C.
+  int gate;
+  long long gate_H;
 };
 // Number of contraction ranges worth using for this product (1 = do not split): > 1 when the
 // output has too few 256x256 tiles to occupy the chip but a long contraction (weight gradients).
@@ -196,6 +203,13 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream);
 // fp16 storage (fp32 accumulate) on the 128x128 MFMA kernel; same argument conventions.
 bool gemm_f16_supported(const GemmArgs& a);
 void launch_gemm_f16(const GemmArgs& a, hipStream_t stream);
+// GemmArgs::gate 1 / 2 in `dtype` (kBF16 or kF16); any extents, odd ones included.
+bool gemm_gate_supported(const GemmArgs& a, int dtype);
+long long gemm_gate_colsum_rows(const GemmArgs& a, int dtype);  // 0: this launch takes no column sums
+void launch_gemm_gate(const GemmArgs& a, int dtype, hipStream_t stream);
+// The same on float32 (or any) products that exist already: h = act(g) * u; dgu = dh u act'(g) | dh act(g).
+void launch_gate_fwd(const void* gu, void* h, long long M, long long H, int dtype, int act, hipStream_t stream);
+void launch_gate_bwd(const void* dh, const void* gu, void* dgu, long long M, long long H, int dtype, int act, hipStream_t stream);
 
 // dst [rows_total][C] (bf16, 16-byte aligned): row guard_front + q is haloed pixel q of x [B][H][W][C] -- zero on the
 // one-pixel frame of every image -- and every row outside [guard_front, guard_front + B*(H+2)*(W+2)) is zero.

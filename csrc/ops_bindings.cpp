@@ -618,6 +618,103 @@ std::tuple<Tensor, c10::optional<Tensor>> linear_forward(Tensor x, Tensor w, c10
   return {y, pre};
 }
 
+// ------------------------------------------------------------------ gated pair of projections
+// h [M, H] = act(g) * u with g | u = x W^T + b; W [2 H, K] holds the gate's rows before the up projection's.  Returns (h, g | u [M, 2 H] or
+// None).  act: ACT_SILU, ACT_GELU or ACT_RELU.
+std::tuple<Tensor, c10::optional<Tensor>> gated_forward(Tensor x, Tensor w, c10::optional<Tensor> bias, int64_t act, bool save) {
+  check_gpu(x, "x");
+  check_gpu(w, "weight");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && w.size(0) % 2 == 0 && w.size(0) > 0 && w.size(1) > 0,
+              "gated_forward: x [M, K] and weight [2 H, K] expected");
+  TORCH_CHECK(x.scalar_type() == w.scalar_type() && x.get_device() == w.get_device(), "gated_forward: x and weight differ in dtype or device");
+  TORCH_CHECK(act == kernels::kActSilu || act == kernels::kActGelu || act == kernels::kActRelu, "gated_forward: act must be silu, gelu or relu");
+  const int64_t M = x.size(0), K = x.size(1), H = w.size(0) / 2;
+  const int dt = kdtype(x);
+  DevGuard guard(x);
+  hipStream_t s = stream_of(x);
+  if (dt == kernels::kF32) {
+    Tensor gu = std::get<0>(linear_forward(x, w, bias, kernels::kActNone, false));
+    Tensor h = at::empty({M, H}, x.options());
+    kernels::launch_gate_fwd(gu.data_ptr(), h.data_ptr(), M, H, dt, static_cast<int>(act), s);
+    return {h, save ? c10::optional<Tensor>(gu) : c10::nullopt};
+  }
+  kernels::GemmArgs a{};
+  if (bias.has_value() && bias->defined()) {
+    check_gpu(*bias, "bias");
+    TORCH_CHECK(bias->numel() == 2 * H && bias->scalar_type() == w.scalar_type() && bias->get_device() == w.get_device(),
+                "gated_forward: bias must be [2 H] like the weight");
+    a.bias = bias->data_ptr();
+  }
+  Tensor h = at::empty({M, H}, x.options());
+  c10::optional<Tensor> gu;
+  if (save) gu = at::empty({M, 2 * H}, x.options());
+  if (M == 0) return {h, gu};
+  a.A = x.data_ptr(); a.B = w.data_ptr(); a.C = h.data_ptr();
+  a.pre_act = save ? gu->data_ptr() : nullptr;
+  a.M = M; a.N = 2 * H; a.K = K; a.lda = K; a.ldb = K; a.ldc = H;
+  a.a_kmajor = 1; a.b_kmajor = 1; a.act = static_cast<int>(act); a.alpha = 1.f; a.gate = 1; a.gate_H = H;
+  TORCH_CHECK(kernels::gemm_gate_supported(a, dt), "gated_forward: shape M=", M, " H=", H, " K=", K, " is not supported");
+  const Tensor counters = dt == kernels::kBF16 ? tile_counters_for(a, x) : Tensor();
+  kernels::launch_gemm_gate(a, dt, s);
+  return {h, gu};
+}
+
+// g | u's gradient [M, 2 H] from dy [M, N], the output projection W [N, H] and the saved g | u; with want_db also its column sums (the bias gradient).
+std::tuple<Tensor, c10::optional<Tensor>> gated_backward(Tensor dy, Tensor w, Tensor gu, int64_t act, bool want_db) {
+  check_gpu(dy, "dy");
+  check_gpu(w, "weight");
+  check_gpu(gu, "gu");
+  TORCH_CHECK(dy.dim() == 2 && w.dim() == 2 && gu.dim() == 2 && dy.size(1) == w.size(0) && gu.size(0) == dy.size(0) && gu.size(1) == 2 * w.size(1),
+              "gated_backward: dy [M, N], weight [N, H] and gu [M, 2 H] expected");
+  TORCH_CHECK(dy.scalar_type() == w.scalar_type() && gu.scalar_type() == w.scalar_type() && dy.get_device() == w.get_device() &&
+                  gu.get_device() == w.get_device(),
+              "gated_backward: tensors differ in dtype or device");
+  TORCH_CHECK(act == kernels::kActSilu || act == kernels::kActGelu || act == kernels::kActRelu, "gated_backward: act must be silu, gelu or relu");
+  const int64_t M = dy.size(0), N = dy.size(1), H = w.size(1);
+  const int dt = kdtype(dy);
+  DevGuard guard(dy);
+  hipStream_t s = stream_of(dy);
+  Tensor dgu = at::empty({M, 2 * H}, dy.options());
+  c10::optional<Tensor> db;
+  if (want_db) db = at::empty({2 * H}, dy.options());
+  if (M == 0) {
+    if (want_db) db->zero_();
+    return {dgu, db};
+  }
+  kernels::GemmArgs a{};
+  a.A = dy.data_ptr(); a.B = w.data_ptr();
+  a.M = M; a.N = H; a.K = N; a.lda = N; a.ldb = H; a.a_kmajor = 1; a.b_kmajor = 0; a.alpha = 1.f;
+  Tensor partial;
+  long long sums = 0;
+  if (dt == kernels::kF32) {
+    Tensor dh = at::empty({M, H}, dy.options());
+    a.C = dh.data_ptr();
+    a.ldc = H;
+    TORCH_CHECK(gemm_path_ok(a, dt), "gated_backward: shape M=", M, " N=", N, " H=", H, " is not supported");
+    run_gemm(a, dt, s, dy);
+    kernels::launch_gate_bwd(dh.data_ptr(), gu.data_ptr(), dgu.data_ptr(), M, H, dt, static_cast<int>(act), s);
+  } else {
+    a.C = dgu.data_ptr();
+    a.ldc = 2 * H;
+    a.aux = gu.data_ptr();
+    a.act = static_cast<int>(act); a.gate = 2; a.gate_H = H;
+    TORCH_CHECK(kernels::gemm_gate_supported(a, dt), "gated_backward: shape M=", M, " N=", N, " H=", H, " is not supported");
+    sums = want_db ? kernels::gemm_gate_colsum_rows(a, dt) : 0;
+    if (sums > 0) {
+      partial = at::empty({sums, 2 * H}, dy.options().dtype(at::kFloat));
+      a.colsum_partial = partial.data_ptr<float>();
+    }
+    kernels::launch_gemm_gate(a, dt, s);
+  }
+  if (sums > 0) {
+    kernels::launch_reduce_partials(partial.data_ptr<float>(), db->data_ptr(), 2 * H, static_cast<int>(sums), dt, s);
+  } else if (want_db) {
+    Tensor ws = at::empty({kernels::colreduce_workspace(M, 2 * H)}, dy.options().dtype(at::kFloat));
+    kernels::launch_colsum(dgu.data_ptr(), db->data_ptr(), ws.data_ptr<float>(), M, 2 * H, dt, s);
+  }
+  return {dgu, db};
+}
+
 // ------------------------------------------------------------------ Linear(1,H) -> act -> Linear(H,N<=16), fused
 namespace {
 const void* opt_ptr(const c10::optional<Tensor>& t, const Tensor& like, int64_t numel, const char* what) {
@@ -1249,6 +1346,8 @@ void init_ops(py::module_& m) {
         py::arg("dw_out") = py::none());
   m.def("rank1_mlp_forward", &rank1_mlp_forward, py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("b2"), py::arg("act") = 0);
   m.def("rank1_mlp_backward", &rank1_mlp_backward, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("act") = 0);
+  m.def("gated_forward", &gated_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("save") = true);
+  m.def("gated_backward", &gated_backward, py::arg("dy"), py::arg("weight"), py::arg("gu"), py::arg("act"), py::arg("want_db") = false);
   m.def("act_backward", &act_backward, py::arg("dy"), py::arg("saved"), py::arg("act"), py::arg("need_db") = false);
   m.def("colsum", &colsum);
   m.def("conv3x3_pad", &conv3x3_pad, py::arg("x_nhwc"));
@@ -1273,4 +1372,5 @@ void init_ops(py::module_& m) {
   m.attr("ACT_NONE") = static_cast<int>(kernels::kActNone);
   m.attr("ACT_RELU") = static_cast<int>(kernels::kActRelu);
   m.attr("ACT_GELU") = static_cast<int>(kernels::kActGelu);
+  m.attr("ACT_SILU") = static_cast<int>(kernels::kActSilu);
 }

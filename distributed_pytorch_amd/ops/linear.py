@@ -18,7 +18,7 @@ import torch.nn.functional as F
 from .. import _ext
 from .grad_sink import weight_grad_buffer
 
-ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3  # (SiLU: as the gate of mlp.gated_mlp only)
 _ACT_CODES = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "gelu": ACT_GELU}
 
 
