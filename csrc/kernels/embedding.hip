@@ -142,6 +142,13 @@ __global__ __launch_bounds__(kTokThreads) void embed_bwd_tok_join_kernel(const l
   }
 }
 
+// -1: no long run starts in the chunk.  (A kernel, not a memory set: captured into a graph, the latter has given wrong results on
+// replays after the first.)
+__global__ __launch_bounds__(256) void embed_no_runs_kernel(long long* head_tok, long long chunks) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < chunks) head_tok[i] = -1;
+}
+
 }  // namespace
 
 bool embedding_supported(long long rows, long long T, long long C, long long V, long long P) {
@@ -168,7 +175,7 @@ void launch_embedding_bwd(const void* grad, const long long* tok_sorted, const l
   hipLaunchKernelGGL(embed_bwd_pos_kernel, dim3(static_cast<unsigned>((per_batch + kEmbedThreads - 1) / kEmbedThreads)), dim3(kEmbedThreads),
                      0, stream, static_cast<const u32x4*>(grad), static_cast<u32x4*>(dwpe), B, per_batch);
   const long long chunks = embedding_bwd_chunks(rows);
-  (void)hipMemsetAsync(head_tok, 0xFF, static_cast<size_t>(chunks) * sizeof(long long), stream);  // -1: no long run starts in the chunk
+  hipLaunchKernelGGL(embed_no_runs_kernel, dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, stream, head_tok, chunks);
   hipLaunchKernelGGL(embed_bwd_tok_kernel, dim3(static_cast<unsigned>(rows)), dim3(kTokThreads), 0, stream, tok_sorted, perm,
                      static_cast<const u32x4*>(grad), static_cast<u32x4*>(dwte), rows, vpr, V, head_part, body_part, head_tok);
   hipLaunchKernelGGL(embed_bwd_tok_join_kernel, dim3(static_cast<unsigned>(chunks)), dim3(kTokThreads), 0, stream, tok_sorted,
