@@ -10,9 +10,10 @@
 //
 // One workgroup per row.  The row is read once: every thread keeps its 16-byte vectors packed in registers through the
 // maximum, the two sums of exponentials and the gradient, so a fused call moves exactly one read and one write of the
-// logits (rows too wide for the registers are read again, out of L2 / Infinity Cache).  With one temperature in play (tau = 1, a = 0 or a = 1) there is one
-// exponential per element and pass, otherwise two (DUAL).
-// The K teacher entries are a scatter into the row.  A vector that is about to be stored has to know its entries: LDS
+// logits (rows too wide for the registers are read again, out of L2 / Infinity Cache).  With one temperature in play (tau = 1, a = 0
+// or a = 1) there is one exponential per element and pass; otherwise the one at temperature 1 is a power of the other where tau is 2 or 4,
+// and a second exponential for other tau (an exponential takes four issue slots, a power one or two).
+// The K teacher entries (and the label, as one more) are a scatter into the row.  A vector that is about to be stored has to know its entries: LDS
 // holds one bit per vector (a wave's 64 vectors are one 64-bit word, so most waves skip the look-up on a scalar
 // branch) and a chained hash from vector to entries.  Entries of one class are summed beforehand in index order by the
 // first of them, which makes the result independent of the order in which the chains were built.
@@ -29,7 +30,7 @@ namespace kernels {
 namespace {
 
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kNone = 0x7fffffff;
 enum Mode : int { kForward = 0, kBackward = 1, kFused = 2 };
 
@@ -48,21 +49,24 @@ __device__ __forceinline__ float teacher_at(const DistillArgs& a, long long i) {
   return a.teacher_dtype == kBF16 ? BF16::to_f32(raw) : F16::to_f32(raw);
 }
 
-// THREADS x KEEP 16-byte vectors are held in registers (KEEP = 0: none, every pass reads memory).
-template <typename TR, int THREADS, int KEEP, int MODE, bool DUAL, int WAVES_PER_SIMD>
+// THREADS x KEEP 16-byte vectors are held in registers (KEEP = 0: none, every pass reads memory).  SECOND: how the exponentials at
+// temperature 1 come about when both temperatures are needed -- 0: they are not, 1: by an exponential of their own, 2 / 4: as the square /
+// fourth power of those at temperature 2 / 4.
+template <typename TR, int THREADS, int KEEP, int MODE, int SECOND, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(DistillArgs a) {
   using T = typename TR::T;
   constexpr int V = TR::kVec, NW = THREADS / 64;
   constexpr bool GRAD = MODE != kForward;
   static_assert(KEEP == 0 || MODE != kBackward, "the backward reads every vector once");
-  extern __shared__ int s_dyn[];  // ids[K] | p[K] | x[K] | next[K] | head[hash] | bits[2 * words]
-  __shared__ float s_m[NW], s_s[NW], s_s1[NW], s_teacher[2], s_xy;
-  __shared__ int s_arg[NW], s_best;
+  extern __shared__ int s_dyn[];  // ids[K + 1] | p[K + 1] | x[K + 1] | next[K + 1] | head[hash] | bits[2 * words]
+  __shared__ float s_m[NW], s_s[NW], s_s1[NW], s_b, s_xy;
+  __shared__ int s_arg[NW], s_some, s_first;
+  const int entries = a.K + 1;  // the hard label is the last entry
   int* const s_id = s_dyn;
-  float* const s_p = reinterpret_cast<float*>(s_dyn + a.K);
-  float* const s_x = s_p + a.K;
-  int* const s_next = s_dyn + 3 * a.K;
-  int* const s_head = s_next + a.K;
+  float* const s_p = reinterpret_cast<float*>(s_dyn + entries);
+  float* const s_x = s_p + entries;
+  int* const s_next = s_dyn + 3 * entries;
+  int* const s_head = s_next + entries;
   unsigned* const s_bits = reinterpret_cast<unsigned*>(s_head + a.hash);
 
   const long long r = blockIdx.x;
@@ -76,7 +80,7 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
   const long long target = a.targets ? a.targets[r] : -1;
   const bool ignored = a.targets && (target == a.ignore_index || target < 0 || target >= C);
 
-  auto store_vec = [&](int k, const float (&d)[V]) {
+  auto store_vec = [&](int k, const float (&d)[V]) __attribute__((always_inline)) {
     const int j0 = k * V - shift;
     T* out = reinterpret_cast<T*>(grid_out + 16u * static_cast<unsigned>(k));
     if (j0 >= 0 && j0 + V <= ld) {
@@ -110,13 +114,18 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
       if (k < nvec) kept[q] = load_vec(k);
     }
   }
-  // One pass over the row's vectors: f(k, packed vector).
+  // One pass over the row's vectors: f(k, packed vector).  WHOLE tells vectors of nothing but classes from those at the row's ends.
   auto each_vec = [&](auto&& f) __attribute__((always_inline)) {
+    auto one = [&](int k, const raw16& v) __attribute__((always_inline)) {
+      const int j0 = k * V - shift;
+      if (j0 >= 0 && j0 + V <= C) f(k, v, std::true_type{});
+      else f(k, v, std::false_type{});
+    };
     if constexpr (KEEP > 0) {
 #pragma unroll
       for (int q = 0; q < KEEP; ++q) {
         const int k = tid + q * THREADS;
-        if (k < nvec) f(k, kept[q]);
+        if (k < nvec) one(k, kept[q]);
         __builtin_amdgcn_sched_barrier(0);  // one vector at a time: interleaved, the expansions of all of them would be live at once
       }
       // opaque between the passes, or the compiler keeps the fp32 expansions of one pass for the next and spills
@@ -125,12 +134,14 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     } else {
       for (int k = tid; k < nvec; k += THREADS) {
         raw16 v = *reinterpret_cast<const raw16*>(grid_in + 16u * static_cast<unsigned>(k));
-        f(k, v);
+        one(k, v);
       }
     }
   };
+  // Element j of a vector outside the classes?
+  auto outside = [&](int k, int j) { const int at = k * V - shift + j; return at < 0 || at >= C; };
 
-  // ---- the teacher's entries: ids, scaled logits, the student's logits at those classes
+  // ---- the teacher's entries: ids, scaled logits, the student's logits at those classes; the label behind them
   if (GRAD) {
     for (int i = tid; i < a.hash; i += THREADS) s_head[i] = -1;
     for (int i = tid; i < a.words * 2; i += THREADS) s_bits[i] = 0u;
@@ -145,10 +156,13 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     s_p[k] = t;
     if (MODE != kBackward) s_x[k] = there ? TR::to_f32(row[id]) : 0.f;
   }
-  if (MODE != kBackward && tid == 0) s_xy = a.targets ? TR::to_f32(row[target]) : 0.f;
+  if (tid == 0) {
+    s_id[a.K] = a.hard_weight != 0.f ? static_cast<int>(target) : -1;
+    if (MODE != kBackward) s_xy = a.targets ? TR::to_f32(row[target]) : 0.f;
+  }
   __syncthreads();
   if (GRAD) {
-    for (int k = tid; k < a.K; k += THREADS) {
+    for (int k = tid; k < entries; k += THREADS) {
       const int id = s_id[k];
       if (id < 0) continue;
       const int vec = (id + shift) / V;
@@ -157,61 +171,80 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     }
   }
 
-  // ---- row maximum (lowest index among equals)
-  float m, ls, ls1 = 0.f;
+  // ---- row maximum: of whole vectors, three values an instruction; which element it is, only its owners look up
+  const float c = a.exp_scale;  // log2(e) / temperature of the first exponential
+  float m, mt = kNegInf, S = 0.f, S1 = 0.f;
+  int best = kNone;
   if (MODE == kBackward) {
     m = a.row_stats[3 * r];
-    ls = a.row_stats[3 * r + 1];
-    ls1 = a.row_stats[3 * r + 2];
+    S = a.row_stats[3 * r + 1];
+    S1 = a.row_stats[3 * r + 2];
   } else {
-    m = kNegInf;
-    int arg = kNone;
-    each_vec([&](int k, const raw16& v) __attribute__((always_inline)) {
+    each_vec([&](int k, const raw16& v, auto whole) __attribute__((always_inline)) {
       float x[V];
       raw_to_f32<TR, V>(v, x);
-      const int j0 = k * V - shift;
-      if (j0 >= 0 && j0 + V <= C) {
+      float vm = kNegInf;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (x[j] > m) { m = x[j]; arg = j0 + j; }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j0 + j >= 0 && j0 + j < C && x[j] > m) { m = x[j]; arg = j0 + j; }
-      }
+      for (int j = 0; j < V; ++j) vm = fmaxf(vm, decltype(whole)::value || !outside(k, j) ? x[j] : kNegInf);
+      if (vm > mt) { mt = vm; best = k; }
     });
+    m = mt;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const float om = __shfl_xor(m, off, 64);
-      const int oa = __shfl_xor(arg, off, 64);
-      if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
-    }
-    if (lane == 0) { s_m[wid] = m; s_arg[wid] = arg; }
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    if (lane == 0) s_m[wid] = m;
     __syncthreads();
     m = s_m[0];
-    arg = s_arg[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w)
-      if (s_m[w] > m || (s_m[w] == m && s_arg[w] < arg)) { m = s_m[w]; arg = s_arg[w]; }
-    if (tid == 0) s_best = arg;  // read by the same thread only
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w]);
+  }
+  // Exponents are fma(x, c, -mc): the rounding of mc is the same in every term and in the sums, so it cancels wherever the same mc is used.
+  const float mc = m * c, mc1 = m * kLog2e;
+  auto second = [&](float x, float e) __attribute__((always_inline)) {
+    if (SECOND == 1) return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -mc1));
+    const float e2 = e * e;
+    return SECOND == 2 ? e2 : e2 * e2;
+  };
+  if (MODE != kBackward) {
+    int arg = kNone;
+    if (__any(mt == m)) {
+      if (mt == m) {
+        raw16 v = raw16{0u, 0u, 0u, 0u};
+        if constexpr (KEEP > 0) {
+#pragma unroll
+          for (int q = 0; q < KEEP; ++q)
+            if (best == tid + q * THREADS) v = kept[q];
+        } else {
+          if (best != kNone) v = *reinterpret_cast<const raw16*>(grid_in + 16u * static_cast<unsigned>(best));
+        }
+        float x[V];
+        raw_to_f32<TR, V>(v, x);
+#pragma unroll
+        for (int j = V - 1; j >= 0; --j)
+          if (best != kNone && x[j] == m && !outside(best, j)) arg = best * V - shift + j;
+      }
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) {
+        const int oa = __shfl_xor(arg, off, 64);
+        arg = oa < arg ? oa : arg;
+      }
+    }
+    if (lane == 0) s_arg[wid] = arg;
 
     // ---- sums of exponentials at both temperatures
     float s = 0.f, s1 = 0.f;
-    const float c = a.exp_scale;
-    each_vec([&](int k, const raw16& v) __attribute__((always_inline)) {
+    each_vec([&](int k, const raw16& v, auto whole) __attribute__((always_inline)) {
       float x[V];
       raw_to_f32<TR, V>(v, x);
-      const int j0 = k * V - shift;
-      const bool full = j0 >= 0 && j0 + V <= C;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const bool in = full || (j0 + j >= 0 && j0 + j < C);
-        s += in ? __builtin_amdgcn_exp2f((x[j] - m) * c) : 0.f;
-        if (DUAL) s1 += in ? __builtin_amdgcn_exp2f((x[j] - m) * kLog2e) : 0.f;
+        if (!decltype(whole)::value && outside(k, j)) x[j] = kNegInf;
+        const float e = __builtin_amdgcn_exp2f(fmaf(x[j], c, -mc));
+        s += e;
+        if (SECOND) s1 += second(x[j], e);
       }
     });
     s = wave_sum(s);
-    if (DUAL) s1 = wave_sum(s1);
+    if (SECOND) s1 = wave_sum(s1);
     if (lane == 0) { s_s[wid] = s; s_s1[wid] = s1; }
   }
   if (MODE == kBackward) __syncthreads();  // the chains are complete
@@ -219,68 +252,72 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
   // ---- one wave turns the teacher's logits into probabilities
   if (wid == 0) {
     float tm = kNegInf;
-    int best = kNone;  // first entry with the largest logit
+    int first = kNone;  // first entry with the largest logit
     for (int k = lane; k < a.K; k += 64)
-      if (s_id[k] >= 0 && !(s_p[k] <= tm)) { tm = s_p[k]; best = k; }
+      if (s_id[k] >= 0 && !(s_p[k] <= tm)) { tm = s_p[k]; first = k; }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
       const float om = __shfl_xor(tm, off, 64);
-      const int ob = __shfl_xor(best, off, 64);
-      if (om > tm || (om == tm && ob < best)) { tm = om; best = ob; }
+      const int ob = __shfl_xor(first, off, 64);
+      if (om > tm || (om == tm && ob < first)) { tm = om; first = ob; }
     }
-    const bool some = best != kNone;
     float z = 0.f;
     for (int k = lane; k < a.K; k += 64)
       if (s_id[k] >= 0) z += __builtin_amdgcn_exp2f((s_p[k] - tm) * kLog2e);
     z = wave_sum(z);
     const float log_z = logf(z), inv_z = 1.f / z;
-    float b = 0.f;  // sum_k p_k (log p_k - (x_k - m) / tau); with log(sum) added it is the divergence
+    float b = 0.f;  // sum_k p_k (log p_k - log(exponential of x_k)); with log(sum) added it is the divergence
     for (int k = lane; k < a.K; k += 64) {
       if (s_id[k] < 0) continue;
       const float t = s_p[k] - tm;
       const float p = __builtin_amdgcn_exp2f(t * kLog2e) * inv_z;
-      if (MODE != kBackward && !(p == 0.f)) b += p * ((t - log_z) - (s_x[k] - m) * a.inv_tau);
-      s_p[k] = p;
+      if (MODE != kBackward && !(p == 0.f)) b += p * ((t - log_z) - fmaf(s_x[k], c, -mc) * kLn2);
+      s_p[k] = p * (a.soft_weight * a.tau);  // its share of the gradient
     }
+    if (lane == 0) s_p[a.K] = a.hard_weight;
     b = wave_sum(b);
     if (GRAD) {
-      // p summed over the entries of one class, kept by the first of them: s_x[k]
-      for (int k = lane; k < a.K; k += 64) {
+      // shares of the entries of one class, added up by the first of them: s_x[k]
+      for (int k = lane; k < entries; k += 64) {
         const int id = s_id[k];
         if (id < 0) continue;
-        bool first = true, alone = true;
+        bool leads = true, alone = true;
         for (int e = s_head[((id + shift) / V) & (a.hash - 1)]; e >= 0; e = s_next[e])
           if (e != k && s_id[e] == id) {
             alone = false;
-            first = first && k < e;
+            leads = leads && k < e;
           }
         float p = s_p[k];
-        if (!alone && first)
-          for (int e = k + 1; e < a.K; ++e) p += s_id[e] == id ? s_p[e] : 0.f;
-        s_x[k] = first ? p : 0.f;
+        if (!alone && leads)
+          for (int e = k + 1; e < entries; ++e) p += s_id[e] == id ? s_p[e] : 0.f;
+        s_x[k] = leads ? p : 0.f;
       }
     }
     if (lane == 0) {
-      s_teacher[0] = some ? 1.f : 0.f;
-      s_teacher[1] = b;
-      if (MODE != kBackward && !a.targets && some) s_best = s_best == s_id[best] ? 1 : 0;  // (agreement with the teacher's first choice)
-      else if (MODE != kBackward) s_best = a.targets && s_best == target ? 1 : 0;
+      s_some = first != kNone;
+      s_first = first != kNone ? s_id[first] : -1;
+      s_b = b;
     }
   }
   __syncthreads();
-  const bool some = s_teacher[0] != 0.f;
+  const bool some = s_some != 0;
   if (MODE != kBackward) {
-    ls = logf(sum_of_waves<NW>(s_s));
-    if (DUAL) ls1 = logf(sum_of_waves<NW>(s_s1));
+    S = sum_of_waves<NW>(s_s);
+    if (SECOND) S1 = sum_of_waves<NW>(s_s1);
     if (tid == 0) {
-      const float soft = some && a.soft_weight != 0.f ? (s_teacher[1] + ls) * a.tau * a.tau * a.soft_weight : 0.f;
-      const float hard = a.hard_weight != 0.f ? ((m - s_xy) + (DUAL ? ls1 : ls)) * a.hard_weight : 0.f;
+      int arg = s_arg[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) arg = s_arg[w] < arg ? s_arg[w] : arg;
+      const float soft = some && a.soft_weight != 0.f ? (s_b + logf(S)) * a.tau * a.tau * a.soft_weight : 0.f;
+      const float hard =
+          a.hard_weight != 0.f ? (logf(SECOND ? S1 : S) - (SECOND ? fmaf(s_xy, kLog2e, -mc1) : fmaf(s_xy, c, -mc)) * kLn2) * a.hard_weight : 0.f;
       a.row_loss[r] = soft + hard;
-      a.correct[r] = static_cast<unsigned char>(s_best);
+      // without targets: agreement with the teacher's first choice
+      a.correct[r] = arg == (a.targets ? static_cast<int>(target) : s_first) ? 1 : 0;
       if (MODE == kForward) {
         a.row_stats[3 * r] = m;
-        a.row_stats[3 * r + 1] = ls;
-        a.row_stats[3 * r + 2] = ls1;
+        a.row_stats[3 * r + 1] = S;
+        a.row_stats[3 * r + 2] = S1;
       }
     }
   }
@@ -289,31 +326,28 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
   // ---- gradient
   float w = a.scale[0];
   if (MODE == kBackward) w *= a.grad_out[a.grad_out_rows ? r : 0];
-  const float cs = w * a.soft_weight * a.tau;       // per unit of q - p
-  const float ch = w * a.hard_weight;               // per unit of q1 - [j = y]
+  const float cs = some ? w * a.soft_weight * a.tau : 0.f, ch = w * a.hard_weight;
   // coefficients of the exponentials: with one temperature both terms share it (tau = 1) or one of them is absent
-  const float c0 = DUAL ? (some ? cs : 0.f) : (some ? cs : 0.f) + ch;
-  const float c = a.exp_scale;
-  const int y = a.hard_weight != 0.f ? static_cast<int>(target) : -1;
-  each_vec([&](int k, const raw16& v) __attribute__((always_inline)) {
+  const float c0 = (SECOND ? cs : cs + ch) / S, c1 = SECOND ? ch / S1 : 0.f;
+  each_vec([&](int k, const raw16& v, auto whole) __attribute__((always_inline)) {
     float x[V], d[V];
     raw_to_f32<TR, V>(v, x);
-    const int j0 = k * V - shift;
-    const bool full = j0 >= 0 && j0 + V <= C;
-    const unsigned long long word = *reinterpret_cast<const unsigned long long*>(s_bits + 2 * (k >> 6));
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      // exp(x - m - log(sum)): the logarithm is scaled with the argument so that one multiply serves both
-      float g = c0 * __builtin_amdgcn_exp2f((x[j] - m) * c - ls * kLog2e);
-      if (DUAL) g += ch * __builtin_amdgcn_exp2f((x[j] - m) * kLog2e - ls1 * kLog2e);
-      if (j0 + j == y) g -= ch;
-      d[j] = full || (j0 + j >= 0 && j0 + j < C) ? g : 0.f;
+      const float e = __builtin_amdgcn_exp2f(fmaf(x[j], c, -mc));
+      d[j] = c0 * e;
+      if (SECOND) d[j] = fmaf(c1, second(x[j], e), d[j]);
+      if (!decltype(whole)::value && outside(k, j)) d[j] = 0.f;
     }
-    if (word >> (k & 63) & 1ull) {
+    // a wave's vectors are 64 consecutive ones: one word of bits, the same for all its lanes
+    const unsigned* bits = s_bits + 2 * (k >> 6);
+    const unsigned mine = bits[lane >> 5];
+    if (__any(mine != 0u) && (mine >> (k & 31) & 1u)) {
+      const int j0 = k * V - shift;
       for (int e = s_head[k & (a.hash - 1)]; e >= 0; e = s_next[e]) {
         const int at = s_id[e] - j0;
         if (at < 0 || at >= V) continue;
-        const float p = cs * s_x[e];
+        const float p = w * s_x[e];
 #pragma unroll
         for (int j = 0; j < V; ++j) d[j] -= j == at ? p : 0.f;
       }
@@ -395,19 +429,21 @@ void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t st
   // one exponential: at the temperature of the term that is there (tau = 1: of both)
   a.exp_scale = (a.soft_weight != 0.f ? a.inv_tau : 1.f) * kLog2e;
   a.hash = 64;
-  while (a.hash < a.K) a.hash *= 2;
+  while (a.hash <= a.K) a.hash *= 2;
   dispatch_dtype(dtype, [&](auto tr) {
     using TR = decltype(tr);
     constexpr int V = TR::kVec;
     const long long nvec = (a.ld + 2 * V - 2) / V;  // worst alignment
     a.words = static_cast<int>((nvec + 63) / 64);
-    const size_t lds = (static_cast<size_t>(4) * a.K + a.hash + 2 * static_cast<size_t>(a.words)) * 4;
+    const size_t lds = (static_cast<size_t>(4) * (a.K + 1) + a.hash + 2 * static_cast<size_t>(a.words)) * 4;
     const dim3 grid(static_cast<unsigned>(a.N));
     auto go = [&](auto threads_c, auto keep_c, auto mode_c, auto waves_c) {
       constexpr int THREADS = decltype(threads_c)::value, KEEP = decltype(keep_c)::value, MODE = decltype(mode_c)::value;
       constexpr int WAVES = decltype(waves_c)::value;
-      if (dual) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, true, WAVES>), grid, dim3(THREADS), lds, stream, a);
-      else hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, false, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      if (!dual) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 0, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else if (a.tau == 2.f) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 2, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else if (a.tau == 4.f) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 4, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 1, WAVES>), grid, dim3(THREADS), lds, stream, a);
     };
     using std::integral_constant;
     auto by_size = [&](auto mode_c) {

@@ -97,7 +97,7 @@ void launch_xent_fused(void* logits, int dtype, const long long* targets, long l
 // logits [N, ld] (first C columns are classes); ids [N, K] int64 / int32 and teacher [N, K] fp32 / bf16 / fp16: the teacher's
 // entries, an id outside [0, C) or a logit of -inf means "no entry".  targets [N] int64 or nullptr (then every row counts).
 //   row loss = soft_weight tau^2 KL(p || softmax(z / tau)) + hard_weight CE(z, target), 0 for ignored rows
-// mode 0: row losses, correct flags, row_stats[3 r ..] = {max z, log sum at tau, log sum at 1} (dual) | {max, log sum, 0}
+// mode 0: row losses, correct flags, row_stats[3 r ..] = {max z, sum of exponentials, sum at temperature 1 where both are needed}
 // mode 1: dlogits from row_stats, scaled by scale[0] * grad_out[grad_out_rows ? r : 0]
 // mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits
 // dlogits [N, ld]: columns [C, ld) are written as zero; its address must equal that of logits modulo 16.
