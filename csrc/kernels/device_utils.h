@@ -17,6 +17,9 @@ typedef __attribute__((ext_vector_type(4))) unsigned short u16x4;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
+// The same values at addresses that are multiples of their elements only: the hardware loads and stores them whole all the same.
+typedef u16x8 __attribute__((aligned(2))) u16x8_any;
+typedef u16x4 __attribute__((aligned(2))) u16x4_any;
 
 struct F32 {
   using T = float;

@@ -117,11 +117,11 @@ __device__ __forceinline__ void store_gate_fwd(const GemmArgs& p, const f32x4& a
     gr[e] = TR::from_f32(g);
     ur[e] = TR::from_f32(u);
   }
-  if (n == 4 && (H & 3) == 0 && (p.ldc & 3) == 0) {  // (outputs start on 16-byte boundaries)
-    *reinterpret_cast<u16x4*>(C + col) = h;
+  if (n == 4) {
+    *reinterpret_cast<u16x4_any*>(C + col) = h;
     if (P) {
-      *reinterpret_cast<u16x4*>(P + col) = gr;
-      *reinterpret_cast<u16x4*>(P + H + col) = ur;
+      *reinterpret_cast<u16x4_any*>(P + col) = gr;
+      *reinterpret_cast<u16x4_any*>(P + H + col) = ur;
     }
   } else {
 #pragma unroll
@@ -144,11 +144,11 @@ __device__ __forceinline__ void store_gate_bwd(const GemmArgs& p, const f32x4& d
   const u16* GU = static_cast<const u16*>(p.aux) + row * 2 * H + col;
   u16* C = static_cast<u16*>(p.C) + row * p.ldc + col;
   const int n = H - col < 4 ? static_cast<int>(H - col) : 4;
-  const bool whole = n == 4 && (H & 3) == 0;
+  const bool whole = n == 4;
   u16x4 g4, u4, dg, du;
   if (whole) {
-    g4 = *reinterpret_cast<const u16x4*>(GU);
-    u4 = *reinterpret_cast<const u16x4*>(GU + H);
+    g4 = *reinterpret_cast<const u16x4_any*>(GU);
+    u4 = *reinterpret_cast<const u16x4_any*>(GU + H);
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -164,8 +164,8 @@ __device__ __forceinline__ void store_gate_bwd(const GemmArgs& p, const f32x4& d
     du[e] = TR::from_f32(dh[e] * value);
   }
   if (whole) {
-    *reinterpret_cast<u16x4*>(C) = dg;
-    *reinterpret_cast<u16x4*>(C + H) = du;
+    *reinterpret_cast<u16x4_any*>(C) = dg;
+    *reinterpret_cast<u16x4_any*>(C + H) = du;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -181,10 +181,20 @@ __device__ __forceinline__ int kmajor_off(int row, int c) { return row * 128 + (
 // Byte offset of 16-byte chunk c (8 rows) of contraction index k in the swizzled [64][128] image.
 __device__ __forceinline__ int rmajor_off(int k, int c) { return k * 256 + ((c ^ (2 * ((k & 3) + 4 * ((k >> 3) & 1)))) << 4); }
 
+// The first n (8 at most) of eight elements that may start anywhere; the others are zero.
+__device__ __forceinline__ u32x4 load_piece(const u16* src, long long n) {
+  if (n >= 8) return __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_any*>(src));
+  u16x8 e;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = j < n ? src[j] : static_cast<u16>(0);
+  return __builtin_bit_cast(u32x4, e);
+}
+
 // ALIGNED: every 8-element piece is either wholly inside the matrix and 16-byte aligned or wholly outside (base
 // address, leading dimension and contiguous extent are multiples of 8 elements): one 16-byte load per piece.
-// Otherwise (odd extents, leading dimensions or base addresses) the piece is gathered element by element with a
-// bounds check each -- the tail path that lets every shape run here; it costs load instructions, not correctness.
+// Otherwise (odd extents, leading dimensions or base addresses) a piece inside the matrix is one 16-byte load from wherever it starts,
+// and only the pieces across the edge of a row are gathered element by element -- the tail path that lets every shape run here.  (Gathering
+// every piece, the fp16 product 1003 x 520 x 1386 took 166 us; with whole loads and its contraction spread over the chip it takes 20.)
 // PAIRED: the rows are the interleaved ones of a gated pair of R rows each (see gate_row).
 template <bool KMAJOR, bool ALIGNED, bool PAIRED = false>
 __device__ __forceinline__ void load_tile(const u16* __restrict__ base, long long ld, long long r0, long long R, long long k0,
@@ -198,42 +208,22 @@ __device__ __forceinline__ void load_tile(const u16* __restrict__ base, long lon
       const long long vr = r0 + (id >> 3), h = gate_row(vr), k = k0 + ((id & 7) << 3);
       if (h < R && k < K) {
         const u16* src = base + (h + (vr & 16 ? R : 0)) * ld + k;
-        if (ALIGNED) {
-          v = *reinterpret_cast<const u32x4*>(src);
-        } else {
-          const int n = K - k < 8 ? static_cast<int>(K - k) : 8;
-          unsigned short e[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) e[j] = j < n ? src[j] : static_cast<unsigned short>(0);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = static_cast<unsigned>(e[2 * j]) | (static_cast<unsigned>(e[2 * j + 1]) << 16);
-        }
+        if (ALIGNED) v = *reinterpret_cast<const u32x4*>(src);
+        else v = load_piece(src, K - k);
       }
     } else if (KMAJOR) {
       const long long row = r0 + (id >> 3), k = k0 + ((id & 7) << 3);
       if (ALIGNED) {
         if (row < R && k < K) v = *reinterpret_cast<const u32x4*>(base + row * ld + k);
       } else if (row < R && k < K) {
-        const u16* src = base + row * ld + k;
-        const int n = K - k < 8 ? static_cast<int>(K - k) : 8;
-        unsigned short e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = j < n ? src[j] : static_cast<unsigned short>(0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = static_cast<unsigned>(e[2 * j]) | (static_cast<unsigned>(e[2 * j + 1]) << 16);
+        v = load_piece(base + row * ld + k, K - k);
       }
     } else {
       const long long k = k0 + (id >> 4), row = r0 + ((id & 15) << 3);
       if (ALIGNED) {
         if (k < K && row < R) v = *reinterpret_cast<const u32x4*>(base + k * ld + row);
       } else if (k < K && row < R) {
-        const u16* src = base + k * ld + row;
-        const int n = R - row < 8 ? static_cast<int>(R - row) : 8;
-        unsigned short e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = j < n ? src[j] : static_cast<unsigned short>(0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = static_cast<unsigned>(e[2 * j]) | (static_cast<unsigned>(e[2 * j + 1]) << 16);
+        v = load_piece(base + k * ld + row, R - row);
       }
     }
     regs[i] = v;
@@ -271,9 +261,11 @@ __device__ __forceinline__ bf16x8 read_frag(const char* lds, int tile_row0, int 
 }
 
 // TR = BF16 or F16: the two 16-bit types share everything but the MFMA opcode and the epilogue's conversions.
-// GATE / GACT: GemmArgs::gate with its activation.
-template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED, typename TR, int GATE = 0, int GACT = kActNone>
+// GATE / GACT: GemmArgs::gate with its activation.  SPREAD: blockIdx.y takes its share of the contraction (p.split_k shares) and leaves raw
+// fp32 sums in p.workspace[share][M][N rounded up to 4] for spread_reduce_kernel.
+template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED, typename TR, int GATE = 0, int GACT = kActNone, bool SPREAD = false>
 __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int tiles_m, int tiles_n) {
+  static_assert(!SPREAD || GATE == 0, "plain products only");
   extern __shared__ __attribute__((aligned(16))) char smem_bf16[];
 
   const int nwg = tiles_m * tiles_n;
@@ -295,16 +287,17 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   u32x4 ra[4], rb[4];
-  const long long nk = (p.K + BK - 1) / BK;
-  load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, 0, p.K, ra);
+  const long long nk_all = (p.K + BK - 1) / BK;
+  const long long kt0 = SPREAD ? nk_all * blockIdx.y / p.split_k : 0, nk = SPREAD ? nk_all * (blockIdx.y + 1) / p.split_k : nk_all;
+  load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, kt0 * BK, p.K, ra);
   const long long b_rows = GATE == 1 ? p.gate_H : p.N;
-  load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, 0, p.K, rb);
+  load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, kt0 * BK, p.K, rb);
   store_tile<A_KMAJOR>(smem_bf16, ra);
   store_tile<B_KMAJOR>(smem_bf16 + kTileBytes, rb);
   __syncthreads();
 
   int cur = 0;
-  for (long long kt = 0; kt < nk; ++kt) {
+  for (long long kt = kt0; kt < nk; ++kt) {
     const bool more = kt + 1 < nk;
     if (more) {
       load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, (kt + 1) * BK, p.K, ra);
@@ -341,6 +334,18 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
   }
 
   // Epilogue (operands were swapped in the MFMA: see store_tile_bf16).
+  if constexpr (SPREAD) {
+    const long long pitch = (p.N + 3) & ~3ll;
+    float* ws = p.workspace + static_cast<long long>(blockIdx.y) * p.M * pitch;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long row = m0 + wm + 16 * i + (lane & 15), col = n0 + wn + 16 * j + 4 * (lane >> 4);
+        if (row < p.M && col < p.N) *reinterpret_cast<f32x4*>(ws + row * pitch + col) = acc[i][j];
+      }
+    return;
+  }
   if constexpr (GATE == 1) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -1561,6 +1566,19 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(GemmArgs p) {
   store_tile_bf16(p, acc, row, col0);
 }
 
+// Adds the shares of a spread product up in order and finishes it (bias, rounding).
+template <typename TR>
+__global__ __launch_bounds__(256) void spread_reduce_kernel(GemmArgs p) {
+  const long long pitch = (p.N + 3) & ~3ll, nq = pitch >> 2;
+  const long long quad = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (quad >= p.M * nq) return;
+  const long long row = quad / nq, col0 = (quad - row * nq) << 2, plane = p.M * pitch;
+  const float* src = p.workspace + row * pitch + col0;
+  f32x4 acc = *reinterpret_cast<const f32x4*>(src);
+  for (int s = 1; s < p.split_k; ++s) acc += *reinterpret_cast<const f32x4*>(src + s * plane);
+  store_tile_bf16<TR>(p, acc, row, col0);
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // 16-byte global loads everywhere: contiguous extents, leading dimensions and base addresses in multiples of 8
@@ -1710,8 +1728,6 @@ bool gemm_gate_supported(const GemmArgs& a, int dtype) {
   if (dtype != kBF16 && dtype != kF16) return false;
   if (a.act != kActRelu && a.act != kActGelu && a.act != kActSilu) return false;
   if (a.gate_H <= 0 || a.gate_H >= (1ll << 30)) return false;
-  // 8-byte accesses of the epilogues where H is a multiple of 4
-  if (reinterpret_cast<uintptr_t>(a.C) % 8 || reinterpret_cast<uintptr_t>(a.pre_act) % 8 || reinterpret_cast<uintptr_t>(a.aux) % 8) return false;
   if (a.gate == 1) return a.a_kmajor && a.b_kmajor && a.N == 2 * a.gate_H && a.ldc == a.gate_H && gemm_bf16_supported(a);
   return a.gate == 2 && a.a_kmajor && !a.b_kmajor && a.N == a.gate_H && a.ldc == 2 * a.gate_H && a.aux != nullptr && gemm_bf16_supported(a);
 }
@@ -1859,6 +1875,40 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream) {
   else if (a.a_kmajor && !a.b_kmajor) go(std::true_type{}, std::false_type{});
   else if (!a.a_kmajor && a.b_kmajor) go(std::false_type{}, std::true_type{});
   else go(std::false_type{}, std::false_type{});
+}
+
+// Shares of the contraction that let a product with few 128x128 tiles fill the chip: two workgroups per compute unit, at least three k-steps a
+// share (its start and the fp32 sums then stay small beside it), 64 MiB of sums at most.  1: not worth it.
+int gemm_spread(const GemmArgs& a) {
+  const long long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN), nk = (a.K + BK - 1) / BK;
+  const int cus = compute_units();
+  if (tiles >= cus || nk < 6) return 1;
+  long long s = 2ll * cus / tiles;
+  if (s > nk / 3) s = nk / 3;
+  const long long plane = a.M * ((a.N + 3) & ~3ll) * 4;
+  if (s > (64ll << 20) / plane) s = (64ll << 20) / plane;
+  return s < 2 ? 1 : static_cast<int>(s);
+}
+
+void launch_gemm_spread(const GemmArgs& a, int dtype, hipStream_t stream) {
+  const int tiles_m = static_cast<int>((a.M + BM - 1) / BM), tiles_n = static_cast<int>((a.N + BN - 1) / BN);
+  const dim3 grid(static_cast<unsigned>(tiles_m) * static_cast<unsigned>(tiles_n), static_cast<unsigned>(a.split_k));
+  const bool vec = gemm_bf16_vector_aligned(a);
+  auto typed = [&](auto tr) {
+    using TR = decltype(tr);
+    auto go = [&](auto ak, auto bk) {
+      constexpr bool AK = decltype(ak)::value, BKM = decltype(bk)::value;
+      if (vec) hipLaunchKernelGGL((gemm_bf16_kernel<AK, BKM, true, TR, 0, kActNone, true>), grid, dim3(kThreads), 4 * kTileBytes, stream, a, tiles_m, tiles_n);
+      else hipLaunchKernelGGL((gemm_bf16_kernel<AK, BKM, false, TR, 0, kActNone, true>), grid, dim3(kThreads), 4 * kTileBytes, stream, a, tiles_m, tiles_n);
+    };
+    if (a.a_kmajor && a.b_kmajor) go(std::true_type{}, std::true_type{});
+    else if (a.a_kmajor) go(std::true_type{}, std::false_type{});
+    else go(std::false_type{}, std::false_type{});  // (the three layouts of a linear layer)
+    const long long quads = a.M * (((a.N + 3) & ~3ll) >> 2);
+    hipLaunchKernelGGL((spread_reduce_kernel<TR>), dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, a);
+  };
+  if (dtype == kF16) typed(F16{});
+  else typed(BF16{});
 }
 
 // fp16 products: the 128x128 kernel with the fp16 MFMA (the LDS-DMA kernel and split-K are bf16 only).

@@ -203,6 +203,14 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream);
 // fp16 storage (fp32 accumulate) on the 128x128 MFMA kernel; same argument conventions.
 bool gemm_f16_supported(const GemmArgs& a);
 void launch_gemm_f16(const GemmArgs& a, hipStream_t stream);
+// Products with few output tiles (bf16 / fp16; the layouts NT, NN and TN of a linear layer; bias, no act / pre_act / beta): the contraction cut
+// into gemm_spread() shares (a.split_k, a.workspace of split_k * M * (N rounded up to 4) floats) on the 128x128 kernel.
+int gemm_spread(const GemmArgs& a);
+void launch_gemm_spread(const GemmArgs& a, int dtype, hipStream_t stream);
+// At most kFewRows rows of A (bf16 / fp16, NT layout, plain with bias or gate 1): a kernel bound by reading B once.
+constexpr int kFewRows = 64;
+bool few_rows_supported(const GemmArgs& a, int dtype);
+void launch_few_rows(const GemmArgs& a, int dtype, hipStream_t stream);
 // GemmArgs::gate 1 / 2 in `dtype` (kBF16 or kF16); any extents, odd ones included.
 bool gemm_gate_supported(const GemmArgs& a, int dtype);
 long long gemm_gate_colsum_rows(const GemmArgs& a, int dtype);  // 0: this launch takes no column sums

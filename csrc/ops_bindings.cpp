@@ -535,8 +535,24 @@ Tensor tile_counters_for(kernels::GemmArgs& a, const Tensor& like) {
   return t;
 }
 
-// `like` supplies the device for the split-K workspace (fp32 partials, caching allocator).
-void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& like) {
+// `like` supplies the device for the split-K workspace (fp32 partials, caching allocator).  spread: products of few rows take the kernel made
+// for them and products of few output tiles cut their contraction over the chip (another order of summation than without).
+void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& like, bool spread = false) {
+  if (spread && kernels::few_rows_supported(a, dt)) {
+    kernels::launch_few_rows(a, dt, s);
+    return;
+  }
+  if (spread && dt != kernels::kF32 && (dt == kernels::kF16 || kernels::gemm_bf16_split_k(a) == 1)) {
+    const int shares = kernels::gemm_spread(a);
+    if (shares > 1) {
+      kernels::GemmArgs b = a;
+      Tensor ws = at::empty({shares * a.M * ((a.N + 3) / 4 * 4)}, like.options().dtype(at::kFloat));
+      b.workspace = ws.data_ptr<float>();
+      b.split_k = shares;
+      kernels::launch_gemm_spread(b, dt, s);
+      return;
+    }
+  }
   if (dt == kernels::kF32) {
     kernels::launch_gemm_f32(a, s);
     return;
@@ -578,7 +594,9 @@ std::string linear_route(int64_t M, int64_t N, int64_t K, int dt) {
 }
 
 // y = act(x W^T + b).  x: [M, K], W: [N, K], b: [N] or None.  Returns (y, pre_activation or None).
-std::tuple<Tensor, c10::optional<Tensor>> linear_forward(Tensor x, Tensor w, c10::optional<Tensor> bias, int64_t act, bool save_pre_act) {
+// spread: see run_gemm (no activation).
+std::tuple<Tensor, c10::optional<Tensor>> linear_forward(Tensor x, Tensor w, c10::optional<Tensor> bias, int64_t act, bool save_pre_act, bool spread) {
+  TORCH_CHECK(!spread || act == kernels::kActNone, "linear_forward: a spread product has no activation");
   check_gpu(x, "x");
   check_gpu(w, "weight");
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "linear_forward: x [M,K] and weight [N,K] expected");
@@ -613,7 +631,7 @@ std::tuple<Tensor, c10::optional<Tensor>> linear_forward(Tensor x, Tensor w, c10
       a.pre_act = pre->data_ptr();
     }
     TORCH_CHECK(gemm_path_ok(a, dt), "linear_forward: shape M=", M, " N=", N, " K=", K, " is not supported by the MFMA GEMM for dtype ", x.scalar_type());
-    run_gemm(a, dt, s, x);
+    run_gemm(a, dt, s, x, spread);
   }
   return {y, pre};
 }
@@ -633,7 +651,7 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_forward(Tensor x, Tensor w, c10:
   DevGuard guard(x);
   hipStream_t s = stream_of(x);
   if (dt == kernels::kF32) {
-    Tensor gu = std::get<0>(linear_forward(x, w, bias, kernels::kActNone, false));
+    Tensor gu = std::get<0>(linear_forward(x, w, bias, kernels::kActNone, false, false));
     Tensor h = at::empty({M, H}, x.options());
     kernels::launch_gate_fwd(gu.data_ptr(), h.data_ptr(), M, H, dt, static_cast<int>(act), s);
     return {h, save ? c10::optional<Tensor>(gu) : c10::nullopt};
@@ -654,6 +672,10 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_forward(Tensor x, Tensor w, c10:
   a.M = M; a.N = 2 * H; a.K = K; a.lda = K; a.ldb = K; a.ldc = H;
   a.a_kmajor = 1; a.b_kmajor = 1; a.act = static_cast<int>(act); a.alpha = 1.f; a.gate = 1; a.gate_H = H;
   TORCH_CHECK(kernels::gemm_gate_supported(a, dt), "gated_forward: shape M=", M, " H=", H, " K=", K, " is not supported");
+  if (kernels::few_rows_supported(a, dt)) {
+    kernels::launch_few_rows(a, dt, s);
+    return {h, gu};
+  }
   const Tensor counters = dt == kernels::kBF16 ? tile_counters_for(a, x) : Tensor();
   kernels::launch_gemm_gate(a, dt, s);
   return {h, gu};
@@ -777,8 +799,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rank1_mlp_backward(Tensor dy, Tensor 
 
 // Gradients of y = x W^T + b given g = dL/d(xW^T+b).  Returns (dx or None, dW, db or None).
 // dw_out: write the weight gradient into this tensor (a slice of a gradient bucket) instead of a fresh one.
+// spread: see run_gemm.
 std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward(Tensor g, Tensor x, Tensor w, bool need_dx, bool need_db,
-                                                                                   c10::optional<Tensor> dw_out) {
+                                                                                   c10::optional<Tensor> dw_out, bool spread) {
   check_gpu(g, "grad");
   check_gpu(x, "x");
   check_gpu(w, "weight");
@@ -821,14 +844,14 @@ std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward
     a.A = g.data_ptr(); a.B = x.data_ptr(); a.C = dW.data_ptr();
     a.M = N; a.N = K; a.K = M; a.lda = N; a.ldb = K; a.ldc = K; a.a_kmajor = 0; a.b_kmajor = 0; a.alpha = 1.f;
     TORCH_CHECK(gemm_path_ok(a, dt), "linear_backward: weight-gradient shape not supported by the MFMA GEMM");
-    run_gemm(a, dt, s, g);
+    run_gemm(a, dt, s, g, spread);
     if (need_dx) {
       // dx[M,K] = g W : contraction over N; A = g is contraction-contiguous, B = W is stored [N(contraction), K].
       kernels::GemmArgs b{};
       b.A = g.data_ptr(); b.B = w.data_ptr(); b.C = dx->data_ptr();
       b.M = M; b.N = K; b.K = N; b.lda = N; b.ldb = K; b.ldc = K; b.a_kmajor = 1; b.b_kmajor = 0; b.alpha = 1.f;
       TORCH_CHECK(gemm_path_ok(b, dt), "linear_backward: input-gradient shape not supported by the MFMA GEMM");
-      run_gemm(b, dt, s, g);
+      run_gemm(b, dt, s, g, spread);
     }
     if (need_db) {
       Tensor ws = at::empty({kernels::colreduce_workspace(M, N)}, fopt);
@@ -1341,9 +1364,10 @@ void init_ops(py::module_& m) {
     const int dt = dtype == "float32" ? kernels::kF32 : (dtype == "bfloat16" ? kernels::kBF16 : kernels::kF16);
     return linear_route(M, N, K, dt);
   });
-  m.def("linear_forward", &linear_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act") = 0, py::arg("save_pre_act") = false);
+  m.def("linear_forward", &linear_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act") = 0, py::arg("save_pre_act") = false,
+        py::arg("spread") = false);
   m.def("linear_backward", &linear_backward, py::arg("grad"), py::arg("x"), py::arg("weight"), py::arg("need_dx") = true, py::arg("need_db") = true,
-        py::arg("dw_out") = py::none());
+        py::arg("dw_out") = py::none(), py::arg("spread") = false);
   m.def("rank1_mlp_forward", &rank1_mlp_forward, py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("b2"), py::arg("act") = 0);
   m.def("rank1_mlp_backward", &rank1_mlp_backward, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("act") = 0);
   m.def("gated_forward", &gated_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("save") = true);

@@ -108,7 +108,7 @@ class _GatedMLP(torch.autograd.Function):
     def forward(ctx, x2, w_fc, b_fc, w_proj, b_proj, act: int):
         C = _ext.C()
         h, gu = C.gated_forward(x2, w_fc, b_fc, act, True)
-        y, _ = C.linear_forward(h, w_proj, b_proj, 0, False)
+        y, _ = C.linear_forward(h, w_proj, b_proj, 0, False, True)
         ctx.save_for_backward(x2, w_fc, w_proj, gu, h)
         ctx.act = act
         ctx.biases = (b_fc is not None, b_proj is not None)
@@ -123,13 +123,13 @@ class _GatedMLP(torch.autograd.Function):
         has_fc, has_proj = ctx.biases
         dx = dw_fc = db_fc = dw_proj = db_proj = None
         if need[3]:
-            _, dw_proj, db_proj = C.linear_backward(dy, h, w_proj, False, has_proj and need[4], _sink(w_proj))
+            _, dw_proj, db_proj = C.linear_backward(dy, h, w_proj, False, has_proj and need[4], _sink(w_proj), True)
         elif has_proj and need[4]:
             db_proj = C.colsum(dy)
         if need[0] or need[1] or need[2]:
             dgu, db_fc = C.gated_backward(dy, w_proj, gu, ctx.act, has_fc and need[2])
             if need[1]:
-                dx, dw_fc, _ = C.linear_backward(dgu, x2, w_fc, need[0], False, _sink(w_fc))
+                dx, dw_fc, _ = C.linear_backward(dgu, x2, w_fc, need[0], False, _sink(w_fc), True)
             elif need[0]:
                 dx = C.gemm(dgu, w_fc, True, False)
         return dx, dw_fc, db_fc, dw_proj, db_proj, None
@@ -182,5 +182,5 @@ def gated_mlp(x: torch.Tensor, w_fc: torch.Tensor, b_fc: Optional[torch.Tensor],
     else:
         C = _ext.C()
         h, _ = C.gated_forward(x2, tensors[0], tensors[1], code, False)
-        y, _ = C.linear_forward(h, tensors[2], tensors[3], 0, False)
+        y, _ = C.linear_forward(h, tensors[2], tensors[3], 0, False, True)
     return y.reshape(*x.shape[:-1], w_proj.shape[0])
