@@ -138,18 +138,18 @@ template <int D>
 struct TileSource {
   static constexpr int kPieces = D / 16;
   static constexpr int kPieceRows = 512 / D;   // rows of 2 D bytes per 1 KiB
+  static constexpr int kLanesPerRow = 64 / kPieceRows;
   unsigned off[kPieces];
   unsigned pitch;   // bytes between rows
-  int row[kPieces], chunk[kPieces];
+  int row0;         // this lane's row of the first piece
+  static __device__ __forceinline__ unsigned chunk_of(int row, int lane) {
+    return static_cast<unsigned>(((lane % kLanesPerRow) ^ swz<D>(row)) * 16);
+  }
   __device__ __forceinline__ void init(long long stride, int piece0, int lane) {
     pitch = static_cast<unsigned>(stride) * 2u;
-    constexpr int kLanesPerRow = 64 / kPieceRows;
+    row0 = piece0 * kPieceRows + lane / kLanesPerRow;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      row[i] = (piece0 + i) * kPieceRows + lane / kLanesPerRow;
-      chunk[i] = ((lane % kLanesPerRow) ^ swz<D>(row[i])) * 16;
-      off[i] = static_cast<unsigned>(row[i]) * pitch + static_cast<unsigned>(chunk[i]);
-    }
+    for (int i = 0; i < kPieces; ++i) off[i] = static_cast<unsigned>(row0 + i * kPieceRows) * pitch + chunk_of(row0 + i * kPieceRows, lane);
   }
   // `first`: the tile's first row; only `valid` (>= 1) of its rows may be read, the others repeat the last of those.
   __device__ __forceinline__ void request(const u16* first, int valid, unsigned lds) const {
@@ -158,10 +158,11 @@ struct TileSource {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) dma_16B(base, off[i], lds + i * 1024);
     } else {
+      const int lane = threadIdx.x & 63;
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        const int r = row[i] < valid ? row[i] : valid - 1;
-        dma_16B(base, static_cast<unsigned>(r) * pitch + static_cast<unsigned>(chunk[i]), lds + i * 1024);
+        const int row = row0 + i * kPieceRows, r = row < valid ? row : valid - 1;
+        dma_16B(base, static_cast<unsigned>(r) * pitch + chunk_of(row, lane), lds + i * 1024);
       }
     }
   }
@@ -241,12 +242,34 @@ struct KeyTiles {
   }
 };
 
-// What a wave of 32 queries from qw has to do with the 64 keys from key0.
-__device__ __forceinline__ bool wave_sees(const WindowAttnArgs& p, int qw, int key0) {
-  return key0 <= qw + 31 && (key0 + kTile - 1 > qw - p.window || key0 < p.sinks);
+// What a wave of 32 queries from qw has to do with the 32 keys from k0.  A border of the mask crosses few of these squares, and most of
+// those are crossed by one border only: the comparisons are instantiated for the border (two instructions a score) and only squares
+// with several take all of them.
+enum Border : int { kClear = 0, kCausal = 1, kWindow = 2, kSinks = 3, kSeveral = 4, kUnseen = 5 };
+__device__ __forceinline__ int border_of(const WindowAttnArgs& p, int qw, int k0) {
+  if (k0 > qw + 31) return kUnseen;
+  const bool future = k0 + 31 > qw, past = k0 <= qw + 31 - p.window && k0 + 31 >= p.sinks;
+  if (!past) return future ? kCausal : kClear;
+  if (k0 + 31 <= qw - p.window) return k0 < p.sinks ? kSinks : kUnseen;  // behind every query's window: sinks or nothing
+  return future || k0 < p.sinks ? kSeveral : kWindow;
 }
-__device__ __forceinline__ bool needs_mask(const WindowAttnArgs& p, int qw, int key0) {
-  return key0 + kTile - 1 > qw || !(key0 > qw + 31 - p.window || key0 + kTile - 1 < p.sinks);
+// Hides key index j of a lane whose query is at index `rel`; sinks end at index `sink`.
+template <int BORDER>
+__device__ __forceinline__ bool hidden(const WindowAttnArgs& p, int j, int rel, int sink) {
+  if (BORDER == kCausal) return j > rel;
+  if (BORDER == kWindow) return j <= rel - p.window;
+  if (BORDER == kSinks) return j >= sink;
+  if (BORDER == kSeveral) return j > rel || (j <= rel - p.window && j >= sink);
+  return false;
+}
+// f(std::integral_constant<int, border>) for a border other than kUnseen.
+template <typename F>
+__device__ __forceinline__ void with_border(int border, F&& f) {
+  if (border == kClear) f(std::integral_constant<int, kClear>{});
+  else if (border == kCausal) f(std::integral_constant<int, kCausal>{});
+  else if (border == kWindow) f(std::integral_constant<int, kWindow>{});
+  else if (border == kSinks) f(std::integral_constant<int, kSinks>{});
+  else f(std::integral_constant<int, kSeveral>{});
 }
 
 // ---------------------------------------------------------------------------------------------------- forward
@@ -256,39 +279,36 @@ __device__ __forceinline__ bool needs_mask(const WindowAttnArgs& p, int qw, int 
 constexpr float kDefer = 8.f;
 constexpr float kLowest = -1e30f;  // a start below every score that keeps exp2(-inf - m) at zero where a query sees nothing yet
 
-template <typename TR, int D, bool MASK>
-__device__ __forceinline__ void fwd_tile(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], f32x4 (&o)[2][D / 16],
-                                         float (&m)[2], f32x4 (&lsum)[2], int key0, int qw, int lane) {
+// The 32 keys in rows 32 half .. of a tile, key k0 first.
+template <typename TR, int D, int BORDER>
+__device__ __forceinline__ void fwd_half(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], f32x4 (&o)[2][D / 16],
+                                         float (&m)[2], f32x4 (&lsum)[2], int half, int k0, int qw, int lane) {
   const int g = lane >> 4, li = lane & 15;
   const float c = p.scale_log2;
-  f32x4 s[2][4];
+  f32x4 s[2][2];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
+  for (int t = 0; t < 2; ++t) {
 #pragma unroll
     for (int st = 0; st < 2; ++st) s[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk) {
-      const s16x8 kf = row_frag<D>(ks, t, kk, lane);
+      const s16x8 kf = row_frag<D>(ks, 2 * half + t, kk, lane);
 #pragma unroll
       for (int st = 0; st < 2; ++st) s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
     }
   }
-  s16x8 pf[2][2];
+  s16x8 pf[2];
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
-    if (MASK) {  // register (t, e) is key key0 + 4 g + 16 t + e
-      const int rel = qw + 16 * st + li - key0 - 4 * g, sink = p.sinks - key0 - 4 * g;
+    if (BORDER != kClear) {  // register (t, e) is key k0 + 4 g + 16 t + e
+      const int rel = qw + 16 * st + li - k0 - 4 * g, sink = p.sinks - k0 - 4 * g;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = 16 * t + e;
-          if (j > rel || (j <= rel - p.window && j >= sink)) s[st][t][e] = kNegInf;
-        }
+      for (int i = 0; i < 8; ++i)
+        if (hidden<BORDER>(p, 16 * (i >> 2) + (i & 3), rel, sink)) s[st][i >> 2][i & 3] = kNegInf;
     }
     float mx = s[st][0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[st][i >> 2][i & 3]);
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[st][i >> 2][i & 3]);
     mx *= c;  // c > 0
     if (__any(mx > m[st] + kDefer)) {
       const float mg = groups_max(mx);
@@ -304,26 +324,19 @@ __device__ __forceinline__ void fwd_tile(const WindowAttnArgs& p, const char* ks
     }
     const float nm = -m[st];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[st][t][e] = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, nm));
-#pragma unroll
-    for (int sk = 0; sk < 2; ++sk) pf[st][sk] = pack8<TR>(s[st][2 * sk], s[st][2 * sk + 1]);
+    for (int i = 0; i < 8; ++i) s[st][i >> 2][i & 3] = __builtin_amdgcn_exp2f(fmaf(s[st][i >> 2][i & 3], c, nm));
+    pf[st] = pack8<TR>(s[st][0], s[st][1]);
   }
   const short one = std::is_same<TR, F16>::value ? 0x3C00 : 0x3F80;
   const s16x8 ones = {one, one, one, one, one, one, one, one};
 #pragma unroll
-  for (int sk = 0; sk < 2; ++sk)
+  for (int st = 0; st < 2; ++st) lsum[st] = mfma<TR>(ones, pf[st], lsum[st]);
 #pragma unroll
-    for (int st = 0; st < 2; ++st) lsum[st] = mfma<TR>(ones, pf[st][sk], lsum[st]);
+  for (int td = 0; td < D / 16; ++td) {
+    const s16x8 vf = tr_frag<D>(vs, 32 * half, td, lane);
 #pragma unroll
-  for (int td = 0; td < D / 16; ++td)
-#pragma unroll
-    for (int sk = 0; sk < 2; ++sk) {
-      const s16x8 vf = tr_frag<D>(vs, 32 * sk, td, lane);
-#pragma unroll
-      for (int st = 0; st < 2; ++st) o[st][td] = mfma<TR>(vf, pf[st][sk], o[st][td]);
-    }
+    for (int st = 0; st < 2; ++st) o[st][td] = mfma<TR>(vf, pf[st], o[st][td]);
+  }
 }
 
 // Workgroup -> (batch, query head, query block): the heads of a group next to each other, then the blocks, the long ones first.
@@ -390,9 +403,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
     if (it + S - 1 < tiles.count) request(it + S - 1, stage == 0 ? S - 1 : stage - 1);
     const char* ks = smem + stage * 2 * TB;
     const int key0 = tiles.key0(it);
-    if (wave_sees(p, qw, key0)) {
-      if (needs_mask(p, qw, key0)) fwd_tile<TR, D, true>(p, ks, ks + TB, qf, o, m, lsum, key0, qw, lane);
-      else fwd_tile<TR, D, false>(p, ks, ks + TB, qf, o, m, lsum, key0, qw, lane);
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      const int k0 = key0 + 32 * half, border = border_of(p, qw, k0);
+      if (border != kUnseen)
+        with_border(border, [&](auto b_c) __attribute__((always_inline)) {
+          fwd_half<TR, D, decltype(b_c)::value>(p, ks, ks + TB, qf, o, m, lsum, half, k0, qw, lane);
+        });
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -409,53 +426,45 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
 }
 
 // ---------------------------------------------------------------------------------------------------- backward: dQ
-template <typename TR, int D, bool MASK>
-__device__ __forceinline__ void dq_tile(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], const s16x8 (&dof)[2][D / 32],
-                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const float (&delta)[2], int key0, int qw, int lane) {
+template <typename TR, int D, int BORDER>
+__device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], const s16x8 (&dof)[2][D / 32],
+                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const float (&delta)[2], int half, int k0, int qw, int lane) {
   const int g = lane >> 4, li = lane & 15;
   const float c = p.scale_log2;
-  s16x8 dsf[2][2];
-  // two 16-key tiles at a time: one operand of the next product
+  f32x4 s[2][2], dp[2][2];
 #pragma unroll
-  for (int sk = 0; sk < 2; ++sk) {
-    f32x4 s[2][2], dp[2][2];
+  for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int st = 0; st < 2; ++st) s[st][t] = dp[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int st = 0; st < 2; ++st) s[st][t] = dp[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kk = 0; kk < D / 32; ++kk) {
+      const s16x8 kf = row_frag<D>(ks, 2 * half + t, kk, lane), vf = row_frag<D>(vs, 2 * half + t, kk, lane);
 #pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk) {
-        const s16x8 kf = row_frag<D>(ks, 2 * sk + t, kk, lane), vf = row_frag<D>(vs, 2 * sk + t, kk, lane);
-#pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
-          dp[st][t] = mfma<TR>(vf, dof[st][kk], dp[st][t]);
-        }
+      for (int st = 0; st < 2; ++st) {
+        s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
+        dp[st][t] = mfma<TR>(vf, dof[st][kk], dp[st][t]);
       }
     }
+  }
+  s16x8 dsf[2];
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const int rel = qw + 16 * st + li - key0 - 4 * g - 32 * sk, sink = p.sinks - key0 - 4 * g - 32 * sk;
+  for (int st = 0; st < 2; ++st) {
+    const int rel = qw + 16 * st + li - k0 - 4 * g, sink = p.sinks - k0 - 4 * g;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = 16 * t + e;
-          const float pe = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, -lse2[st]));
-          const float ds = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
-          s[st][t][e] = MASK && (j > rel || (j <= rel - p.window && j >= sink)) ? 0.f : ds;
-        }
-      dsf[st][sk] = pack8<TR>(s[st][0], s[st][1]);
+    for (int i = 0; i < 8; ++i) {
+      const int t = i >> 2, e = i & 3;
+      const float pe = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, -lse2[st]));
+      const float ds = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
+      s[st][t][e] = hidden<BORDER>(p, 16 * t + e, rel, sink) ? 0.f : ds;
     }
+    dsf[st] = pack8<TR>(s[st][0], s[st][1]);
   }
 #pragma unroll
-  for (int td = 0; td < D / 16; ++td)
+  for (int td = 0; td < D / 16; ++td) {
+    const s16x8 kt = tr_frag<D>(ks, 32 * half, td, lane);
 #pragma unroll
-    for (int sk = 0; sk < 2; ++sk) {
-      const s16x8 kt = tr_frag<D>(ks, 32 * sk, td, lane);
-#pragma unroll
-      for (int st = 0; st < 2; ++st) dq[st][td] = mfma<TR>(kt, dsf[st][sk], dq[st][td]);
-    }
+    for (int st = 0; st < 2; ++st) dq[st][td] = mfma<TR>(kt, dsf[st], dq[st][td]);
+  }
 }
 
 template <typename TR, int D>
@@ -525,9 +534,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p
     if (it + S - 1 < tiles.count) request(it + S - 1, stage == 0 ? S - 1 : stage - 1);
     const char* ks = smem + stage * 2 * TB;
     const int key0 = tiles.key0(it);
-    if (wave_sees(p, qw, key0)) {
-      if (needs_mask(p, qw, key0)) dq_tile<TR, D, true>(p, ks, ks + TB, qf, dof, dq, lse2, delta, key0, qw, lane);
-      else dq_tile<TR, D, false>(p, ks, ks + TB, qf, dof, dq, lse2, delta, key0, qw, lane);
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      const int k0 = key0 + 32 * half, border = border_of(p, qw, k0);
+      if (border != kUnseen)
+        with_border(border, [&](auto b_c) __attribute__((always_inline)) {
+          dq_half<TR, D, decltype(b_c)::value>(p, ks, ks + TB, qf, dof, dq, lse2, delta, half, k0, qw, lane);
+        });
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -582,8 +595,8 @@ template <int D>
 constexpr int kDkdvStageBytes = 2 * kTileBytes<D> + 2 * kTile * 4;  // Q | dO | lse2 | delta
 constexpr int kDkdvStages = 3;
 
-template <typename TR, int D, bool MASK>
-__device__ __forceinline__ void dkdv_tile(const WindowAttnArgs& p, const char* qs_, const char* dos_, const char* stats, const s16x8 (&kf)[2][D / 32],
+template <typename TR, int D, int BORDER>
+__device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* qs_, const char* dos_, const char* stats, const s16x8 (&kf)[2][D / 32],
                                           const s16x8 (&vf)[2][D / 32], f32x4 (&dk)[2][D / 16], f32x4 (&dv)[2][D / 16], int half, int q0, int kw,
                                           int len, int lane) {
   // the 32 queries from q0, rows 32 half .. of the stage's tiles, against the wave's 32 keys from kw
@@ -613,9 +626,10 @@ __device__ __forceinline__ void dkdv_tile(const WindowAttnArgs& p, const char* q
   s16x8 pB[2], dsB[2];
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    const int key = kw + 16 * kt + li, rel = key - q0 - 4 * g;   // register (qs, e) is query index 16 qs + e against rel
-    const int far = key < p.sinks ? 0x7fffffff : rel + p.window;  // first index beyond the window
-    const int end = len - q0 - 4 * g;                             // first index beyond the sequence
+    const int key = kw + 16 * kt + li, rel = key - q0 - 4 * g;  // register (qs, e) is query index 16 qs + e against rel
+    const bool sink = key < p.sinks;
+    const int far = BORDER == kSeveral && sink ? 0x7fffffff : rel + p.window;  // first index beyond the window
+    const int end = len - q0 - 4 * g;                                            // first index beyond the sequence
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs)
 #pragma unroll
@@ -623,7 +637,11 @@ __device__ __forceinline__ void dkdv_tile(const WindowAttnArgs& p, const char* q
         const int i = 16 * qs + e;
         float pe = __builtin_amdgcn_exp2f(fmaf(s[kt][qs][e], c, -l2[qs][e]));
         float ds = pe * (dp[kt][qs][e] - dl[qs][e]);
-        if (MASK && (i < rel || i >= far || i >= end)) pe = ds = 0.f;
+        const bool hide = BORDER == kCausal   ? i < rel
+                          : BORDER == kWindow ? i >= far
+                          : BORDER == kSinks  ? !sink
+                                              : BORDER == kSeveral && (i < rel || i >= far || i >= end);
+        if (hide) pe = ds = 0.f;
         s[kt][qs][e] = pe;
         dp[kt][qs][e] = ds;
       }
@@ -735,13 +753,14 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int q0 = (first_qt + ct) * kTile + 32 * half;
-          // the half precedes all of the wave's keys, lies behind the window of the last one and no sink is among them, or behind the sequence
-          const bool skip = q0 + 31 < kw || (q0 >= kw + 31 + p.window && kw >= p.sinks) || q0 >= len;
-          if (!skip) {
-            const bool clear = q0 >= kw + 31 && (q0 + 31 < kw + p.window || kw + 31 < p.sinks) && q0 + 31 < len;
-            if (clear) dkdv_tile<TR, D, false>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
-            else dkdv_tile<TR, D, true>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
-          }
+          // as border_of, with the 32 queries and the wave's keys in each other's place, and the end of the sequence as one more border
+          const bool past = q0 + 31 >= kw + p.window && kw + 31 >= p.sinks, gone = q0 >= kw + 31 + p.window;
+          if (q0 + 31 < kw || (past && gone && kw >= p.sinks) || q0 >= len) continue;
+          const bool future = q0 < kw + 31, ends = q0 + 31 >= len;
+          const int border = ends ? kSeveral : !past ? (future ? kCausal : kClear) : gone ? kSinks : future || kw < p.sinks ? kSeveral : kWindow;
+          with_border(border, [&](auto b_c) __attribute__((always_inline)) {
+            dkdv_half<TR, D, decltype(b_c)::value>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
+          });
         }
         if (++ct == ne) ct = 0;
         stage = stage + 1 == S ? 0 : stage + 1;
@@ -768,10 +787,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
   }
 }
 
-// Adds up the partial sums of the block that piece `blockIdx.x` begins in the middle of, if it is the first such piece.
+// Adds up the partial sums of the block that piece `blockIdx.x` + 1 begins in the middle of, if it is the first such piece.  blockIdx.y: the part of the
+// block that was wave y / 2's, dK (y even) or dV; a wave here takes a quarter of the columns.
 template <typename TR, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_join_kernel(WindowAttnArgs p) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+__global__ __launch_bounds__(kThreads) void window_join_kernel(WindowAttnArgs p) {
   const int G = p.H / p.KV;
   const Units units(p.T, p.window, p.sinks, G);
   const long long per_head = units.all(), total = per_head * p.KV * p.B;
@@ -781,29 +800,40 @@ __global__ __launch_bounds__(kThreads, 2) void window_join_kernel(WindowAttnArgs
   const int b = static_cast<int>(bk / p.KV), kv = static_cast<int>(bk - static_cast<long long>(b) * p.KV);
   const int kb = units.block_of(s - bk * per_head);
   const long long start = bk * per_head + units.before(kb), stop = start + static_cast<long long>(units.tiles(kb)) * G;
-  if (s == start || s == total || piece_start(p, total, w - 1) > start) return;
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int len = length_of(p, b), kw = kb * kRows + wid * 32;
-  f32x4 dk[2][D / 16], dv[2][D / 16];
+  if (s == start || piece_start(p, total, w - 1) > start) return;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, g = lane >> 4, li = lane & 15;
+  const int owner = blockIdx.y >> 1, is_dv = blockIdx.y & 1;
+  const int len = length_of(p, b), kw = kb * kRows + owner * 32;
+  constexpr int Q = D / 64;  // 16-column tiles per wave
+  f32x4 sum[2][Q];
   auto add = [&](int piece, int slot, bool first) {
-    const f32x4* ws = reinterpret_cast<const f32x4*>(p.partial + (2LL * piece + slot) * kPartialFloats<D>) + wid * (4 * (D / 16) * 64) + lane;
+    const f32x4* ws = reinterpret_cast<const f32x4*>(p.partial + (2LL * piece + slot) * kPartialFloats<D>) + owner * (4 * (D / 16) * 64) + lane;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int td = 0; td < D / 16; ++td) {
-        const f32x4 a = ws[(kt * (D / 16) + td) * 64], c = ws[((2 + kt) * (D / 16) + td) * 64];
-        dk[kt][td] = first ? a : dk[kt][td] + a;
-        dv[kt][td] = first ? c : dv[kt][td] + c;
+      for (int q = 0; q < Q; ++q) {
+        const f32x4 a = ws[((2 * is_dv + kt) * (D / 16) + wid * Q + q) * 64];
+        sum[kt][q] = first ? a : sum[kt][q] + a;
       }
   };
   add(w - 1, 1, true);
   for (int piece = w; piece < p.pieces && piece_start(p, total, piece) < stop; ++piece)
     if (piece_start(p, total, piece + 1) > piece_start(p, total, piece)) add(piece, 0, false);
   const long long g_stride = static_cast<long long>(p.H + 2 * p.KV) * D;
-  u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(p.H + kv) * D;
-  const float by_scale[2] = {p.scale, p.scale}, one[2] = {1.f, 1.f};
-  store_rows<TR, D>(smem + wid * kStripBytes<D>, dk, by_scale, out, g_stride, kw, len, p.T, lane);
-  store_rows<TR, D>(smem + wid * kStripBytes<D>, dv, one, out + static_cast<long long>(p.KV) * D, g_stride, kw, len, p.T, lane);
+  u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(p.H + kv + is_dv * p.KV) * D;
+  const float scale = is_dv ? 1.f : p.scale;
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const int key = kw + 16 * kt + li;
+    if (key >= p.T) continue;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      u16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = key < len ? TR::from_f32(sum[kt][q][e] * scale) : static_cast<u16>(0);
+      *reinterpret_cast<u16x4*>(out + key * g_stride + 16 * (wid * Q + q) + 4 * g) = v;
+    }
+  }
 }
 
 // More than 64 KiB of dynamic LDS has to be asked for.
@@ -877,7 +907,7 @@ void launch_window_attention_bwd(const WindowAttnArgs& args, int dtype, hipStrea
     allow_lds(dkdv, kDkdvLds<D>);
     hipLaunchKernelGGL(dq, grid, dim3(kThreads), kQueryLds<D>, stream, a);
     hipLaunchKernelGGL(dkdv, dim3(static_cast<unsigned>(a.pieces)), dim3(kThreads), kDkdvLds<D>, stream, a);
-    if (a.pieces > 1) hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(a.pieces - 1)), dim3(kThreads), 4 * kStripBytes<D>, stream, a);
+    if (a.pieces > 1) hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(a.pieces - 1), 8), dim3(kThreads), 0, stream, a);
   });
 }
 
