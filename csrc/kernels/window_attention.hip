@@ -262,6 +262,8 @@ __device__ __forceinline__ bool hidden(const WindowAttnArgs& p, int j, int rel, 
   if (BORDER == kSeveral) return j > rel || (j <= rel - p.window && j >= sink);
   return false;
 }
+// Keeps a selection in front of the conversion that follows it: behind it, values are converted one by one instead of in pairs.
+__device__ __forceinline__ void stay_f32(float& x) { asm volatile("" : "+v"(x)); }
 // f(std::integral_constant<int, border>) for a border other than kUnseen.
 template <typename F>
 __device__ __forceinline__ void with_border(int border, F&& f) {
@@ -297,7 +299,7 @@ __device__ __forceinline__ void fwd_half(const WindowAttnArgs& p, const char* ks
       for (int st = 0; st < 2; ++st) s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
     }
   }
-  s16x8 pf[2];
+  float mx[2];
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
     if (BORDER != kClear) {  // register (t, e) is key k0 + 4 g + 16 t + e
@@ -306,22 +308,33 @@ __device__ __forceinline__ void fwd_half(const WindowAttnArgs& p, const char* ks
       for (int i = 0; i < 8; ++i)
         if (hidden<BORDER>(p, 16 * (i >> 2) + (i & 3), rel, sink)) s[st][i >> 2][i & 3] = kNegInf;
     }
-    float mx = s[st][0][0];
+    mx[st] = s[st][0][0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[st][i >> 2][i & 3]);
-    mx *= c;  // c > 0
-    if (__any(mx > m[st] + kDefer)) {
-      const float mg = groups_max(mx);
+    for (int i = 1; i < 8; ++i) mx[st] = fmaxf(mx[st], s[st][i >> 2][i & 3]);
+    mx[st] *= c;  // c > 0
+  }
+  if (__any(mx[0] > m[0] + kDefer || mx[1] > m[1] + kDefer)) {
+    // Rare.  The rescale is done in place, as assembly: as plain products the accumulators would get new registers here, and every pass that
+    // does NOT come this way would pay 42 moves a strip to reconcile the two.  The assembly waits out the matrix pipe itself.
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const float mg = groups_max(mx[st]);
       const float m_new = mg > m[st] + kDefer ? mg : m[st];
       const float alpha = __builtin_amdgcn_exp2f(m[st] - m_new);
       m[st] = m_new;
 #pragma unroll
       for (int td = 0; td < D / 16; ++td)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[st][td][e] *= alpha;
+        for (int e = 0; e < 4; ++e) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(o[st][td][e]) : "v"(alpha));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) lsum[st][e] *= alpha;
+      for (int e = 0; e < 4; ++e) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(lsum[st][e]) : "v"(alpha));
     }
+    asm volatile("s_nop 4" ::: "memory");  // and the products leave the vector pipe before a matrix instruction reads them
+  }
+  s16x8 pf[2];
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
     const float nm = -m[st];
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[st][i >> 2][i & 3] = __builtin_amdgcn_exp2f(fmaf(s[st][i >> 2][i & 3], c, nm));
@@ -455,7 +468,9 @@ __device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks,
       const int t = i >> 2, e = i & 3;
       const float pe = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, -lse2[st]));
       const float ds = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
-      s[st][t][e] = hidden<BORDER>(p, 16 * t + e, rel, sink) ? 0.f : ds;
+      float kept = hidden<BORDER>(p, 16 * t + e, rel, sink) ? 0.f : ds;
+      if (BORDER != kClear) stay_f32(kept);
+      s[st][t][e] = kept;
     }
     dsf[st] = pack8<TR>(s[st][0], s[st][1]);
   }
@@ -642,6 +657,10 @@ __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* q
                           : BORDER == kSinks  ? !sink
                                               : BORDER == kSeveral && (i < rel || i >= far || i >= end);
         if (hide) pe = ds = 0.f;
+        if (BORDER != kClear) {
+          stay_f32(pe);
+          stay_f32(ds);
+        }
         s[kt][qs][e] = pe;
         dp[kt][qs][e] = ds;
       }
@@ -665,16 +684,55 @@ constexpr long long kPartialFloats = 2LL * kRows * D;
 
 __device__ __forceinline__ long long piece_start(const WindowAttnArgs& p, long long total, int w) { return total * w / p.pieces; }
 
+// A key block of the unit list and the part of it that belongs to a piece.
+struct Part {
+  int b, kv, kb;
+  long long start, stop;  // the block's units
+  int len, n, ne;         // sequence length; query tiles per head at full length, and those that hold anything
+  int ua, left;           // the part's first unit in the block; how many of its units are walked (those with a tile index below ne)
+  __device__ __forceinline__ void open(const WindowAttnArgs& p, const Units& units, long long u0, long long u1) {
+    len = length_of(p, b);
+    n = units.tiles(kb);
+    stop = start + static_cast<long long>(n) * units.G;
+    ne = (len + kTile - 1) / kTile - 2 * kb;
+    ne = ne < 0 ? 0 : ne < n ? ne : n;
+    ua = u0 > start ? static_cast<int>(u0 - start) : 0;
+    const int ub = stop <= u1 ? n * units.G : static_cast<int>(u1 - start);
+    left = walked(ub, units.G) - walked(ua, units.G);
+  }
+  __device__ __forceinline__ int walked(int x, int G) const {
+    if (x == 0) return 0;
+    if (x == n * G) return ne * G;
+    const int q = x / n, r = x - q * n;
+    return q * ne + (r < ne ? r : ne);
+  }
+  __device__ __forceinline__ void next(const WindowAttnArgs& p, const Units& units, long long u0, long long u1) {
+    start = stop;
+    if (++kb == units.n_blocks) {
+      kb = 0;
+      if (++kv == p.KV) {
+        kv = 0;
+        ++b;
+      }
+    }
+    open(p, units, u0, u1);
+  }
+};
+
+// A piece is walked as one stream: the requests run two units ahead of the products, across the end of a block into the next one, and the
+// next block's K and V rows are fetched while the finished one is stored (18 KiB of LDS of its own for that), so only a piece's first
+// block waits for memory.  (Starting every block by itself -- unit arithmetic with 64-bit divisions, requests, K / V, two trips to memory --
+// cost about as much as 4 of its 6 units at a window of 256.)
 template <typename TR, int D>
 __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(WindowAttnArgs p) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stages][Q | dO | lse2 | delta], then the output strips
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stages][Q | dO | lse2 | delta] | output strips
   constexpr int S = kDkdvStages, TB = kTileBytes<D>, SB = kDkdvStageBytes<D>, NP = TileSource<D>::kPieces;
   const int G = p.H / p.KV;
   const Units units(p.T, p.window, p.sinks, G);
   const long long per_head = units.all(), total = per_head * p.KV * p.B;
   const int piece = xcd_order(blockIdx.x, p.pieces);
-  long long u = piece_start(p, total, piece);
-  const long long u_end = piece_start(p, total, piece + 1);
+  const long long u0 = piece_start(p, total, piece), u1 = piece_start(p, total, piece + 1);
+  if (u0 >= u1) return;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, li = lane & 15;
   const long long o_stride = static_cast<long long>(p.H) * D, g_stride = static_cast<long long>(p.H + 2 * p.KV) * D;
@@ -684,97 +742,128 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
   const unsigned lds0 = lds_address(smem);
   const unsigned dst = lds0 + (moves_do ? TB : 0) + (wid & 1) * NP * 1024;
   const unsigned stat_dst = lds0 + 2 * TB + (moves_do ? kTile * 4 : 0);
+  char* const strip = smem + S * SB + wid * kStripBytes<D>;
 
-  while (u < u_end) {
-    const long long bk = u / per_head, in_head = u - bk * per_head;
-    const int b = static_cast<int>(bk / p.KV), kv = static_cast<int>(bk - static_cast<long long>(b) * p.KV);
-    const int kb = units.block_of(in_head);
-    const long long start = bk * per_head + units.before(kb);
-    const int n = units.tiles(kb);                              // query tiles per head, at full length
-    const long long stop = start + static_cast<long long>(n) * G;
-    const long long upto = stop < u_end ? stop : u_end;
-    const int len = length_of(p, b), k0 = kb * kRows, kw = k0 + wid * 32;
-    const int first_qt = 2 * kb;
-    int ne = (len + kTile - 1) / kTile - first_qt;              // query tiles that hold anything
-    ne = ne < 0 ? 0 : ne < n ? ne : n;
-    // this piece's part of the block: units ua .. ub - 1 of it, of which those with a tile index below ne are walked
-    const int ua = static_cast<int>(u - start), ub = static_cast<int>(upto - start);
-    auto walked = [&](int x) { const int q = x / n, r = x - q * n; return q * ne + (r < ne ? r : ne); };
-    const int steps = walked(ub) - walked(ua);
-    int rg = ua / n, rt = ua - rg * n;                          // request cursor: head of the group, tile
-    if (rt >= ne) { rt = 0; ++rg; }
-    int ct = rt;                                                // tile being multiplied
-    const u16* base = static_cast<const u16*>(p.qkv) + static_cast<long long>(b) * p.batch_stride;
-    auto request = [&](int stage) {
-      const int row = (first_qt + rt) * kTile, h = kv * G + rg;
-      const u16* src = moves_do ? static_cast<const u16*>(p.d_o) + (static_cast<long long>(b) * p.T + row) * o_stride + static_cast<long long>(h) * D
-                                : base + static_cast<long long>(row) * p.row_stride + static_cast<long long>(h) * D;
-      ts.request(src, len - row, dst + stage * SB);
-      if (moves_stat) {
-        const float* st = (moves_do ? p.delta : p.lse2) + (static_cast<long long>(b) * p.H + h) * p.T + row;
-        const int i = lane < len - row ? lane : len - row - 1;
-        dma_4B(uniform_ptr(st), static_cast<unsigned>(i) * 4u, stat_dst + stage * SB);
+  Part cp;  // the part being multiplied
+  {
+    const long long bk = u0 / per_head;
+    cp.b = static_cast<int>(bk / p.KV);
+    cp.kv = static_cast<int>(bk - static_cast<long long>(cp.b) * p.KV);
+    cp.kb = units.block_of(u0 - bk * per_head);
+    cp.start = bk * per_head + units.before(cp.kb);
+    cp.open(p, units, u0, u1);
+  }
+  Part rp = cp;  // the part being requested, with the head of the group and the tile that come next
+  int rg = rp.ua / rp.n, rt = rp.ua - rg * rp.n;
+  auto tile_in_part = [](const Part& q, int& head, int& tile) {  // a unit beyond the sequence: the next head's first
+    if (tile >= q.ne) {
+      tile = 0;
+      ++head;
+    }
+  };
+  tile_in_part(rp, rg, rt);
+  int ahead = 0, fill = 0;  // units requested and not multiplied yet; stage that is filled next
+  auto request = [&]() __attribute__((always_inline)) {
+    while (rp.left == 0) {
+      if (rp.stop >= u1) return;
+      rp.next(p, units, u0, u1);
+      rg = rt = 0;
+    }
+    const int row = (2 * rp.kb + rt) * kTile, h = rp.kv * G + rg;
+    const u16* src = moves_do ? static_cast<const u16*>(p.d_o) + (static_cast<long long>(rp.b) * p.T + row) * o_stride + static_cast<long long>(h) * D
+                              : static_cast<const u16*>(p.qkv) + static_cast<long long>(rp.b) * p.batch_stride +
+                                    static_cast<long long>(row) * p.row_stride + static_cast<long long>(h) * D;
+    ts.request(src, rp.len - row, dst + fill * SB);
+    if (moves_stat) {
+      const float* st = (moves_do ? p.delta : p.lse2) + (static_cast<long long>(rp.b) * p.H + h) * p.T + row;
+      const int i = lane < rp.len - row ? lane : rp.len - row - 1;
+      dma_4B(uniform_ptr(st), static_cast<unsigned>(i) * 4u, stat_dst + fill * SB);
+    }
+    if (++rt == rp.ne) {
+      rt = 0;
+      ++rg;
+    }
+    --rp.left;
+    ++ahead;
+    fill = fill + 1 == S ? 0 : fill + 1;
+  };
+  s16x8 kf[2][D / 32], vf[2][D / 32];
+  auto load_kv = [&](const Part& q) __attribute__((always_inline)) {
+    const u16* K = static_cast<const u16*>(p.qkv) + static_cast<long long>(q.b) * p.batch_stride + static_cast<long long>(p.H + q.kv) * D;
+    const u16* V = K + static_cast<long long>(p.KV) * D;
+    const int kw = q.kb * kRows + wid * 32;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const long long key = kw + 16 * kt + li < q.len ? kw + 16 * kt + li : (q.len > 0 ? q.len - 1 : 0);
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk) {
+        kf[kt][kk] = *reinterpret_cast<const s16x8*>(K + key * p.row_stride + 32 * kk + 8 * g);
+        vf[kt][kk] = *reinterpret_cast<const s16x8*>(V + key * p.row_stride + 32 * kk + 8 * g);
       }
-      if (++rt == ne) { rt = 0; ++rg; }
-    };
+    }
+  };
+  request();
+  request();
+  load_kv(cp);
+  int stage = 0;
+  bool stored_whole = false;  // the last part left exactly kStores stores per wave behind its K / V loads
+  constexpr int kStores = 2 * 32 / (64 / (D / 8));
+
+  while (true) {
+    const int kw = cp.kb * kRows + wid * 32, len = cp.len;
     f32x4 dk[2][D / 16], dv[2][D / 16];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int td = 0; td < D / 16; ++td) dk[kt][td] = dv[kt][td] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (steps > 0) {
-      __syncthreads();  // the previous block's output strips (same memory) have been read back
-      request(0);
-      if (steps > 1) request(1);
-      s16x8 kf[2][D / 32], vf[2][D / 32];
-      const u16* K = base + static_cast<long long>(p.H + kv) * D;
-      const u16* V = K + static_cast<long long>(p.KV) * D;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const long long key = kw + 16 * kt + li < len ? kw + 16 * kt + li : len - 1;
-#pragma unroll
-        for (int kk = 0; kk < D / 32; ++kk) {
-          kf[kt][kk] = *reinterpret_cast<const s16x8*>(K + key * p.row_stride + 32 * kk + 8 * g);
-          vf[kt][kk] = *reinterpret_cast<const s16x8*>(V + key * p.row_stride + 32 * kk + 8 * g);
-        }
+    int ct = cp.ua - (cp.ua / cp.n) * cp.n;  // tile being multiplied
+    if (ct >= cp.ne) ct = 0;
+    for (int it = 0; it < cp.left; ++it) {
+      // This wave's pieces of the unit have landed.  A part's first unit is older than its K / V loads; behind those only the stores of the part before.
+      if (it == 0) {
+        if (stored_whole) wait_vmem_at_most<kStores>();
+        else wait_vmem_at_most<0>();
+      } else if (ahead > 1) {
+        if (moves_stat) wait_vmem_at_most<NP + 1>();
+        else wait_vmem_at_most<NP>();
+      } else {
+        wait_vmem_at_most<0>();
       }
-      wait_vmem_at_most<0>();
-      int stage = 0;
-      for (int it = 0; it < steps; ++it) {
-        if (it + 1 < steps) {
-          if (moves_stat) wait_vmem_at_most<NP + 1>();
-          else wait_vmem_at_most<NP>();
-        } else {
-          wait_vmem_at_most<0>();
-        }
-        __syncthreads();
-        if (it + 2 < steps) request(stage == 0 ? 2 : stage - 1);
-        const char* qs = smem + stage * SB;
+      __syncthreads();  // everybody's have; nobody still reads the stage that is filled next
+      --ahead;
+      request();
+      const char* qs = smem + stage * SB;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int q0 = (first_qt + ct) * kTile + 32 * half;
-          // as border_of, with the 32 queries and the wave's keys in each other's place, and the end of the sequence as one more border
-          const bool past = q0 + 31 >= kw + p.window && kw + 31 >= p.sinks, gone = q0 >= kw + 31 + p.window;
-          if (q0 + 31 < kw || (past && gone && kw >= p.sinks) || q0 >= len) continue;
-          const bool future = q0 < kw + 31, ends = q0 + 31 >= len;
-          const int border = ends ? kSeveral : !past ? (future ? kCausal : kClear) : gone ? kSinks : future || kw < p.sinks ? kSeveral : kWindow;
-          with_border(border, [&](auto b_c) __attribute__((always_inline)) {
-            dkdv_half<TR, D, decltype(b_c)::value>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
-          });
-        }
-        if (++ct == ne) ct = 0;
-        stage = stage + 1 == S ? 0 : stage + 1;
+      for (int half = 0; half < 2; ++half) {
+        const int q0 = (2 * cp.kb + ct) * kTile + 32 * half;
+        // as border_of, with the 32 queries and the wave's keys in each other's place, and the end of the sequence as one more border
+        const bool past = q0 + 31 >= kw + p.window && kw + 31 >= p.sinks, gone = q0 >= kw + 31 + p.window;
+        if (q0 + 31 < kw || (past && gone && kw >= p.sinks) || q0 >= len) continue;
+        const bool future = q0 < kw + 31, ends = q0 + 31 >= len;
+        const int border = ends ? kSeveral : !past ? (future ? kCausal : kClear) : gone ? kSinks : future || kw < p.sinks ? kSeveral : kWindow;
+        with_border(border, [&](auto b_c) __attribute__((always_inline)) {
+          dkdv_half<TR, D, decltype(b_c)::value>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
+        });
       }
+      if (++ct == cp.ne) ct = 0;
+      stage = stage + 1 == S ? 0 : stage + 1;
     }
-    if (u == start && upto == stop) {
-      __syncthreads();  // tile stages -> output strips
-      u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(p.H + kv) * D;
+    const Part done = cp;
+    const bool last = cp.stop >= u1;
+    if (!last) {
+      cp.next(p, units, u0, u1);
+      load_kv(cp);
+    }
+    stored_whole = false;
+    if (done.ua == 0 && done.stop <= u1) {
+      u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(done.b) * p.T * g_stride + static_cast<long long>(p.H + done.kv) * D;
       const float by_scale[2] = {p.scale, p.scale}, one[2] = {1.f, 1.f};
-      store_rows<TR, D>(smem + wid * kStripBytes<D>, dk, by_scale, out, g_stride, kw, len, p.T, lane);
-      store_rows<TR, D>(smem + wid * kStripBytes<D>, dv, one, out + static_cast<long long>(p.KV) * D, g_stride, kw, len, p.T, lane);
+      store_rows<TR, D>(strip, dk, by_scale, out, g_stride, kw, len, p.T, lane);
+      store_rows<TR, D>(strip, dv, one, out + static_cast<long long>(p.KV) * D, g_stride, kw, len, p.T, lane);
+      stored_whole = kw + 32 <= p.T;
     } else {
       // slot 0: the block began in an earlier piece; slot 1: it began here
-      f32x4* ws = reinterpret_cast<f32x4*>(p.partial + (2LL * piece + (u == start ? 1 : 0)) * kPartialFloats<D>) + wid * (4 * (D / 16) * 64) + lane;
+      f32x4* ws = reinterpret_cast<f32x4*>(p.partial + (2LL * piece + (done.ua == 0 ? 1 : 0)) * kPartialFloats<D>) + wid * (4 * (D / 16) * 64) + lane;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -783,7 +872,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
           ws[((2 + kt) * (D / 16) + td) * 64] = dv[kt][td];
         }
     }
-    u = upto;
+    if (last) return;
   }
 }
 
@@ -845,7 +934,7 @@ void allow_lds(Kernel k, int bytes) {
 template <int D>
 constexpr int kQueryLds = kStages<D> * 2 * kTileBytes<D> > 4 * kStripBytes<D> ? kStages<D> * 2 * kTileBytes<D> : 4 * kStripBytes<D>;
 template <int D>
-constexpr int kDkdvLds = kDkdvStages * kDkdvStageBytes<D> > 4 * kStripBytes<D> ? kDkdvStages * kDkdvStageBytes<D> : 4 * kStripBytes<D>;
+constexpr int kDkdvLds = kDkdvStages * kDkdvStageBytes<D> + 4 * kStripBytes<D>;
 
 template <typename F>
 void dispatch(int dtype, int D, F&& f) {
