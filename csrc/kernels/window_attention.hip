@@ -262,16 +262,28 @@ __device__ __forceinline__ bool hidden(const WindowAttnArgs& p, int j, int rel, 
   if (BORDER == kSeveral) return j > rel || (j <= rel - p.window && j >= sink);
   return false;
 }
-// Keeps a selection in front of the conversion that follows it: behind it, values are converted one by one instead of in pairs.
-__device__ __forceinline__ void stay_f32(float& x) { asm volatile("" : "+v"(x)); }
-// f(std::integral_constant<int, border>) for a border other than kUnseen.
+// f(std::integral_constant<int, border>) for a border other than kClear and kUnseen.
 template <typename F>
 __device__ __forceinline__ void with_border(int border, F&& f) {
-  if (border == kClear) f(std::integral_constant<int, kClear>{});
-  else if (border == kCausal) f(std::integral_constant<int, kCausal>{});
+  if (border == kCausal) f(std::integral_constant<int, kCausal>{});
   else if (border == kWindow) f(std::integral_constant<int, kWindow>{});
   else if (border == kSinks) f(std::integral_constant<int, kSinks>{});
   else f(std::integral_constant<int, kSeveral>{});
+}
+// Scores of hidden pairs become -inf: their probabilities are then exactly 0, and with them all they contribute.  Register (t, e) of s[st] is query
+// qw + 16 st + (lane & 15) and key k0 + 16 t + 4 (lane >> 4) + e.  (Only this step depends on the border.  With the whole square instantiated for each,
+// the five copies' accumulators met in 42 moves a square.)
+__device__ __forceinline__ void hide_keys(const WindowAttnArgs& p, f32x4 (&s)[2][2], int qw, int k0, int border, int lane) {
+  if (border == kClear) return;
+  with_border(border, [&](auto b_c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const int rel = qw + 16 * st + (lane & 15) - k0 - 4 * (lane >> 4), sink = p.sinks - k0 - 4 * (lane >> 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (hidden<decltype(b_c)::value>(p, 16 * (i >> 2) + (i & 3), rel, sink)) s[st][i >> 2][i & 3] = kNegInf;
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------- forward
@@ -282,10 +294,9 @@ constexpr float kDefer = 8.f;
 constexpr float kLowest = -1e30f;  // a start below every score that keeps exp2(-inf - m) at zero where a query sees nothing yet
 
 // The 32 keys in rows 32 half .. of a tile, key k0 first.
-template <typename TR, int D, int BORDER>
+template <typename TR, int D>
 __device__ __forceinline__ void fwd_half(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], f32x4 (&o)[2][D / 16],
-                                         float (&m)[2], f32x4 (&lsum)[2], int half, int k0, int qw, int lane) {
-  const int g = lane >> 4, li = lane & 15;
+                                         float (&m)[2], f32x4 (&lsum)[2], int half, int k0, int qw, int border, int lane) {
   const float c = p.scale_log2;
   f32x4 s[2][2];
 #pragma unroll
@@ -299,15 +310,10 @@ __device__ __forceinline__ void fwd_half(const WindowAttnArgs& p, const char* ks
       for (int st = 0; st < 2; ++st) s[st][t] = mfma<TR>(kf, qf[st][kk], s[st][t]);
     }
   }
+  hide_keys(p, s, qw, k0, border, lane);
   float mx[2];
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
-    if (BORDER != kClear) {  // register (t, e) is key k0 + 4 g + 16 t + e
-      const int rel = qw + 16 * st + li - k0 - 4 * g, sink = p.sinks - k0 - 4 * g;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (hidden<BORDER>(p, 16 * (i >> 2) + (i & 3), rel, sink)) s[st][i >> 2][i & 3] = kNegInf;
-    }
     mx[st] = s[st][0][0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) mx[st] = fmaxf(mx[st], s[st][i >> 2][i & 3]);
@@ -419,10 +425,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       const int k0 = key0 + 32 * half, border = border_of(p, qw, k0);
-      if (border != kUnseen)
-        with_border(border, [&](auto b_c) __attribute__((always_inline)) {
-          fwd_half<TR, D, decltype(b_c)::value>(p, ks, ks + TB, qf, o, m, lsum, half, k0, qw, lane);
-        });
+      if (border != kUnseen) fwd_half<TR, D>(p, ks, ks + TB, qf, o, m, lsum, half, k0, qw, border, lane);
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -439,10 +442,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
 }
 
 // ---------------------------------------------------------------------------------------------------- backward: dQ
-template <typename TR, int D, int BORDER>
+template <typename TR, int D>
 __device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], const s16x8 (&dof)[2][D / 32],
-                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const float (&delta)[2], int half, int k0, int qw, int lane) {
-  const int g = lane >> 4, li = lane & 15;
+                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const float (&delta)[2], int half, int k0, int qw, int border, int lane) {
   const float c = p.scale_log2;
   f32x4 s[2][2], dp[2][2];
 #pragma unroll
@@ -459,18 +461,15 @@ __device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks,
       }
     }
   }
+  hide_keys(p, s, qw, k0, border, lane);
   s16x8 dsf[2];
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
-    const int rel = qw + 16 * st + li - k0 - 4 * g, sink = p.sinks - k0 - 4 * g;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int t = i >> 2, e = i & 3;
       const float pe = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, -lse2[st]));
-      const float ds = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
-      float kept = hidden<BORDER>(p, 16 * t + e, rel, sink) ? 0.f : ds;
-      if (BORDER != kClear) stay_f32(kept);
-      s[st][t][e] = kept;
+      s[st][t][e] = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
     }
     dsf[st] = pack8<TR>(s[st][0], s[st][1]);
   }
@@ -552,10 +551,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       const int k0 = key0 + 32 * half, border = border_of(p, qw, k0);
-      if (border != kUnseen)
-        with_border(border, [&](auto b_c) __attribute__((always_inline)) {
-          dq_half<TR, D, decltype(b_c)::value>(p, ks, ks + TB, qf, dof, dq, lse2, delta, half, k0, qw, lane);
-        });
+      if (border != kUnseen) dq_half<TR, D>(p, ks, ks + TB, qf, dof, dq, lse2, delta, half, k0, qw, border, lane);
     }
     stage = stage + 1 == S ? 0 : stage + 1;
   }
@@ -610,12 +606,12 @@ template <int D>
 constexpr int kDkdvStageBytes = 2 * kTileBytes<D> + 2 * kTile * 4;  // Q | dO | lse2 | delta
 constexpr int kDkdvStages = 3;
 
-template <typename TR, int D, int BORDER>
+template <typename TR, int D>
 __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* qs_, const char* dos_, const char* stats, const s16x8 (&kf)[2][D / 32],
                                           const s16x8 (&vf)[2][D / 32], f32x4 (&dk)[2][D / 16], f32x4 (&dv)[2][D / 16], int half, int q0, int kw,
-                                          int len, int lane) {
+                                          int len, int border, int lane) {
   // the 32 queries from q0, rows 32 half .. of the stage's tiles, against the wave's 32 keys from kw
-  const int g = lane >> 4, li = lane & 15;
+  const int g = lane >> 4;
   const float c = p.scale_log2;
   f32x4 l2[2], dl[2];  // register (qs, e): query q0 + 16 qs + 4 g + e
 #pragma unroll
@@ -638,32 +634,37 @@ __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* q
       }
     }
   }
+  if (border != kClear) {
+    with_border(border, [&](auto b_c) __attribute__((always_inline)) {
+      constexpr int BORDER = decltype(b_c)::value;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int key = kw + 16 * kt + (lane & 15), rel = key - q0 - 4 * g;  // register (qs, e) is query index 16 qs + e against rel
+        const bool sink = key < p.sinks;
+        const int far = BORDER == kSeveral && sink ? 0x7fffffff : rel + p.window;  // first index beyond the window
+        const int end = len - q0 - 4 * g;                                            // first index beyond the sequence
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = 16 * (j >> 2) + (j & 3);
+          const bool hide = BORDER == kCausal   ? i < rel
+                            : BORDER == kWindow ? i >= far
+                            : BORDER == kSinks  ? !sink
+                                                : i < rel || i >= far || i >= end;
+          if (hide) s[kt][j >> 2][j & 3] = kNegInf;
+        }
+      }
+    });
+  }
   s16x8 pB[2], dsB[2];
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    const int key = kw + 16 * kt + li, rel = key - q0 - 4 * g;  // register (qs, e) is query index 16 qs + e against rel
-    const bool sink = key < p.sinks;
-    const int far = BORDER == kSeveral && sink ? 0x7fffffff : rel + p.window;  // first index beyond the window
-    const int end = len - q0 - 4 * g;                                            // first index beyond the sequence
 #pragma unroll
-    for (int qs = 0; qs < 2; ++qs)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 16 * qs + e;
-        float pe = __builtin_amdgcn_exp2f(fmaf(s[kt][qs][e], c, -l2[qs][e]));
-        float ds = pe * (dp[kt][qs][e] - dl[qs][e]);
-        const bool hide = BORDER == kCausal   ? i < rel
-                          : BORDER == kWindow ? i >= far
-                          : BORDER == kSinks  ? !sink
-                                              : BORDER == kSeveral && (i < rel || i >= far || i >= end);
-        if (hide) pe = ds = 0.f;
-        if (BORDER != kClear) {
-          stay_f32(pe);
-          stay_f32(ds);
-        }
-        s[kt][qs][e] = pe;
-        dp[kt][qs][e] = ds;
-      }
+    for (int j = 0; j < 8; ++j) {
+      const int qs = j >> 2, e = j & 3;
+      const float pe = __builtin_amdgcn_exp2f(fmaf(s[kt][qs][e], c, -l2[qs][e]));
+      s[kt][qs][e] = pe;
+      dp[kt][qs][e] = pe * (dp[kt][qs][e] - dl[qs][e]);
+    }
     pB[kt] = pack8<TR>(s[kt][0], s[kt][1]);
     dsB[kt] = pack8<TR>(dp[kt][0], dp[kt][1]);
   }
@@ -841,9 +842,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
         if (q0 + 31 < kw || (past && gone && kw >= p.sinks) || q0 >= len) continue;
         const bool future = q0 < kw + 31, ends = q0 + 31 >= len;
         const int border = ends ? kSeveral : !past ? (future ? kCausal : kClear) : gone ? kSinks : future || kw < p.sinks ? kSeveral : kWindow;
-        with_border(border, [&](auto b_c) __attribute__((always_inline)) {
-          dkdv_half<TR, D, decltype(b_c)::value>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, lane);
-        });
+        dkdv_half<TR, D>(p, qs, qs + TB, qs + 2 * TB, kf, vf, dk, dv, half, q0, kw, len, border, lane);
       }
       if (++ct == cp.ne) ct = 0;
       stage = stage + 1 == S ? 0 : stage + 1;
