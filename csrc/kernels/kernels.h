@@ -349,11 +349,15 @@ struct WindowAttnArgs {
   long long row_stride, batch_stride;
   int B, T, H, KV, D, window, sinks;
   float scale;      // > 0
-  int compute_units, pieces;
+  int compute_units;
+  // window_attention_plan(): the work of the dK/dV kernel and the pieces it is cut into
+  int pieces, piece_rest;
+  int cuts;                 // key blocks of a head, from its first, that a piece may end in; 0: no partial sums
+  long long units_per_head, piece_units;
   float scale_log2; // set by the launcher
 };
 bool window_attention_supported(long long B, long long T, long long H, long long KV, long long D, long long row_stride, int dtype);
-int window_attention_pieces(const WindowAttnArgs& a);  // workgroups of the dK/dV kernel: a.pieces
+void window_attention_plan(WindowAttnArgs& a);  // for a backward; needs compute_units and the sizes
 long long window_attention_partial_floats(const WindowAttnArgs& a);
 void launch_window_attention_fwd(const WindowAttnArgs& a, int dtype, hipStream_t stream);
 void launch_window_attention_bwd(const WindowAttnArgs& a, int dtype, hipStream_t stream);

@@ -14,9 +14,9 @@
 // products run transposed (S^T = K Q^T), so a query's softmax statistics are scalars of its lane and the probabilities leave the
 // accumulators as the operand of the next product without changing lanes; the other operand of that product comes
 // from the row-major tile through the transposing LDS read.  Tiles travel global -> LDS by DMA through a ring, requested one or two
-// tiles ahead.  The tile image is one for both kinds of reads: 16-byte chunk c of row r sits at chunk c ^ swz(r), which
-// puts the 16 rows of a row-wise read on 16 different 16-byte bank groups and the 8 rows of a transposing read on 8
-// different 32-byte groups.
+// tile ahead.  The tile image is one for both kinds of reads: 16-byte chunk c of row r sits at chunk c ^ swz(r).  The 16 lanes that a row-wise
+// read serves at once (rows 0-3 and 12-15 at one chunk, rows 4-11 at the next) then fall on 16 different 16-byte bank groups, and the 8
+// rows of a transposing read on 8 different 32-byte groups.
 // Rows at and beyond a sequence's length are never read: source rows are clamped to the last valid one, what they
 // would contribute is masked, and their outputs and gradients are written as zero.
 //
@@ -70,7 +70,7 @@ __device__ __forceinline__ s16x8 pack8(const f32x4& a, const f32x4& b) {
 // Byte offset of 16-byte chunk c of row r in a tile image of [rows][D] 16-bit elements.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
-  return D == 64 ? (((r >> 1) & 3) << 1 | ((r >> 3) & 1)) : ((r & 7) << 1 | ((r >> 3) & 1));
+  return D == 64 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
 }
 template <int D>
 __device__ __forceinline__ int tile_off(int r, int c) { return r * (2 * D) + ((c ^ swz<D>(r)) << 4); }
@@ -170,8 +170,6 @@ struct TileSource {
 
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
-template <int D>
-constexpr int kStages = D == 64 ? 3 : 2;  // two workgroups of D = 128 tiles per CU
 template <int D>
 constexpr int kStripPitch = 2 * D + 16;
 template <int D>
@@ -369,9 +367,9 @@ __device__ __forceinline__ void query_item(const WindowAttnArgs& p, int& b, int&
 }
 
 template <typename TR, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs p) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void window_fwd_kernel(WindowAttnArgs p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stages][K | V], then the output strips
-  constexpr int S = kStages<D>, TB = kTileBytes<D>, NP = TileSource<D>::kPieces;
+  constexpr int TB = kTileBytes<D>, NP = TileSource<D>::kPieces;
   int b, h, qb;
   query_item(p, b, h, qb);
   const int q0 = qb * kRows, len = length_of(p, b);
@@ -397,7 +395,6 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
     ts.request(src + static_cast<long long>(k0) * p.row_stride, tiles.valid(p, it, len), dst + stage * 2 * TB);
   };
   request(0, 0);
-  if (S > 2 && tiles.count > 1) request(1, 1);
   s16x8 qf[2][D / 32];
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
@@ -416,10 +413,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
   wait_vmem_at_most<0>();
   int stage = 0;
   for (int it = 0; it < tiles.count; ++it) {
-    if (S > 2 && it + 1 < tiles.count) wait_vmem_at_most<NP>();  // this wave's pieces of the tile have landed
-    else wait_vmem_at_most<0>();
-    __syncthreads();  // everybody's have; nobody still reads the stage that is requested next
-    if (it + S - 1 < tiles.count) request(it + S - 1, stage == 0 ? S - 1 : stage - 1);
+    wait_vmem_at_most<0>();  // this wave's pieces of the tile have landed
+    __syncthreads();         // everybody's have; nobody still reads the other stage
+    if (it + 1 < tiles.count) request(it + 1, stage ^ 1);
     const char* ks = smem + stage * 2 * TB;
     const int key0 = tiles.key0(it);
 #pragma unroll 1
@@ -427,7 +423,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
       const int k0 = key0 + 32 * half, border = border_of(p, qw, k0);
       if (border != kUnseen) fwd_half<TR, D>(p, ks, ks + TB, qf, o, m, lsum, half, k0, qw, border, lane);
     }
-    stage = stage + 1 == S ? 0 : stage + 1;
+    stage ^= 1;
   }
   float inv[2];
 #pragma unroll
@@ -444,13 +440,16 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WindowAttnArgs 
 // ---------------------------------------------------------------------------------------------------- backward: dQ
 template <typename TR, int D>
 __device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks, const char* vs, const s16x8 (&qf)[2][D / 32], const s16x8 (&dof)[2][D / 32],
-                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const float (&delta)[2], int half, int k0, int qw, int border, int lane) {
+                                        f32x4 (&dq)[2][D / 16], const float (&lse2)[2], const f32x4 (&minus_delta)[2], int half, int k0, int qw, int border, int lane) {
   const float c = p.scale_log2;
   f32x4 s[2][2], dp[2][2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int st = 0; st < 2; ++st) s[st][t] = dp[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int st = 0; st < 2; ++st) {
+      s[st][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      dp[st][t] = minus_delta[st];  // dp - delta without a subtraction per score
+    }
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk) {
       const s16x8 kf = row_frag<D>(ks, 2 * half + t, kk, lane), vf = row_frag<D>(vs, 2 * half + t, kk, lane);
@@ -469,7 +468,7 @@ __device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks,
     for (int i = 0; i < 8; ++i) {
       const int t = i >> 2, e = i & 3;
       const float pe = __builtin_amdgcn_exp2f(fmaf(s[st][t][e], c, -lse2[st]));
-      s[st][t][e] = pe * (dp[st][t][e] - delta[st]);  // the softmax scale is applied once, to the finished rows
+      s[st][t][e] = pe * dp[st][t][e];  // the softmax scale is applied once, to the finished rows
     }
     dsf[st] = pack8<TR>(s[st][0], s[st][1]);
   }
@@ -482,9 +481,9 @@ __device__ __forceinline__ void dq_half(const WindowAttnArgs& p, const char* ks,
 }
 
 template <typename TR, int D>
-__global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void window_dq_kernel(WindowAttnArgs p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  constexpr int S = kStages<D>, TB = kTileBytes<D>, NP = TileSource<D>::kPieces;
+  constexpr int TB = kTileBytes<D>, NP = TileSource<D>::kPieces;
   int b, h, qb;
   query_item(p, b, h, qb);
   const int q0 = qb * kRows, len = length_of(p, b);
@@ -510,13 +509,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p
     ts.request(src + static_cast<long long>(k0) * p.row_stride, tiles.valid(p, it, len), dst + stage * 2 * TB);
   };
   request(0, 0);
-  if (S > 2 && tiles.count > 1) request(1, 1);
   const long long ho = static_cast<long long>(b) * p.T * o_stride + static_cast<long long>(h) * D;
   const u16* O = static_cast<const u16*>(p.o) + ho;
   const u16* DO = static_cast<const u16*>(p.d_o) + ho;
   const long long stat = (static_cast<long long>(b) * p.H + h) * p.T;
   s16x8 qf[2][D / 32], dof[2][D / 32];
-  float lse2[2], delta[2];
+  float lse2[2];
+  f32x4 minus_delta[2];
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
     const bool live = qw + 16 * st + li < len;
@@ -531,8 +530,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p
       for (int j = 0; j < 8; ++j) part = fmaf(TR::to_f32(static_cast<u16>(dof[st][kk][j])), TR::to_f32(static_cast<u16>(of[j])), part);
     }
     lse2[st] = p.lse2[stat + qi];
-    delta[st] = groups_sum(part);  // the four lane groups hold D / 4 values each
-    if (g == 0 && live) p.delta[stat + qi] = delta[st];
+    const float delta = groups_sum(part);  // the four lane groups hold D / 4 values each
+    minus_delta[st] = f32x4{-delta, -delta, -delta, -delta};
+    if (g == 0 && live) p.delta[stat + qi] = -delta;  // as the dK/dV kernel wants it
   }
   f32x4 dq[2][D / 16];
 #pragma unroll
@@ -542,18 +542,17 @@ __global__ __launch_bounds__(kThreads, 2) void window_dq_kernel(WindowAttnArgs p
   wait_vmem_at_most<0>();
   int stage = 0;
   for (int it = 0; it < tiles.count; ++it) {
-    if (S > 2 && it + 1 < tiles.count) wait_vmem_at_most<NP>();
-    else wait_vmem_at_most<0>();
+    wait_vmem_at_most<0>();
     __syncthreads();
-    if (it + S - 1 < tiles.count) request(it + S - 1, stage == 0 ? S - 1 : stage - 1);
+    if (it + 1 < tiles.count) request(it + 1, stage ^ 1);
     const char* ks = smem + stage * 2 * TB;
     const int key0 = tiles.key0(it);
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       const int k0 = key0 + 32 * half, border = border_of(p, qw, k0);
-      if (border != kUnseen) dq_half<TR, D>(p, ks, ks + TB, qf, dof, dq, lse2, delta, half, k0, qw, border, lane);
+      if (border != kUnseen) dq_half<TR, D>(p, ks, ks + TB, qf, dof, dq, lse2, minus_delta, half, k0, qw, border, lane);
     }
-    stage = stage + 1 == S ? 0 : stage + 1;
+    stage ^= 1;
   }
   __syncthreads();
   const float by_scale[2] = {p.scale, p.scale};
@@ -604,7 +603,8 @@ struct Units {
 
 template <int D>
 constexpr int kDkdvStageBytes = 2 * kTileBytes<D> + 2 * kTile * 4;  // Q | dO | lse2 | delta
-constexpr int kDkdvStages = 3;
+template <int D>
+constexpr int kDkdvStages = D == 64 ? 2 : 3;
 
 template <typename TR, int D>
 __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* qs_, const char* dos_, const char* stats, const s16x8 (&kf)[2][D / 32],
@@ -613,25 +613,31 @@ __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* q
   // the 32 queries from q0, rows 32 half .. of the stage's tiles, against the wave's 32 keys from kw
   const int g = lane >> 4;
   const float c = p.scale_log2;
-  f32x4 l2[2], dl[2];  // register (qs, e): query q0 + 16 qs + 4 g + e
+  // D = 64: probabilities first, then dP -- the two products' operands and statistics are then not live together, which lets three waves share a
+  // SIMD (257 -> 211 us at 64 x 1024 x 12 heads).  D = 128 has one wave a SIMD either way and overlaps the two products instead (275 -> 241 us).
+  constexpr bool TOGETHER = D == 128;
+  f32x4 s[2][2], dp[2][2];  // register (qs, e): query q0 + 16 qs + 4 g + e
+  auto start_dp = [&](int qs) __attribute__((always_inline)) {
+    const f32x4 minus_delta = *reinterpret_cast<const f32x4*>(stats + (kTile + 32 * half + 16 * qs + 4 * g) * 4);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) dp[kt][qs] = minus_delta;  // dp - delta without a subtraction per score
+  };
+  auto step_dp = [&](int qs, int kk) __attribute__((always_inline)) {
+    const s16x8 dr = row_frag<D>(dos_, 2 * half + qs, kk, lane);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) dp[kt][qs] = mfma<TR>(dr, vf[kt][kk], dp[kt][qs]);
+  };
 #pragma unroll
   for (int qs = 0; qs < 2; ++qs) {
-    l2[qs] = *reinterpret_cast<const f32x4*>(stats + (32 * half + 16 * qs + 4 * g) * 4);
-    dl[qs] = *reinterpret_cast<const f32x4*>(stats + (kTile + 32 * half + 16 * qs + 4 * g) * 4);
-  }
-  f32x4 s[2][2], dp[2][2];
 #pragma unroll
-  for (int qs = 0; qs < 2; ++qs) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) s[kt][qs] = dp[kt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int kt = 0; kt < 2; ++kt) s[kt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (TOGETHER) start_dp(qs);
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk) {
-      const s16x8 qr = row_frag<D>(qs_, 2 * half + qs, kk, lane), dr = row_frag<D>(dos_, 2 * half + qs, kk, lane);
+      const s16x8 qr = row_frag<D>(qs_, 2 * half + qs, kk, lane);
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        s[kt][qs] = mfma<TR>(qr, kf[kt][kk], s[kt][qs]);
-        dp[kt][qs] = mfma<TR>(dr, vf[kt][kk], dp[kt][qs]);
-      }
+      for (int kt = 0; kt < 2; ++kt) s[kt][qs] = mfma<TR>(qr, kf[kt][kk], s[kt][qs]);
+      if (TOGETHER) step_dp(qs, kk);
     }
   }
   if (border != kClear) {
@@ -657,17 +663,33 @@ __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* q
   }
   s16x8 pB[2], dsB[2];
 #pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    const f32x4 l2 = *reinterpret_cast<const f32x4*>(stats + (32 * half + 16 * qs + 4 * g) * 4);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kt][qs][e] = __builtin_amdgcn_exp2f(fmaf(s[kt][qs][e], c, -l2[e]));
+  }
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) pB[kt] = pack8<TR>(s[kt][0], s[kt][1]);
+  if (!TOGETHER) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) {
+      start_dp(qs);
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk) step_dp(qs, kk);
+    }
+  }
+#pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int qs = j >> 2, e = j & 3;
-      const float pe = __builtin_amdgcn_exp2f(fmaf(s[kt][qs][e], c, -l2[qs][e]));
-      s[kt][qs][e] = pe;
-      dp[kt][qs][e] = pe * (dp[kt][qs][e] - dl[qs][e]);
-    }
-    pB[kt] = pack8<TR>(s[kt][0], s[kt][1]);
+    for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[kt][qs][e] *= s[kt][qs][e];
     dsB[kt] = pack8<TR>(dp[kt][0], dp[kt][1]);
   }
+  if (!TOGETHER) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int td = 0; td < D / 16; ++td) {
     const s16x8 dot = tr_frag<D>(dos_, 32 * half, td, lane), qt = tr_frag<D>(qs_, 32 * half, td, lane);
@@ -683,7 +705,31 @@ __device__ __forceinline__ void dkdv_half(const WindowAttnArgs& p, const char* q
 template <int D>
 constexpr long long kPartialFloats = 2LL * kRows * D;
 
-__device__ __forceinline__ long long piece_start(const WindowAttnArgs& p, long long total, int w) { return total * w / p.pieces; }
+// Where piece w of the unit list begins.  Equal pieces, but a boundary inside a short block moves to the block's nearer end: a cut costs 128 KiB (D = 64) of
+// partial sums written and read, the time of about eight units, and the move at most half a block.  Blocks longer than kShort units -- sinks, wide
+// windows, large groups -- and than a quarter of a piece are cut.
+constexpr int kShort = 16;
+__device__ __forceinline__ long long even_start(const WindowAttnArgs& p, int w) {
+  return p.piece_units * w + (w < p.piece_rest ? w : p.piece_rest);
+}
+__host__ __device__ __forceinline__ bool is_short(const WindowAttnArgs& p, long long units) { return units <= kShort || 4 * units <= p.piece_units; }
+struct UnitPlace {  // a unit's (batch, key / value head) and key block
+  long long bk, start;
+  int kb, units;
+  __device__ __forceinline__ UnitPlace(const WindowAttnArgs& p, const Units& u, long long s) {
+    bk = s < (1ll << 32) && p.units_per_head < (1ll << 32) ? static_cast<unsigned>(s) / static_cast<unsigned>(p.units_per_head) : s / p.units_per_head;
+    kb = u.block_of(s - bk * p.units_per_head);
+    start = bk * p.units_per_head + u.before(kb);
+    units = u.tiles(kb) * u.G;
+  }
+};
+__device__ __forceinline__ long long piece_start(const WindowAttnArgs& p, const Units& u, int w) {
+  const long long s = even_start(p, w);
+  if (w == 0 || w == p.pieces) return s;
+  const UnitPlace at(p, u, s);
+  if (!is_short(p, at.units)) return s;
+  return 2 * (s - at.start) < at.units ? at.start : at.start + at.units;
+}
 
 // A key block of the unit list and the part of it that belongs to a piece.
 struct Part {
@@ -725,14 +771,13 @@ struct Part {
 // block waits for memory.  (Starting every block by itself -- unit arithmetic with 64-bit divisions, requests, K / V, two trips to memory --
 // cost about as much as 4 of its 6 units at a window of 256.)
 template <typename TR, int D>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(WindowAttnArgs p) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 1) void window_dkdv_kernel(WindowAttnArgs p) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stages][Q | dO | lse2 | delta] | output strips
-  constexpr int S = kDkdvStages, TB = kTileBytes<D>, SB = kDkdvStageBytes<D>, NP = TileSource<D>::kPieces;
+  constexpr int S = kDkdvStages<D>, TB = kTileBytes<D>, SB = kDkdvStageBytes<D>, NP = TileSource<D>::kPieces;
   const int G = p.H / p.KV;
   const Units units(p.T, p.window, p.sinks, G);
-  const long long per_head = units.all(), total = per_head * p.KV * p.B;
   const int piece = xcd_order(blockIdx.x, p.pieces);
-  const long long u0 = piece_start(p, total, piece), u1 = piece_start(p, total, piece + 1);
+  const long long u0 = piece_start(p, units, piece), u1 = piece_start(p, units, piece + 1);
   if (u0 >= u1) return;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, li = lane & 15;
@@ -747,11 +792,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
 
   Part cp;  // the part being multiplied
   {
-    const long long bk = u0 / per_head;
-    cp.b = static_cast<int>(bk / p.KV);
-    cp.kv = static_cast<int>(bk - static_cast<long long>(cp.b) * p.KV);
-    cp.kb = units.block_of(u0 - bk * per_head);
-    cp.start = bk * per_head + units.before(cp.kb);
+    const UnitPlace at(p, units, u0);
+    cp.b = static_cast<int>(at.bk / p.KV);
+    cp.kv = static_cast<int>(at.bk - static_cast<long long>(cp.b) * p.KV);
+    cp.kb = at.kb;
+    cp.start = at.start;
     cp.open(p, units, u0, u1);
   }
   Part rp = cp;  // the part being requested, with the head of the group and the tile that come next
@@ -803,8 +848,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
       }
     }
   };
-  request();
-  request();
+  for (int i = 0; i < S - 1; ++i) request();
   load_kv(cp);
   int stage = 0;
   bool stored_whole = false;  // the last part left exactly kStores stores per wave behind its K / V loads
@@ -875,20 +919,17 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void window_dkdv_kernel(
   }
 }
 
-// Adds up the partial sums of the block that piece `blockIdx.x` + 1 begins in the middle of, if it is the first such piece.  blockIdx.y: the part of the
-// block that was wave y / 2's, dK (y even) or dV; a wave here takes a quarter of the columns.
+// Adds up the partial sums of a long block, if it was cut: blockIdx.x numbers the long blocks (the first p.cuts of every head).  blockIdx.y: the
+// part of the block that was wave y / 2's, dK (y even) or dV; a wave here takes a quarter of the columns.
 template <typename TR, int D>
 __global__ __launch_bounds__(kThreads) void window_join_kernel(WindowAttnArgs p) {
-  const int G = p.H / p.KV;
-  const Units units(p.T, p.window, p.sinks, G);
-  const long long per_head = units.all(), total = per_head * p.KV * p.B;
-  const int w = blockIdx.x + 1;
-  const long long s = piece_start(p, total, w);
-  const long long bk = s / per_head;
-  const int b = static_cast<int>(bk / p.KV), kv = static_cast<int>(bk - static_cast<long long>(b) * p.KV);
-  const int kb = units.block_of(s - bk * per_head);
-  const long long start = bk * per_head + units.before(kb), stop = start + static_cast<long long>(units.tiles(kb)) * G;
-  if (s == start || piece_start(p, total, w - 1) > start) return;
+  const Units units(p.T, p.window, p.sinks, p.H / p.KV);
+  const int bk = blockIdx.x / p.cuts, kb = blockIdx.x - bk * p.cuts, b = bk / p.KV, kv = bk - b * p.KV;
+  const long long start = bk * p.units_per_head + units.before(kb), stop = start + static_cast<long long>(units.tiles(kb)) * units.G;
+  // the first piece that begins behind the block's first unit
+  int w = static_cast<int>(start / (p.piece_units + 1));
+  while (even_start(p, w) <= start) ++w;
+  if (even_start(p, w) >= stop) return;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, g = lane >> 4, li = lane & 15;
   const int owner = blockIdx.y >> 1, is_dv = blockIdx.y & 1;
   const int len = length_of(p, b), kw = kb * kRows + owner * 32;
@@ -905,8 +946,8 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WindowAttnArgs p)
       }
   };
   add(w - 1, 1, true);
-  for (int piece = w; piece < p.pieces && piece_start(p, total, piece) < stop; ++piece)
-    if (piece_start(p, total, piece + 1) > piece_start(p, total, piece)) add(piece, 0, false);
+#pragma unroll 4
+  for (int piece = w; piece < p.pieces && even_start(p, piece) < stop; ++piece) add(piece, 0, false);
   const long long g_stride = static_cast<long long>(p.H + 2 * p.KV) * D;
   u16* out = static_cast<u16*>(p.dqkv) + static_cast<long long>(b) * p.T * g_stride + static_cast<long long>(p.H + kv + is_dv * p.KV) * D;
   const float scale = is_dv ? 1.f : p.scale;
@@ -931,9 +972,10 @@ void allow_lds(Kernel k, int bytes) {
 }
 
 template <int D>
-constexpr int kQueryLds = kStages<D> * 2 * kTileBytes<D> > 4 * kStripBytes<D> ? kStages<D> * 2 * kTileBytes<D> : 4 * kStripBytes<D>;
+constexpr int kQueryLds = 4 * kTileBytes<D>;  // [2 stages][K | V]
+static_assert(4 * kStripBytes<64> <= kQueryLds<64> && 4 * kStripBytes<128> <= kQueryLds<128>, "the output strips reuse the tiles' memory");
 template <int D>
-constexpr int kDkdvLds = kDkdvStages * kDkdvStageBytes<D> + 4 * kStripBytes<D>;
+constexpr int kDkdvLds = kDkdvStages<D> * kDkdvStageBytes<D> + 4 * kStripBytes<D>;
 
 template <typename F>
 void dispatch(int dtype, int D, F&& f) {
@@ -957,15 +999,21 @@ bool window_attention_supported(long long B, long long T, long long H, long long
   return B * H * ((T + kRows - 1) / kRows) < (1ll << 31);
 }
 
-// One piece per workgroup that the chip holds at once, and none of less than four units.
-int window_attention_pieces(const WindowAttnArgs& a) {
+// One piece per workgroup that the chip holds at once; at least a unit each, or four where blocks are long enough to be cut.
+void window_attention_plan(WindowAttnArgs& a) {
   const Units units(a.T, a.window, a.sinks, a.H / a.KV);
-  const long long total = units.all() * a.KV * a.B;
-  long long n = a.compute_units * (a.D == 64 ? 2 : 1);
-  if (n > (total + 3) / 4) n = (total + 3) / 4;
-  return static_cast<int>(n < 1 ? 1 : n);
+  a.units_per_head = units.all();
+  const long long total = a.units_per_head * a.KV * a.B;
+  long long n = a.compute_units * (a.D == 64 ? 3 : 1);
+  const long long most = units.tiles(0) * units.G <= kShort ? total : total / 4;  // (no block is longer than the first)
+  if (n > most) n = most;
+  a.pieces = static_cast<int>(n < 1 ? 1 : n);
+  a.piece_units = total / a.pieces;
+  a.piece_rest = static_cast<int>(total % a.pieces);
+  a.cuts = 0;  // blocks get no longer from first to last
+  while (a.pieces > 1 && a.cuts < units.n_blocks && !is_short(a, static_cast<long long>(units.tiles(a.cuts)) * units.G)) ++a.cuts;
 }
-long long window_attention_partial_floats(const WindowAttnArgs& a) { return a.pieces > 1 ? 2LL * a.pieces * 2 * kRows * a.D : 0; }
+long long window_attention_partial_floats(const WindowAttnArgs& a) { return a.cuts ? 2LL * a.pieces * 2 * kRows * a.D : 0; }
 
 void launch_window_attention_fwd(const WindowAttnArgs& args, int dtype, hipStream_t stream) {
   WindowAttnArgs a = args;
@@ -995,7 +1043,7 @@ void launch_window_attention_bwd(const WindowAttnArgs& args, int dtype, hipStrea
     allow_lds(dkdv, kDkdvLds<D>);
     hipLaunchKernelGGL(dq, grid, dim3(kThreads), kQueryLds<D>, stream, a);
     hipLaunchKernelGGL(dkdv, dim3(static_cast<unsigned>(a.pieces)), dim3(kThreads), kDkdvLds<D>, stream, a);
-    if (a.pieces > 1) hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(a.pieces - 1), 8), dim3(kThreads), 0, stream, a);
+    if (a.cuts) hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(a.B) * a.KV * a.cuts, 8), dim3(kThreads), 0, stream, a);
   });
 }
 

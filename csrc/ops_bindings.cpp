@@ -1259,7 +1259,7 @@ Tensor window_attention_backward(Tensor d_o, Tensor qkv, Tensor o, Tensor lse2, 
   a.lse2 = lse2.data_ptr<float>();
   a.delta = delta.data_ptr<float>();
   a.compute_units = compute_units_of(qkv);
-  a.pieces = kernels::window_attention_pieces(a);
+  if (a.B > 0 && a.T > 0) kernels::window_attention_plan(a);
   Tensor partial;
   if (const long long n = kernels::window_attention_partial_floats(a)) {
     partial = at::empty({n}, lse2.options());
