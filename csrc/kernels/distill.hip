@@ -32,6 +32,7 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kNone = 0x7fffffff;
+constexpr long long kRowsPerLaunch = 1 << 21;  // a launch counts its threads (1024 a row at most) in 32 bits
 enum Mode : int { kForward = 0, kBackward = 1, kFused = 2 };
 
 // Sum / maximum over the threads of a workgroup, in a fixed order.
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
   int* const s_head = s_next + entries;
   unsigned* const s_bits = reinterpret_cast<unsigned*>(s_head + a.hash);
 
-  const long long r = blockIdx.x;
+  const long long r = a.row0 + blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int C = static_cast<int>(a.C), ld = static_cast<int>(a.ld);
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
@@ -419,7 +420,7 @@ __global__ __launch_bounds__(256) void distill_apply_upstream_kernel(typename TR
 }  // namespace
 
 bool distill_supported(long long C, long long ld, long long K) {
-  return C >= 1 && C <= ld && ld < (1ll << 28) && K >= 1 && K <= kDistillMaxEntries;
+  return C >= 1 && C <= ld && ld <= kDistillMaxWidth && K >= 1 && K <= kDistillMaxEntries;
 }
 
 void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t stream) {
@@ -436,15 +437,17 @@ void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t st
     const long long nvec = (a.ld + 2 * V - 2) / V;  // worst alignment
     a.words = static_cast<int>((nvec + 63) / 64);
     const size_t lds = (static_cast<size_t>(4) * (a.K + 1) + a.hash + 2 * static_cast<size_t>(a.words)) * 4;
-    const dim3 grid(static_cast<unsigned>(a.N));
     auto go = [&](auto threads_c, auto keep_c, auto mode_c, auto waves_c) {
       constexpr int THREADS = decltype(threads_c)::value, KEEP = decltype(keep_c)::value, MODE = decltype(mode_c)::value;
       constexpr int WAVES = decltype(waves_c)::value;
+      const dim3 grid(static_cast<unsigned>(args.N - a.row0 < kRowsPerLaunch ? args.N - a.row0 : kRowsPerLaunch));
       if (!dual) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 0, WAVES>), grid, dim3(THREADS), lds, stream, a);
       else if (a.tau == 2.f) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 2, WAVES>), grid, dim3(THREADS), lds, stream, a);
       else if (a.tau == 4.f) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 4, WAVES>), grid, dim3(THREADS), lds, stream, a);
       else hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 1, WAVES>), grid, dim3(THREADS), lds, stream, a);
     };
+    static_assert(((4 * (kDistillMaxEntries + 1) + 2 * kDistillMaxEntries + 2 * ((kDistillMaxWidth / 4 + 64) / 64)) * 4) <= 60 * 1024,
+                  "a workgroup's tables fit the 64 KiB that a launch may have without asking");
     using std::integral_constant;
     auto by_size = [&](auto mode_c) {
       constexpr int MODE = decltype(mode_c)::value;
@@ -467,9 +470,11 @@ void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t st
         else go(t1024, none, m, w8);
       }
     };
-    if (mode == kForward) by_size(integral_constant<int, kForward>{});
-    else if (mode == kBackward) by_size(integral_constant<int, kBackward>{});
-    else by_size(integral_constant<int, kFused>{});
+    for (a.row0 = 0; a.row0 < args.N; a.row0 += kRowsPerLaunch) {
+      if (mode == kForward) by_size(integral_constant<int, kForward>{});
+      else if (mode == kBackward) by_size(integral_constant<int, kBackward>{});
+      else by_size(integral_constant<int, kFused>{});
+    }
   });
 }
 

@@ -102,6 +102,7 @@ void launch_xent_fused(void* logits, int dtype, const long long* targets, long l
 // mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits
 // dlogits [N, ld]: columns [C, ld) are written as zero; its address must equal that of logits modulo 16.
 constexpr int kDistillMaxEntries = 1024;
+constexpr long long kDistillMaxWidth = 1 << 20;  // of ld: one bit per 16 bytes of a row is kept in LDS
 struct DistillArgs {
   const void* logits;
   void* dlogits;
@@ -120,6 +121,7 @@ struct DistillArgs {
   // set by the launcher
   float exp_scale;
   int hash, words;
+  long long row0;
 };
 bool distill_supported(long long C, long long ld, long long K);
 void launch_distill(const DistillArgs& a, int dtype, int mode, hipStream_t stream);

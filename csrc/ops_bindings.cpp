@@ -306,8 +306,8 @@ kernels::DistillArgs distill_args(const Tensor& logits, const Tensor& ids, const
   TORCH_CHECK(ids.dim() == 2 && ids.size(0) == N && ids.sizes() == teacher.sizes(), who, ": teacher_ids and teacher_logits must both be [N, K]");
   TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, who, ": teacher_ids must be int64 or int32");
   TORCH_CHECK(ids.get_device() == logits.get_device() && teacher.get_device() == logits.get_device(), who, ": tensors on different devices");
-  TORCH_CHECK(kernels::distill_supported(C, ld, ids.size(1)), who, ": needs 1 <= n_classes <= width and 1 .. ", kernels::kDistillMaxEntries,
-              " teacher entries (got ", C, ", ", ld, ", ", ids.size(1), ")");
+  TORCH_CHECK(kernels::distill_supported(C, ld, ids.size(1)), who, ": needs 1 <= n_classes <= width <= ", kernels::kDistillMaxWidth, " and 1 .. ",
+              kernels::kDistillMaxEntries, " teacher entries (got ", C, ", ", ld, ", ", ids.size(1), ")");
   TORCH_CHECK(N < (1ll << 31), who, ": too many rows");
   TORCH_CHECK(temperature > 0.0 && hard_weight >= 0.0 && hard_weight <= 1.0, who, ": needs temperature > 0 and 0 <= hard_weight <= 1");
   kernels::DistillArgs a{};
@@ -378,7 +378,7 @@ Tensor distill_backward(Tensor logits, Tensor ids, Tensor teacher, c10::optional
   a.row_stats = row_stats.data_ptr<float>();
   a.scale = scale.data_ptr<float>();
   a.grad_out = grad_out.data_ptr<float>();
-  a.grad_out_rows = grad_out.dim() == 1 ? 1 : 0;
+  a.grad_out_rows = grad_out.dim() == 1 && grad_out.numel() == a.N ? 1 : 0;
   kernels::launch_distill(a, kdtype(logits), 1, stream_of(logits));
   return dlogits;
 }

@@ -35,7 +35,10 @@ class DistillResult(NamedTuple):
 class _TopKDistillation(torch.autograd.Function):
     """Mean and sum: the forward also writes the gradient for a unit upstream gradient, so that the logits are read once
     for both; the backward scales it where the upstream gradient is another one (told apart on the device).  That
-    gradient is handed over by the first backward; a second one through a retained graph computes it again."""
+    gradient is handed over by the first backward; a second one through a retained graph computes it again.
+
+    Not so in fp16: divided by the number of rows, most of that gradient is below the type's smallest value, and the upstream gradient -- a loss
+    scale -- would come too late.  The backward then computes it from the logits with the upstream gradient as a factor ahead of the rounding."""
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, targets, cfg):
@@ -44,7 +47,7 @@ class _TopKDistillation(torch.autograd.Function):
         mean = reduction == "mean"
         ctx.cfg = cfg
         ctx.needs = ctx.needs_input_grad[0]
-        fused = ctx.needs and reduction != "none"
+        fused = ctx.needs and reduction != "none" and logits.dtype != torch.float16
         loss, row_loss, correct, metrics, scale, stats, dlogits = C.distill_forward(
             logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, mean, "new" if fused else "none")
         ctx.dlogits, ctx.scale = dlogits, scale
@@ -70,33 +73,44 @@ class _TopKDistillation(torch.autograd.Function):
 
 class _ProjectionTopKDistillation(torch.autograd.Function):
     """Vocabulary projection and loss as one node: the logits are overwritten with their gradient by the kernel that
-    computes the loss, and the backward is two matrix products (see ``cross_entropy._ProjectionXent``)."""
+    computes the loss, and the backward is two matrix products (see ``cross_entropy._ProjectionXent``).  In fp16 the logits stay and the
+    backward computes their gradient, for the reason given above."""
 
     @staticmethod
     def forward(ctx, x2, weight, ids, teacher, targets, cfg, impl):
         reduction, ignore_index, n_classes, temperature, hard_weight = cfg
         logits = gemm.nt(x2, weight, None, impl)
         grad = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        loss, _, correct, metrics, _, _, _ = _ext.C().distill_forward(
-            logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, reduction == "mean", "inplace" if grad else "none")
-        if grad:
+        inplace = grad and logits.dtype != torch.float16
+        loss, _, correct, metrics, scale, stats, _ = _ext.C().distill_forward(
+            logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, reduction == "mean", "inplace" if inplace else "none")
+        if inplace:
             ctx.save_for_backward(x2, weight, logits)  # `logits` now holds d loss / d logits for a unit upstream gradient
-        ctx.impl = impl
+        elif grad:
+            ctx.save_for_backward(x2, weight, logits, ids, teacher, targets, scale, stats)
+        ctx.impl, ctx.inplace, ctx.cfg = impl, inplace, cfg
         ctx.mark_non_differentiable(correct, metrics)
         return loss, correct, metrics
 
     @staticmethod
     def backward(ctx, dloss, _dcorrect, _dmetrics):
-        x2, weight, dlogits = ctx.saved_tensors
-        g = dloss.detach().to(torch.float32).reshape(1)
+        g = dloss.detach().to(torch.float32).reshape(())
         C = _ext.C()
+        if ctx.inplace:
+            x2, weight, dlogits = ctx.saved_tensors
+        else:
+            x2, weight, logits, ids, teacher, targets, scale, stats = ctx.saved_tensors
+            _, ignore_index, n_classes, temperature, hard_weight = ctx.cfg
+            dlogits = C.distill_backward(logits, ids, teacher, targets, stats, scale, g, n_classes, ignore_index, temperature, hard_weight)
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = gemm.nn(dlogits, weight, ctx.impl)
-            C.distill_apply_upstream(dx, g)
+            if ctx.inplace:
+                C.distill_apply_upstream(dx, g)
         if ctx.needs_input_grad[1]:
             dw = gemm.weight_grad(dlogits, x2, weight, ctx.impl)
-            C.distill_apply_upstream(dw, g)
+            if ctx.inplace:
+                C.distill_apply_upstream(dw, g)
         return dx, dw, None, None, None, None, None
 
 
@@ -164,7 +178,7 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
                       temperature: float = 1.0, hard_weight: float = 0.0, reduction: str = "mean", ignore_index: int = -100,
                       n_classes: Optional[int] = None, check_targets: Optional[bool] = None) -> DistillResult:
     """Distillation loss of ``logits[N, C]`` against a teacher's entries ``teacher_ids[N, K]`` / ``teacher_logits[N, K]``
-    (K <= 1024 on the GPU), see the module's description.
+    (on the GPU K <= 1024 and C <= 2 ** 20), see the module's description.
 
     ``targets[N]`` give the hard term (weight ``hard_weight``) and mark ignored rows; the mean is taken over rows whose
     target is not ``ignore_index`` (over all rows without targets).  ``n_classes`` < C marks trailing columns as padding:

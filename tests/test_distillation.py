@@ -396,3 +396,91 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         want_loss, want_g = step()
         assert torch.equal(loss, want_loss) and torch.equal(g, want_g)
+
+
+@gpu
+def test_widest_rows_and_wider_ones():
+    C = 1 << 20
+    logits, ids, teacher, targets = make(2, C, 5, torch.float32, DEV)
+    check(logits, ids, teacher, targets, 2.0, 0.5)
+    with pytest.raises(RuntimeError, match="width"):
+        topk_distillation(torch.zeros(1, C + 8, device=DEV), ids[:1], teacher[:1])
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_more_rows_than_one_launch_takes(reduction):
+    N, C, K = (1 << 21) + 5, 8, 2
+    g = torch.Generator(device=DEV).manual_seed(3)
+    logits = torch.randn(N, C, generator=g, device=DEV) * 3
+    ids = torch.randint(0, C, (N, K), generator=g, device=DEV)
+    teacher = torch.randn(N, K, generator=g, device=DEV)
+    targets = torch.randint(0, C, (N,), generator=g, device=DEV)
+    x, z = logits.clone().requires_grad_(), logits.double().requires_grad_()
+    got = topk_distillation(x, ids, teacher, targets, 2.0, 0.5, reduction=reduction)
+    want = topk_distillation(z.cpu(), ids.cpu(), teacher.double().cpu(), targets.cpu(), 2.0, 0.5, reduction=reduction)
+    got.loss.sum().backward()
+    want.loss.sum().backward()
+    # exponents below 64 in float32, a few roundings; a sum of N positive rows in blocks: below 2^12 roundings on the way
+    near = 64 * 2.0 ** -23 * 4
+    torch.testing.assert_close(got.loss.detach().double().cpu(), want.loss.detach(), rtol=2.0 ** -12 if reduction == "sum" else 2.0 ** -20, atol=near)
+    torch.testing.assert_close(x.grad.double(), z.grad, rtol=2.0 ** -22, atol=near)
+    assert torch.equal(got.correct.cpu(), want.correct)
+
+
+@gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_half_precision_gradients_survive_the_division_by_the_rows(reduction):
+    # a loss scale has to come in ahead of the rounding: 1 / (1500 * 600) is about the smallest fp16 step
+    N, C, up = 1500, 600, 2.0 ** (16 if reduction == "mean" else 4)
+    logits, ids, teacher, targets = make(N, C, 9, torch.float16, DEV)
+    x = (logits + 20).requires_grad_()
+    rows, grad, n = reference(x, ids, teacher, targets, 2.0, 0.5)
+    grad = grad * up / (n if reduction == "mean" else 1)
+    r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5, reduction=reduction)
+    (r.loss * up).backward()
+    half = 2.0 ** -11
+    # one rounding; a subnormal's is half of 2^-24; float32 arithmetic as in check()
+    near = 64 * 2.0 ** -23 * 2 * up / (n if reduction == "mean" else 1)
+    torch.testing.assert_close(x.grad.double().cpu(), grad, rtol=half * 1.01, atol=near + 2.0 ** -25)
+
+
+@gpu
+def test_half_precision_projection_under_a_loss_scale():
+    N, C, width, K_in, up = 1500, 600, 608, 64, 2.0 ** 16
+    _, ids, teacher, targets = make(N, C, 9, torch.float16, DEV)
+    x = torch.randn(N, K_in, device=DEV).half()
+    w = (torch.randn(width, K_in, device=DEV) / math.sqrt(K_in)).half()
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    r = projection_topk_distillation(xs, ws, ids, teacher, targets, 2.0, 0.5, n_classes=C)
+    first = torch.autograd.grad(r.loss * up, (xs, ws), retain_graph=True)
+    (r.loss * up).backward()
+    assert torch.equal(first[0], xs.grad) and torch.equal(first[1], ws.grad)
+    half, tiny = 2.0 ** -11, 2.0 ** -25
+    logits = x.double() @ w.double().t()
+    _, grad, n = reference(logits, ids, teacher, targets, 2.0, 0.5, C)
+    grad = grad.to(DEV) * up / n
+    zmax = float(logits.abs().max())
+    # as test_projection_against_float64, and every element of dlogits off by half of the smallest step besides
+    factor = math.expm1(2 * half * zmax) + 3 * half + 2e-5
+    z = logits[:, :C]
+    q = grad.abs() + up / n * F.pad(torch.softmax(z / 2, 1) + 0.5 * torch.softmax(z, 1), (0, width - C))
+    on = torch.ones_like(grad)
+    for got, want, bound, steps in ((xs.grad, grad @ w.double(), q @ w.double().abs(), on @ w.double().abs()),
+                                    (ws.grad, grad.t() @ x.double(), q.t() @ x.double().abs(), on.t() @ x.double().abs())):
+        err = (got.double() - want).abs()
+        assert bool((err <= factor * bound + half * want.abs() + tiny * (steps + 1)).all())
+        assert float(err.norm() / want.norm()) < 0.01
+
+
+@gpu
+def test_one_upstream_value_for_many_rows():
+    from distributed_pytorch_amd import _ext
+
+    logits, ids, teacher, targets = make(7, 100, 5, torch.float32, DEV)
+    cfg = (100, -100, 2.0, 0.5)
+    out = _ext.C().distill_forward(logits, ids, teacher, targets, *cfg, True, "none")
+    args = (logits, ids, teacher, targets, out[5], out[4])
+    one = _ext.C().distill_backward(*args, torch.full((), 3.0, device=DEV), *cfg)
+    assert torch.equal(one, _ext.C().distill_backward(*args, torch.full((1,), 3.0, device=DEV), *cfg))
+    assert torch.equal(one, _ext.C().distill_backward(*args, torch.full((7,), 3.0, device=DEV), *cfg))
