@@ -111,7 +111,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_rows_kernel(GemmArgs p) {
 
 bool few_rows_supported(const GemmArgs& a, int dtype) {
   return (dtype == kBF16 || dtype == kF16) && a.a_kmajor && a.b_kmajor && a.M >= 1 && a.M <= kFewRows && a.N >= 1 && a.K >= 1 &&
-         a.N < (1ll << 31) && a.beta == 0.f && a.alpha == 1.f && (a.gate == 1 || (a.gate == 0 && a.act == kActNone && a.pre_act == nullptr));
+         a.N < (1ll << 27) /* a launch counts its threads in 32 bits */ && a.beta == 0.f && a.alpha == 1.f && (a.gate == 1 || (a.gate == 0 && a.act == kActNone && a.pre_act == nullptr));
 }
 
 void launch_few_rows(const GemmArgs& a, int dtype, hipStream_t stream) {

@@ -996,7 +996,7 @@ bool window_attention_supported(long long B, long long T, long long H, long long
   if (!(dtype == kBF16 || dtype == kF16) || !(D == 64 || D == 128)) return false;
   if (B < 0 || T < 0 || H < 1 || KV < 1 || H % KV != 0) return false;
   if (T > (1ll << 30) || row_stride % 8 != 0 || row_stride >= (1ll << 24) || (H + 2 * KV) * D >= (1ll << 24)) return false;  // a tile's byte offsets are 32-bit
-  return B * H * ((T + kRows - 1) / kRows) < (1ll << 31);
+  return B * H * ((T + kRows - 1) / kRows) < (1ll << 24);  // a launch counts its threads in 32 bits
 }
 
 // One piece per workgroup that the chip holds at once; at least a unit each, or four where blocks are long enough to be cut.

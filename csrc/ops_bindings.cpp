@@ -1203,7 +1203,7 @@ kernels::WindowAttnArgs window_args(const Tensor& qkv, int64_t n_head, int64_t n
               ": qkv needs contiguous rows on 16-byte boundaries");
   TORCH_CHECK(kernels::window_attention_supported(B, T, n_head, n_kv_head, D, rs, kdtype(qkv)), who, ": needs bf16 / fp16 and head size 64 or 128 (got ",
               qkv.scalar_type(), ", ", D, ")");
-  TORCH_CHECK(window >= 1 && sinks >= 0 && scale > 0.0, who, ": needs window >= 1, sinks >= 0 and a positive scale");
+  TORCH_CHECK(window >= 1 && sinks >= 0 && scale >= 1e-30 && scale <= 1e30, who, ": needs window >= 1, sinks >= 0 and a scale in 1e-30 .. 1e30");
   kernels::WindowAttnArgs a{};
   if (lens.has_value() && lens->defined()) {
     check_gpu(*lens, "seq_lens");

@@ -20,6 +20,7 @@ from typing import NamedTuple, Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import _ext
 from . import gemm
@@ -56,6 +57,7 @@ class _TopKDistillation(torch.autograd.Function):
         return (row_loss if reduction == "none" else loss), correct, metrics
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, _dcorrect, _dmetrics):
         C = _ext.C()
         g = dloss.detach().to(torch.float32).contiguous()
@@ -93,6 +95,7 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
         return loss, correct, metrics
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss, _dcorrect, _dmetrics):
         g = dloss.detach().to(torch.float32).reshape(())
         C = _ext.C()

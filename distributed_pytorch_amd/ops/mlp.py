@@ -31,6 +31,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import _ext
 from . import gemm
@@ -115,6 +116,7 @@ class _GatedMLP(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         C = _ext.C()
         x2, w_fc, w_proj, gu, h = ctx.saved_tensors

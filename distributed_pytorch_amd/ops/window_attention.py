@@ -17,6 +17,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _ext
 
@@ -32,6 +33,7 @@ class _WindowAttention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o):
         qkv, o, lse2, lens = ctx.saved_tensors
         if not (d_o.is_contiguous() and d_o.data_ptr() % 16 == 0):
@@ -82,9 +84,9 @@ def window_attention_qkvpacked(qkv: torch.Tensor, n_head: int, window: int, sink
 
     ``n_kv_head`` defaults to ``n_head``.  ``seq_lens`` ([B], int32 or int64, on the device of ``qkv``) gives the lengths of a
     padded batch, taken into 0 .. T: positions behind a sequence are never looked at, their outputs and gradients are zero.
-    ``softmax_scale`` (> 0) defaults to D ** -0.5.  impl: "auto", "native" (raise where the kernels do not apply), "composed".
+    ``softmax_scale`` (1e-30 .. 1e30) defaults to D ** -0.5.  impl: "auto", "native" (raise where the kernels do not apply), "composed".
     A NaN or infinity at a position of a sequence reaches the queries that see it, and may reach others within 128 positions
-    of those.
+    of those.  Scaled scores are taken to stay below 2 ** 24 in size, beyond which float32 tells no neighbouring ones apart.
     """
     if impl not in ("auto", "native", "composed"):
         raise ValueError(f"impl must be auto | native | composed, got {impl}")
@@ -99,8 +101,8 @@ def window_attention_qkvpacked(qkv: torch.Tensor, n_head: int, window: int, sink
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(W // heads)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:  # (in float32 neither zero nor infinite, times log2(e) either)
+        raise ValueError(f"softmax_scale must lie in 1e-30 .. 1e30, got {scale}")
     lens = seq_lens
     if lens is not None:
         if lens.shape != (qkv.shape[0],) or lens.dtype not in (torch.int32, torch.int64) or lens.device != qkv.device:

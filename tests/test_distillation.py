@@ -484,3 +484,14 @@ def test_one_upstream_value_for_many_rows():
     one = _ext.C().distill_backward(*args, torch.full((), 3.0, device=DEV), *cfg)
     assert torch.equal(one, _ext.C().distill_backward(*args, torch.full((1,), 3.0, device=DEV), *cfg))
     assert torch.equal(one, _ext.C().distill_backward(*args, torch.full((7,), 3.0, device=DEV), *cfg))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_a_second_derivative_is_refused(dtype):
+    logits, ids, teacher, targets = make(4, 11, 3, dtype, DEV)
+    x, w = logits.requires_grad_(), torch.randn(16, 11, device=DEV).to(dtype)
+    for r in (topk_distillation(x, ids, teacher, targets, 2.0, 0.5), projection_topk_distillation(x, w, ids, teacher, targets, 2.0, 0.5)):
+        (g,) = torch.autograd.grad(r.loss, x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.float().square().sum().backward()

@@ -285,3 +285,13 @@ def test_gradient_against_differences():
         diff = (at[0] - at[1]) / (2 * h)
         # the differences carry 1e-16 of a sum of a few thousand over 1e-6
         assert abs(diff - float((got["d" + k].double() * way).sum())) <= float((want["d" + k][1] * way.abs()).sum()) + 1e-4
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_second_derivative_is_refused(dtype):
+    x = torch.randn(5, 16, device=DEV, dtype=dtype, requires_grad=True)
+    y = gated_mlp(x, torch.randn(24, 16, device=DEV, dtype=dtype), None, torch.randn(8, 12, device=DEV, dtype=dtype), None)
+    (g,) = torch.autograd.grad(y.float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().square().sum().backward()

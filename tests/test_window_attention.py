@@ -317,3 +317,31 @@ def test_gradient_against_differences():
     diff = (at[0] - at[1]) / (2 * h)
     # central differences are exact to h^2 times a third derivative of the order of the values (1e-4 here)
     assert abs(diff - float((g.double() * way).sum())) <= float((eg * way.abs()).sum()) + 1e-3
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_scales_beyond_float32_are_refused(device):
+    qkv = torch.randn(1, 5, 3 * 64, device=device).bfloat16()
+    for scale in (1e-50, 1e-31, 1e31, float("inf")):
+        with pytest.raises(ValueError):
+            window_attention_qkvpacked(qkv, 1, 3, softmax_scale=scale)
+
+
+@gpu
+def test_a_second_derivative_is_refused():
+    qkv = torch.randn(1, 5, 3 * 64, device=DEV).bfloat16().requires_grad_()
+    (g,) = torch.autograd.grad(window_attention_qkvpacked(qkv, 1, 3).float().sum(), qkv, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().square().sum().backward()
+
+
+@gpu
+def test_many_short_sequences():
+    # one position attends to itself alone; a launch counts its threads in 32 bits, so 2^24 blocks of queries are not the kernels' any more
+    qkv = torch.randn(1 << 21, 1, 9 * 64, device=DEV, dtype=torch.bfloat16)[:, :, : 3 * 64]
+    o = window_attention_qkvpacked(qkv, 1, 1)
+    assert torch.equal(o, qkv[..., 128:])
+    from distributed_pytorch_amd import _ext
+
+    assert not _ext.C().window_attention_supported(1 << 24, 1, 1, 1, 64, 192, "bfloat16")
+    assert _ext.C().window_attention_supported((1 << 24) - 1, 1, 1, 1, 64, 192, "bfloat16")
