@@ -190,11 +190,34 @@ __device__ __forceinline__ u32x4 load_piece(const u16* src, long long n) {
   return __builtin_bit_cast(u32x4, e);
 }
 
-// ALIGNED: every 8-element piece is either wholly inside the matrix and 16-byte aligned or wholly outside (base
+// A tile that ends ahead of the contraction's last index (k0 + BK < K; ld >= 8), loaded without branches: rows beyond the matrix repeat its last
+// ones, a piece across the end of a row runs on into the next row, and both end up in outputs that are not stored.
+template <bool KMAJOR, bool ALIGNED, bool PAIRED = false>
+__device__ __forceinline__ void load_inner_tile(const u16* __restrict__ base, long long ld, long long r0, long long R, long long k0, u32x4 (&regs)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    const u16* src;
+    if (PAIRED) {
+      const long long vr = r0 + (id >> 3), h = gate_row(vr);
+      src = base + ((h < R ? h : R - 1) + (vr & 16 ? R : 0)) * ld + k0 + ((id & 7) << 3);
+    } else if (KMAJOR) {
+      const long long row = r0 + (id >> 3);
+      src = base + (row < R ? row : R - 1) * ld + k0 + ((id & 7) << 3);
+    } else {
+      const long long row = r0 + ((id & 15) << 3);
+      src = base + (k0 + (id >> 4)) * ld + (row < R ? row : R - (ALIGNED ? 8 : 1));
+    }
+    if (ALIGNED) regs[i] = *reinterpret_cast<const u32x4*>(src);
+    else regs[i] = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_any*>(src));
+  }
+}
+
+// Any tile.  ALIGNED: every 8-element piece is either wholly inside the matrix and 16-byte aligned or wholly outside (base
 // address, leading dimension and contiguous extent are multiples of 8 elements): one 16-byte load per piece.
 // Otherwise (odd extents, leading dimensions or base addresses) a piece inside the matrix is one 16-byte load from wherever it starts,
-// and only the pieces across the edge of a row are gathered element by element -- the tail path that lets every shape run here.  (Gathering
-// every piece, the fp16 product 1003 x 520 x 1386 took 166 us; with whole loads and its contraction spread over the chip it takes 20.)
+// and only the pieces across the edge of a row are gathered element by element -- the tail path that lets every shape run here.
+// (Gathering every piece, the fp16 product 1003 x 520 x 1386 took 166 us; with whole loads and its contraction spread over the chip it takes 17.)
 // PAIRED: the rows are the interleaved ones of a gated pair of R rows each (see gate_row).
 template <bool KMAJOR, bool ALIGNED, bool PAIRED = false>
 __device__ __forceinline__ void load_tile(const u16* __restrict__ base, long long ld, long long r0, long long R, long long k0,
@@ -286,23 +309,23 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  u32x4 ra[4], rb[4];
+  // Global loads run two k-steps ahead of the products, in two sets of registers: with few workgroups on a compute unit one step (0.4 us of matrix
+  // work) does not cover a trip to memory.  The inner loop loads without branches, so that its waits count loads.  (One step ahead, with a branch per
+  // piece: fp16 4096^3 217 -> 197 us, 1024^3 20 -> 17 us, gated pair 1003 x 520 x 1386 14.0 -> 12.8 us forward, 17.9 -> 16.4 us backward.)
+  u32x4 ra0[4], rb0[4], ra1[4], rb1[4];
   const long long nk_all = (p.K + BK - 1) / BK;
   const long long kt0 = SPREAD ? nk_all * blockIdx.y / p.split_k : 0, nk = SPREAD ? nk_all * (blockIdx.y + 1) / p.split_k : nk_all;
-  load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, kt0 * BK, p.K, ra);
   const long long b_rows = GATE == 1 ? p.gate_H : p.N;
-  load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, kt0 * BK, p.K, rb);
-  store_tile<A_KMAJOR>(smem_bf16, ra);
-  store_tile<B_KMAJOR>(smem_bf16 + kTileBytes, rb);
-  __syncthreads();
-
-  int cur = 0;
-  for (long long kt = kt0; kt < nk; ++kt) {
-    const bool more = kt + 1 < nk;
-    if (more) {
-      load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, (kt + 1) * BK, p.K, ra);
-      load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, (kt + 1) * BK, p.K, rb);
-    }
+  const long long inner = p.lda >= 8 && p.ldb >= 8 ? (p.K - 1) / BK : 0;  // k-steps that load_inner_tile may load
+  auto load_any = [&](long long kt, u32x4 (&ra)[4], u32x4 (&rb)[4]) __attribute__((always_inline)) {
+    load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, kt * BK, p.K, ra);
+    load_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, kt * BK, p.K, rb);
+  };
+  auto load_inner = [&](long long kt, u32x4 (&ra)[4], u32x4 (&rb)[4]) __attribute__((always_inline)) {
+    load_inner_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, kt * BK, ra);
+    load_inner_tile<B_KMAJOR, ALIGNED, GATE == 1>(B, p.ldb, n0, b_rows, kt * BK, rb);
+  };
+  auto multiply = [&](int cur) __attribute__((always_inline)) {
     const char* as = smem_bf16 + cur * 2 * kTileBytes;
     const char* bs = as + kTileBytes;
 #pragma unroll
@@ -324,13 +347,45 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int 
           }
         }
     }
-    if (more) {
-      char* an = smem_bf16 + (cur ^ 1) * 2 * kTileBytes;
-      store_tile<A_KMAJOR>(an, ra);
-      store_tile<B_KMAJOR>(an + kTileBytes, rb);
-    }
+  };
+  auto put = [&](int to, u32x4 (&ra)[4], u32x4 (&rb)[4]) __attribute__((always_inline)) {
+    char* an = smem_bf16 + to * 2 * kTileBytes;
+    store_tile<A_KMAJOR>(an, ra);
+    store_tile<B_KMAJOR>(an + kTileBytes, rb);
+  };
+  const long long stop = nk < inner ? nk : inner;
+  if (kt0 + 1 < stop) {
+    load_inner(kt0, ra0, rb0);
+    load_inner(kt0 + 1, ra1, rb1);
+    put(0, ra0, rb0);
+  } else {
+    load_any(kt0, ra0, rb0);
+    if (kt0 + 1 < nk) load_any(kt0 + 1, ra1, rb1);
+    put(0, ra0, rb0);
+  }
+  __syncthreads();
+  long long kt = kt0;
+  for (; kt + 3 < stop; kt += 2) {
+    load_inner(kt + 2, ra0, rb0);
+    multiply(0);
+    put(1, ra1, rb1);
     __syncthreads();
-    cur ^= 1;
+    load_inner(kt + 3, ra1, rb1);
+    multiply(1);
+    put(0, ra0, rb0);
+    __syncthreads();
+  }
+  while (true) {
+    if (kt + 2 < nk) load_any(kt + 2, ra0, rb0);
+    multiply(0);
+    if (++kt >= nk) break;
+    put(1, ra1, rb1);
+    __syncthreads();
+    if (kt + 2 < nk) load_any(kt + 2, ra1, rb1);
+    multiply(1);
+    if (++kt >= nk) break;
+    put(0, ra0, rb0);
+    __syncthreads();
   }
 
   // Epilogue (operands were swapped in the MFMA: see store_tile_bf16).
@@ -1877,17 +1932,18 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream) {
   else go(std::false_type{}, std::false_type{});
 }
 
-// Shares of the contraction that let a product with few 128x128 tiles fill the chip: two workgroups per compute unit, at least three k-steps a
-// share (its start and the fp32 sums then stay small beside it), 64 MiB of sums at most.  1: not worth it.
+// Shares of the contraction that let a product with few 128x128 tiles fill the chip: two workgroups per compute unit, at least four k-steps a
+// share, 64 MiB of sums at most.  1: not worth it -- writing, reading and adding the sums costs about as much as 10 k-steps, so at least 12 have to
+// be saved (fp16 1003 x 520 x 1386, 18 saved: 21 -> 17 us; bf16 2048 x 1024 x 768, 9 saved: 15 -> 25 us).
 int gemm_spread(const GemmArgs& a) {
   const long long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN), nk = (a.K + BK - 1) / BK;
   const int cus = compute_units();
   if (tiles >= cus || nk < 6) return 1;
   long long s = 2ll * cus / tiles;
-  if (s > nk / 3) s = nk / 3;
+  if (s > nk / 4) s = nk / 4;
   const long long plane = a.M * ((a.N + 3) & ~3ll) * 4;
   if (s > (64ll << 20) / plane) s = (64ll << 20) / plane;
-  return s < 2 ? 1 : static_cast<int>(s);
+  return s < 2 || nk - nk / s < 12 ? 1 : static_cast<int>(s);
 }
 
 void launch_gemm_spread(const GemmArgs& a, int dtype, hipStream_t stream) {
