@@ -248,6 +248,9 @@ void launch_outer_wgrad(const void* dy, const void* x, void* dw, void* db, float
 //   db[N] = colsum(dy[M,N])  (also used by the large-GEMM path)
 void launch_colsum(const void* dy, void* db, float* workspace, long long M, long long N, int dtype,
                    hipStream_t stream);
+//   the same for few rows, in one launch (another order of summation)
+inline bool colsum_few_rows_supported(long long M, long long N) { return M >= 1 && M <= 2048 && N >= 8; }
+void launch_colsum_few_rows(const void* dy, void* db, long long M, long long N, int dtype, hipStream_t stream);
 // Linear(1, H) -> act -> Linear(H, N <= 16) without materialising the hidden layer (rank1_mlp.hip).
 //   forward : y[M,N] = b2 + act(x w1^T + b1) W2^T        x: [M] scalars, w1/b1: [H], W2: [N,H]
 //   backward: grads (length rank1_mlp_bwd_len(H,N), NT = 4 | 8 | 16 >= N) holds

@@ -542,9 +542,12 @@ void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& l
     kernels::launch_few_rows(a, dt, s);
     return;
   }
-  if (spread && dt != kernels::kF32 && (dt == kernels::kF16 || kernels::gemm_bf16_split_k(a) == 1)) {
+  if (spread && dt != kernels::kF32) {
     const int shares = kernels::gemm_spread(a);
-    if (shares > 1) {
+    // The bf16 kernel of larger tiles can split its contraction too, but takes 30 us to get going: up to 16 k-steps a share the smaller tiles are
+    // ahead (weight gradients [768, 768] of 2048 / 8192 / 16384 tokens: 4, 9, 18 steps, 20 / 31 / 45 us against 33 / 37 / 40), and up to 64 shares
+    // ([256, 256] of 8192 / 65536 tokens: 32 and 128 shares, 20 / 60 us against 33 / 48).
+    if (shares > 1 && (dt == kernels::kF16 || kernels::gemm_bf16_split_k(a) == 1 || (a.K <= 16 * 64ll * shares && shares <= 64))) {
       kernels::GemmArgs b = a;
       Tensor ws = at::empty({shares * a.M * ((a.N + 3) / 4 * 4)}, like.options().dtype(at::kFloat));
       b.workspace = ws.data_ptr<float>();
@@ -730,6 +733,8 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_backward(Tensor dy, Tensor w, Te
   }
   if (sums > 0) {
     kernels::launch_reduce_partials(partial.data_ptr<float>(), db->data_ptr(), 2 * H, static_cast<int>(sums), dt, s);
+  } else if (want_db && kernels::colsum_few_rows_supported(M, 2 * H)) {
+    kernels::launch_colsum_few_rows(dgu.data_ptr(), db->data_ptr(), M, 2 * H, dt, s);
   } else if (want_db) {
     Tensor ws = at::empty({kernels::colreduce_workspace(M, 2 * H)}, dy.options().dtype(at::kFloat));
     kernels::launch_colsum(dgu.data_ptr(), db->data_ptr(), ws.data_ptr<float>(), M, 2 * H, dt, s);
@@ -799,7 +804,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rank1_mlp_backward(Tensor dy, Tensor 
 
 // Gradients of y = x W^T + b given g = dL/d(xW^T+b).  Returns (dx or None, dW, db or None).
 // dw_out: write the weight gradient into this tensor (a slice of a gradient bucket) instead of a fresh one.
-// spread: see run_gemm.
+// spread: see run_gemm; the column sums of few rows are then taken in one launch.
 std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward(Tensor g, Tensor x, Tensor w, bool need_dx, bool need_db,
                                                                                    c10::optional<Tensor> dw_out, bool spread) {
   check_gpu(g, "grad");
@@ -853,7 +858,9 @@ std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward
       TORCH_CHECK(gemm_path_ok(b, dt), "linear_backward: input-gradient shape not supported by the MFMA GEMM");
       run_gemm(b, dt, s, g, spread);
     }
-    if (need_db) {
+    if (need_db && spread && kernels::colsum_few_rows_supported(M, N)) {
+      kernels::launch_colsum_few_rows(g.data_ptr(), db->data_ptr(), M, N, dt, s);
+    } else if (need_db) {
       Tensor ws = at::empty({kernels::colreduce_workspace(M, N)}, fopt);
       kernels::launch_colsum(g.data_ptr(), db->data_ptr(), ws.data_ptr<float>(), M, N, dt, s);
     }

@@ -45,6 +45,7 @@ class _TopKDistillation(torch.autograd.Function):
     def forward(ctx, logits, ids, teacher, targets, cfg):
         reduction, ignore_index, n_classes, temperature, hard_weight = cfg
         C = _ext.C()
+        ctx.set_materialize_grads(False)  # (of the two by-products: zeros that nobody reads)
         mean = reduction == "mean"
         ctx.cfg = cfg
         ctx.needs = ctx.needs_input_grad[0]
@@ -59,6 +60,8 @@ class _TopKDistillation(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _dcorrect, _dmetrics):
+        if dloss is None:
+            return (None,) * 5
         C = _ext.C()
         g = dloss.detach().to(torch.float32).contiguous()
         logits, ids, teacher, targets, stats = ctx.saved_tensors
@@ -81,6 +84,7 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2, weight, ids, teacher, targets, cfg, impl):
         reduction, ignore_index, n_classes, temperature, hard_weight = cfg
+        ctx.set_materialize_grads(False)
         logits = gemm.nt(x2, weight, None, impl)
         grad = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         inplace = grad and logits.dtype != torch.float16
@@ -97,6 +101,8 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _dcorrect, _dmetrics):
+        if dloss is None:
+            return (None,) * 7
         g = dloss.detach().to(torch.float32).reshape(())
         C = _ext.C()
         if ctx.inplace:

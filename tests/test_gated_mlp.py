@@ -295,3 +295,20 @@ def test_a_second_derivative_is_refused(dtype):
     (g,) = torch.autograd.grad(y.float().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.float().square().sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,N", [(1, 24), (63, 33), (64, 64), (513, 100), (1003, 2772), (2047, 71), (2048, 40), (2049, 40)])
+def test_bias_gradients_of_few_and_many_rows(M, N, dtype):
+    from distributed_pytorch_amd import _ext
+
+    g = torch.randn(M, N, device=DEV).to(dtype)
+    g[M // 2, N - 1] = float("inf")                      # an infinite sum, not a NaN
+    x, w = torch.randn(M, 8, device=DEV).to(dtype), torch.randn(N, 8, device=DEV).to(dtype)
+    db = _ext.C().linear_backward(g, x, w, False, True, None, True)[2]
+    want = g.double().sum(0)
+    # M float32 additions and one rounding to the type
+    bound = M * 2.0 ** -24 * g.double().abs().sum(0) + torch.finfo(dtype).eps / 2 * want.abs() + 1e-12
+    assert db[N - 1] == float("inf")
+    assert bool(((db.double() - want).abs() <= bound)[: N - 1].all())
