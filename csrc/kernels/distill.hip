@@ -17,6 +17,10 @@
 // holds one bit per vector (a wave's 64 vectors are one 64-bit word, so most waves skip the look-up on a scalar
 // branch) and a chained hash from vector to entries.  Entries of one class are summed beforehand in index order by the
 // first of them, which makes the result independent of the order in which the chains were built.
+// Bound by memory with one temperature: 8192 x 50304 bf16, 32 entries, forward and gradient in 340 us (4.85 TB/s, the rate of a copy); 2049 x 50257
+// fp32 with a second exponential 203 us (4.1 TB/s).  With both temperatures and powers 24576 x 50304 bf16 in place take 1.27 ms (3.9 TB/s):
+// by count 19 issue slots an element, 8 of them its two exponentials, which the two rows that fit a compute unit do not hide entirely.
+// Everything is fp32 but the logits and their gradient; in fp16 the gradient is only ever rounded with the upstream gradient in it.
 // Rows need no alignment: element j of a row sits in vector (j + shift) / V of the 16-byte grid, the vectors at both ends are stored
 // element by element.
 #include <type_traits>

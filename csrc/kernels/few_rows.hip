@@ -5,7 +5,8 @@
 // kernels put 128 x 128 outputs on a workgroup and walk the contraction alone, 6 workgroups for W [768, 2048] (29 us for one token).  Here a
 // workgroup owns 16 outputs (16 of either half of a gated pair), its eight waves take the contraction 64 at a time in turns, each
 // loading 128 consecutive bytes of 16 weight rows straight into matrix operands -- W is never staged, no element of it is used twice -- and
-// the waves' sums meet in LDS.  v_mfma_f32_16x16x32 takes the weight rows as A and 16 rows of x as B, so a lane ends up with
+// the waves' sums meet in LDS.  One token through W [4096, 768] as a gated pair: 4.8 us, through W [768, 2048]: 5.7 us, most of either a launch and two
+// trips to memory.  v_mfma_f32_16x16x32 takes the weight rows as A and 16 rows of x as B, so a lane ends up with
 // four consecutive outputs of one row of x.
 #include <type_traits>
 

@@ -93,7 +93,9 @@ __device__ __forceinline__ void store_tile_bf16(const GemmArgs& p, const f32x4& 
 // Gated pair of projections (GemmArgs::gate).  The gate's and the up projection's rows of the weight are interleaved 16 by 16
 // on their way into a tile: row v of the product's N dimension is row (v >> 5) * 16 + (v & 15) of the gate (bit 4 of v clear) or of the
 // up projection (set).  Neighbouring accumulator tiles of a wave then hold g and u of the same elements in the same registers, and the
-// product of the two needs no exchange between lanes.
+// product of the two needs no exchange between lanes.  h is taken from the fp32 sums; g | u, kept for the backward, are rounded to 16 bits, as
+// h and dg | du are: in fp32 the epilogues would move twice the bytes, and those are what they wait for.  65536 x 768 x (2 * 2048) with SiLU:
+// 474 us where the product with h alone takes 349 us (0.9 GB written, 870 TFLOP/s); backward 367 us (1.2 GB, 240 us at the rate of a copy).
 __device__ __forceinline__ long long gate_row(long long v) { return ((v >> 5) << 4) + (v & 15); }
 
 // h and (when wanted) g | u of four consecutive columns col .. col + 3 of one row, out of accumulators that hold no bias yet.

@@ -13,17 +13,23 @@
 // skips the tiles that miss its own 32 rows, and only tiles that straddle a border of the mask pay for the comparisons.  The
 // products run transposed (S^T = K Q^T), so a query's softmax statistics are scalars of its lane and the probabilities leave the
 // accumulators as the operand of the next product without changing lanes; the other operand of that product comes
-// from the row-major tile through the transposing LDS read.  Tiles travel global -> LDS by DMA through a ring, requested one or two
-// tile ahead.  The tile image is one for both kinds of reads: 16-byte chunk c of row r sits at chunk c ^ swz(r).  The 16 lanes that a row-wise
+// from the row-major tile through the transposing LDS read.  Probabilities and score gradients are rounded to the 16-bit type there, as operands
+// of a matrix instruction have to be; scores, statistics, delta and all sums are fp32, and the row sums add up the rounded probabilities, so that
+// a row's weights sum to 1.  Tiles travel global -> LDS by DMA, requested one tile (two in the dK/dV kernel at head size 128) ahead.  The tile image is one for both kinds of reads: 16-byte chunk c of row r sits at chunk c ^ swz(r).  The 16 lanes that a row-wise
 // read serves at once (rows 0-3 and 12-15 at one chunk, rows 4-11 at the next) then fall on 16 different 16-byte bank groups, and the 8
 // rows of a transposing read on 8 different 32-byte groups.
 // Rows at and beyond a sequence's length are never read: source rows are clamped to the last valid one, what they
 // would contribute is masked, and their outputs and gradients are written as zero.
 //
 // dK/dV: blocks of 128 keys cost unlike amounts -- a block with sinks meets every later query of every head of its group, the
-// others only a window of them -- so the list of (key block, head, query tile) units is cut into equal pieces, one per
+// others only a window of them -- so the list of (key block, head, query tile) units is cut into pieces of about equal length, one per
 // workgroup slot of the chip.  A block inside one piece is written directly; a block that is cut leaves fp32 partial
 // sums, which a last kernel adds up in order: no atomics, the same result every time.
+//
+// Measured (bf16), window 256 / sinks 4 over 64 x 1024 positions, 12 heads of 64: forward 128 us (3.1 TB/s of its inputs and outputs), dQ 174 us
+// (3.5 TB/s), dK/dV 222 us (2.7 TB/s): between the memory's rate and the vector work per score (an exponential, a product and half a
+// conversion beside 2 to 4 x 64 multiply-adds).  Window 1024 / sinks 4 over 16384 positions, 8 heads of 128 on 2: forward 105 us (636 TFLOP/s of
+// the visible pairs), dQ 127 us (784), dK/dV 257 us (520; one workgroup a compute unit, its accumulators and K / V rows fill the registers), join 17 us.
 #include <type_traits>
 
 #include "device_utils.h"
