@@ -170,3 +170,76 @@ def test_optimizer_steps_change_every_parameter():
         loss.backward()
         opt.step()
     assert bool(torch.isfinite(loss.detach())) and all(not torch.equal(p, before[n]) for n, p in m.named_parameters())
+
+
+@pytest.fixture()
+def one_rank():
+    from distributed_pytorch_amd.parallel import process_group as pg
+    from distributed_pytorch_amd.parallel.store import Store
+
+    store = Store("127.0.0.1", 0, is_host=True, bind_addr="127.0.0.1")
+    pg.init_process_group(0, 1, "rccl", store=store)
+    yield pg
+    pg.destroy_process_group()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_student_under_the_reducer_matches_plain_training(one_rank, dtype):
+    """Weight gradients go straight into their bucket slices (the tied embedding's second one, and those of a second backward before
+    the step, have to be added): exactly the weights of training without the wrapper."""
+    from distributed_pytorch_amd.ops import FusedAdamW
+    from distributed_pytorch_amd.parallel.ddp import DistributedDataParallel
+
+    cfg = config()
+    torch.manual_seed(0)
+    plain, twin = GPT2(cfg).to("cuda", dtype), GPT2(cfg).to("cuda", dtype)
+    twin.load_state_dict(plain.state_dict())
+    ddp = DistributedDataParallel(twin, device_ids=[0], bucket_cap_mb=0.25, first_bucket_mb=0.05)
+    optimizers = [FusedAdamW(m.parameters(), 1e-3, master_weights=dtype != torch.float32) for m in (plain, ddp)]
+    losses = ([], [])
+    for step in range(4):
+        for k, (model, opt) in enumerate(zip((plain, ddp), optimizers)):
+            opt.zero_grad(set_to_none=True)
+            for part in range(2 if step == 3 else 1):
+                idx, targets, ids, values = batch(3, 160, cfg.vocab_size, device="cuda", seed=2 * step + part)
+                if part == 0 and step == 3 and model is ddp:
+                    with ddp.no_sync():
+                        loss = model(idx, targets, teacher=(ids, values), temperature=2.0, hard_weight=0.5)
+                        (loss * 0.5).backward()
+                else:
+                    loss = model(idx, targets, teacher=(ids, values), temperature=2.0, hard_weight=0.5)
+                    (loss * 0.5 if step == 3 else loss).backward()
+                losses[k].append(float(loss.detach()))
+            opt.step()
+    assert losses[0] == losses[1], losses
+    for (n, a), b in zip(plain.named_parameters(), ddp.module.parameters()):
+        assert torch.equal(a, b), n
+
+
+@gpu
+@pytest.mark.parametrize("rows", [5, 300])
+def test_a_gated_block_used_twice_under_the_reducer(one_rank, rows):
+    from distributed_pytorch_amd.ops import gated_mlp
+    from distributed_pytorch_amd.parallel.ddp import DistributedDataParallel
+
+    class Twice(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w_fc, self.b_fc = torch.nn.Parameter(torch.randn(2 * 136, 72) / 8), torch.nn.Parameter(torch.randn(2 * 136))
+            self.w_proj, self.b_proj = torch.nn.Parameter(torch.randn(72, 136) / 11), torch.nn.Parameter(torch.randn(72))
+
+        def forward(self, x):
+            for _ in range(2):
+                x = gated_mlp(x, self.w_fc, self.b_fc, self.w_proj, self.b_proj)
+            return x
+
+    torch.manual_seed(0)
+    plain, twin = Twice().to("cuda", torch.bfloat16), Twice().to("cuda", torch.bfloat16)
+    twin.load_state_dict(plain.state_dict())
+    ddp = DistributedDataParallel(twin, device_ids=[0])
+    x = torch.randn(rows, 72, device="cuda").bfloat16()
+    for m in (plain, ddp):
+        m(x).float().square().mean().backward()
+    for a, b in zip(plain.parameters(), ddp.module.parameters()):
+        assert torch.equal(a.grad, b.grad)
