@@ -329,7 +329,19 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
   if (!GRAD) return;
 
   // ---- gradient
-  float w = a.scale[0];
+  float w = 1.f;
+  if (a.scale) {
+    w = a.scale[0];
+  } else if (a.mean) {  // few rows: every wave counts them itself
+    int n = static_cast<int>(a.N);
+    if (a.targets) {
+      n = 0;
+      for (int i = lane; i < a.N; i += 64) n += a.targets[i] != a.ignore_index ? 1 : 0;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+    }
+    w = 1.f / fmaxf(static_cast<float>(n), 1.f);
+  }
   if (MODE == kBackward) w *= a.grad_out[a.grad_out_rows ? r : 0];
   const float cs = some ? w * a.soft_weight * a.tau : 0.f, ch = w * a.hard_weight;
   // coefficients of the exponentials: with one temperature both terms share it (tau = 1) or one of them is absent

@@ -1935,17 +1935,19 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream) {
 }
 
 // Shares of the contraction that let a product with few 128x128 tiles fill the chip: two workgroups per compute unit, at least four k-steps a
-// share, 64 MiB of sums at most.  1: not worth it -- writing, reading and adding the sums costs about as much as 10 k-steps, so at least 12 have to
-// be saved (fp16 1003 x 520 x 1386, 18 saved: 21 -> 17 us; bf16 2048 x 1024 x 768, 9 saved: 15 -> 25 us).
+// share, 64 MiB of sums at most.  1: not worth it -- writing, reading and adding the sums costs about as much as 10 k-steps, and another launch and
+// its workspace cost the host 5 us, which products this small wait for: at least 16 have to be saved (fp16 1003 x 520 x 1386, 18 saved:
+// 21 -> 17 us; 1024^3, 12 saved: 17 -> 19 us; weight gradient [520, 1386] of 1003 rows, 12 saved: 19 -> 14 us, but the training pass of the gated
+// block around it 141 -> 152 us; bf16 2048 x 1024 x 768, 9 saved: 15 -> 25 us).
 int gemm_spread(const GemmArgs& a) {
   const long long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN), nk = (a.K + BK - 1) / BK;
   const int cus = compute_units();
-  if (tiles >= cus || nk < 6) return 1;
+  if (tiles >= cus || nk < 16) return 1;
   long long s = 2ll * cus / tiles;
   if (s > nk / 4) s = nk / 4;
   const long long plane = a.M * ((a.N + 3) & ~3ll) * 4;
   if (s > (64ll << 20) / plane) s = (64ll << 20) / plane;
-  return s < 2 || nk - nk / s < 12 ? 1 : static_cast<int>(s);
+  return s < 2 || nk - nk / s < 16 ? 1 : static_cast<int>(s);
 }
 
 void launch_gemm_spread(const GemmArgs& a, int dtype, hipStream_t stream) {

@@ -102,6 +102,7 @@ void launch_xent_fused(void* logits, int dtype, const long long* targets, long l
 // mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits
 // dlogits [N, ld]: columns [C, ld) are written as zero; its address must equal that of logits modulo 16.
 constexpr int kDistillMaxEntries = 1024;
+constexpr long long kDistillCountRows = 512;
 constexpr long long kDistillMaxWidth = 1 << 20;  // of ld: one bit per 16 bytes of a row is kept in LDS
 struct DistillArgs {
   const void* logits;
@@ -115,7 +116,8 @@ struct DistillArgs {
   float* row_loss;
   float* row_stats;
   unsigned char* correct;
-  const float* scale;
+  const float* scale;      // launch_distill_scale's, or nullptr for few rows (kDistillCountRows at most)
+  int mean;                // of a nullptr scale: 1 / #rows that count, else 1
   const float* grad_out;
   int grad_out_rows;
   // set by the launcher

@@ -332,7 +332,7 @@ kernels::DistillArgs distill_args(const Tensor& logits, const Tensor& ids, const
   return a;
 }
 
-// Returns (loss [], row_loss [N], correct [N], metrics [4], scale [1], row_stats [N, 3] or undefined, dlogits or undefined).
+// Returns (loss [], row_loss [N], correct [N], metrics [4], scale [1] or undefined (few rows), row_stats [N, 3] or undefined, dlogits or undefined).
 // gradient: "none" (row_stats are kept for distill_backward), "new" (dlogits for a unit upstream gradient in a fresh
 // tensor) or "inplace" (the same, over the logits).
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> distill_forward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets,
@@ -343,11 +343,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> distill_forwa
   DevGuard g(logits);
   hipStream_t s = stream_of(logits);
   auto fopt = logits.options().dtype(at::kFloat);
-  Tensor loss = at::empty({}, fopt), row_loss = at::empty({a.N}, fopt), metrics = at::empty({4}, fopt), scale = at::empty({1}, fopt), stats, dlogits;
+  Tensor loss = at::empty({}, fopt), row_loss = at::empty({a.N}, fopt), metrics = at::empty({4}, fopt), scale, stats, dlogits;
   Tensor correct = at::empty({a.N}, logits.options().dtype(at::kBool));
   a.row_loss = row_loss.data_ptr<float>();
   a.correct = reinterpret_cast<unsigned char*>(correct.data_ptr<bool>());
-  a.scale = scale.data_ptr<float>();
+  a.mean = mean ? 1 : 0;
+  if (a.N > kernels::kDistillCountRows) {
+    scale = at::empty({1}, fopt);
+    a.scale = scale.data_ptr<float>();
+    kernels::launch_distill_scale(a.targets, a.N, ignore_index, a.mean, scale.data_ptr<float>(), s);
+  }
   if (gradient == "none") {
     stats = at::empty({a.N, 3}, fopt);
     a.row_stats = stats.data_ptr<float>();
@@ -355,28 +360,32 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> distill_forwa
     dlogits = gradient == "inplace" ? logits : at::empty_like(logits);
     a.dlogits = dlogits.data_ptr();
   }
-  kernels::launch_distill_scale(a.targets, a.N, ignore_index, mean ? 1 : 0, scale.data_ptr<float>(), s);
   kernels::launch_distill(a, kdtype(logits), gradient == "none" ? 0 : 2, s);
   kernels::launch_distill_reduce(a.row_loss, a.correct, a.targets, a.N, ignore_index, mean ? 1 : 0, metrics.data_ptr<float>(), loss.data_ptr<float>(), s);
   return {loss, row_loss, correct, metrics, scale, stats, dlogits};
 }
 
 // dlogits from the statistics of a "none" forward.  grad_out: one value, or one per row.
-Tensor distill_backward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets, Tensor row_stats, Tensor scale, Tensor grad_out,
-                        int64_t n_classes, int64_t ignore_index, double temperature, double hard_weight) {
+Tensor distill_backward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets, Tensor row_stats, c10::optional<Tensor> scale,
+                        Tensor grad_out, int64_t n_classes, int64_t ignore_index, double temperature, double hard_weight, bool mean) {
   kernels::DistillArgs a = distill_args(logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, "distill_backward");
   check_gpu(row_stats, "row_stats");
-  check_gpu(scale, "scale");
   check_gpu(grad_out, "grad_out");
-  TORCH_CHECK(row_stats.scalar_type() == at::kFloat && row_stats.numel() == 3 * a.N && scale.scalar_type() == at::kFloat && scale.numel() == 1,
-              "distill_backward: row_stats [N, 3] and scale [1] must be float32");
+  TORCH_CHECK(row_stats.scalar_type() == at::kFloat && row_stats.numel() == 3 * a.N, "distill_backward: row_stats must be float32 [N, 3]");
+  a.mean = mean ? 1 : 0;
+  if (scale.has_value() && scale->defined()) {
+    check_gpu(*scale, "scale");
+    TORCH_CHECK(scale->scalar_type() == at::kFloat && scale->numel() == 1, "distill_backward: scale must be float32 [1]");
+    a.scale = scale->data_ptr<float>();
+  } else {
+    TORCH_CHECK(a.N <= kernels::kDistillCountRows, "distill_backward: more than ", kernels::kDistillCountRows, " rows need the forward's scale");
+  }
   TORCH_CHECK(grad_out.scalar_type() == at::kFloat && (grad_out.dim() <= 1) && (grad_out.numel() == 1 || grad_out.numel() == a.N),
               "distill_backward: grad_out must be one float32 value or one per row");
   DevGuard g(logits);
   Tensor dlogits = at::empty_like(logits);
   a.dlogits = dlogits.data_ptr();
   a.row_stats = row_stats.data_ptr<float>();
-  a.scale = scale.data_ptr<float>();
   a.grad_out = grad_out.data_ptr<float>();
   a.grad_out_rows = grad_out.dim() == 1 && grad_out.numel() == a.N ? 1 : 0;
   kernels::launch_distill(a, kdtype(logits), 1, stream_of(logits));
@@ -1341,7 +1350,7 @@ void init_ops(py::module_& m) {
         py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"), py::arg("hard_weight"), py::arg("mean"), py::arg("gradient") = "none");
   m.def("distill_backward", &distill_backward, py::arg("logits"), py::arg("teacher_ids"), py::arg("teacher_logits"), py::arg("targets"),
         py::arg("row_stats"), py::arg("scale"), py::arg("grad_out"), py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"),
-        py::arg("hard_weight"));
+        py::arg("hard_weight"), py::arg("mean") = true);
   m.def("distill_apply_upstream", &distill_apply_upstream, py::arg("x"), py::arg("g"));
   m.attr("DISTILL_MAX_ENTRIES") = kernels::kDistillMaxEntries;
   m.def("dgrad_act_backward", &dgrad_act_backward, py::arg("dout"), py::arg("weight"), py::arg("aux"), py::arg("act"), py::arg("want_colsum"));

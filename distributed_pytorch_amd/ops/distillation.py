@@ -72,7 +72,7 @@ class _TopKDistillation(torch.autograd.Function):
         reduction, ignore_index, n_classes, temperature, hard_weight = ctx.cfg
         if stats is None:
             stats = C.distill_forward(logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, reduction == "mean", "none")[5]
-        d = C.distill_backward(logits, ids, teacher, targets, stats, ctx.scale, g, n_classes, ignore_index, temperature, hard_weight)
+        d = C.distill_backward(logits, ids, teacher, targets, stats, ctx.scale, g, n_classes, ignore_index, temperature, hard_weight, reduction == "mean")
         return d, None, None, None, None
 
 
@@ -109,8 +109,8 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
             x2, weight, dlogits = ctx.saved_tensors
         else:
             x2, weight, logits, ids, teacher, targets, scale, stats = ctx.saved_tensors
-            _, ignore_index, n_classes, temperature, hard_weight = ctx.cfg
-            dlogits = C.distill_backward(logits, ids, teacher, targets, stats, scale, g, n_classes, ignore_index, temperature, hard_weight)
+            reduction, ignore_index, n_classes, temperature, hard_weight = ctx.cfg
+            dlogits = C.distill_backward(logits, ids, teacher, targets, stats, scale, g, n_classes, ignore_index, temperature, hard_weight, reduction == "mean")
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = gemm.nn(dlogits, weight, ctx.impl)

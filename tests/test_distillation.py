@@ -495,3 +495,28 @@ def test_a_second_derivative_is_refused(dtype):
         (g,) = torch.autograd.grad(r.loss, x, create_graph=True)
         with pytest.raises(RuntimeError):
             g.float().square().sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("N", [1, 2, 63, 64, 65, 512, 513])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_rows_are_counted_alike_by_few_and_many(N, dtype):
+    logits, ids, teacher, targets = make(N, 40, 6, dtype, DEV)
+    logits = logits + 20
+    targets[N // 2:] = -100 if N > 2 else targets[N // 2:]
+    near = 64 * 2.0 ** -23 * 2
+    for reduction in ("mean", "sum"):
+        x = logits.clone().requires_grad_()
+        r = topk_distillation(x, ids, teacher, targets, 2.0, 0.5, reduction=reduction)
+        rows, grad, n = reference(logits, ids, teacher, targets, 2.0, 0.5)
+        n = n if reduction == "mean" else 1
+        (g,) = torch.autograd.grad(r.loss, x, retain_graph=True)
+        (again,) = torch.autograd.grad(r.loss, x)
+        assert torch.equal(g, again)
+        torch.testing.assert_close(g.double().cpu(), grad / n, rtol=torch.finfo(dtype).eps / 2 * 1.01, atol=near / n + (2.0 ** -25 if dtype == torch.float16 else 0))
+    x = logits.clone().requires_grad_()
+    r = topk_distillation(x, ids, teacher, None, 2.0, 0.0)
+    rows, grad, n = reference(logits, ids, teacher, None, 2.0, 0.0)
+    assert n == N
+    (g,) = torch.autograd.grad(r.loss, x)
+    torch.testing.assert_close(g.double().cpu(), grad / n, rtol=torch.finfo(dtype).eps / 2 * 1.01, atol=near / n + (2.0 ** -25 if dtype == torch.float16 else 0))
