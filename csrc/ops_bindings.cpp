@@ -693,6 +693,28 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_forward(Tensor x, Tensor w, c10:
   return {h, gu};
 }
 
+// The whole block without a backward, y = h W_proj^T + b_proj for x [..., K]; None where the tensors are not such that the kernels take them as they
+// are (the caller then says why, or brings them into shape).  One call, because for single tokens the host is what a call costs.
+c10::optional<Tensor> gated_mlp_forward(Tensor x, Tensor w, c10::optional<Tensor> b, Tensor wp, c10::optional<Tensor> bp, int64_t act) {
+  auto fits = [&](const Tensor& t) {
+    return t.is_cuda() && t.scalar_type() == x.scalar_type() && t.get_device() == x.get_device() && t.is_contiguous() &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  };
+  const auto dt = x.scalar_type();
+  if (dt != at::kFloat && dt != at::kBFloat16 && dt != at::kHalf) return c10::nullopt;
+  if (x.dim() < 1 || x.numel() == 0 || w.dim() != 2 || wp.dim() != 2 || !fits(x) || !fits(w) || !fits(wp)) return c10::nullopt;
+  const int64_t K = x.size(-1), H = wp.size(1), N = wp.size(0);
+  if (H == 0 || N == 0 || w.size(0) != 2 * H || w.size(1) != K) return c10::nullopt;
+  if (b.has_value() && !(fits(*b) && b->dim() == 1 && b->size(0) == 2 * H)) return c10::nullopt;
+  if (bp.has_value() && !(fits(*bp) && bp->dim() == 1 && bp->size(0) == N)) return c10::nullopt;
+  Tensor h = std::get<0>(gated_forward(x.dim() == 2 ? x : x.view({-1, K}), w, b, act, false));
+  Tensor y = std::get<0>(linear_forward(h, wp, bp, kernels::kActNone, false, true));
+  if (x.dim() == 2) return y;
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  return y.view(sizes);
+}
+
 // g | u's gradient [M, 2 H] from dy [M, N], the output projection W [N, H] and the saved g | u; with want_db also its column sums (the bias gradient).
 std::tuple<Tensor, c10::optional<Tensor>> gated_backward(Tensor dy, Tensor w, Tensor gu, int64_t act, bool want_db) {
   check_gpu(dy, "dy");
@@ -1387,6 +1409,7 @@ void init_ops(py::module_& m) {
   m.def("rank1_mlp_forward", &rank1_mlp_forward, py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("b2"), py::arg("act") = 0);
   m.def("rank1_mlp_backward", &rank1_mlp_backward, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("act") = 0);
   m.def("gated_forward", &gated_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("save") = true);
+  m.def("gated_mlp_forward", &gated_mlp_forward, py::arg("x"), py::arg("w_fc"), py::arg("b_fc"), py::arg("w_proj"), py::arg("b_proj"), py::arg("act"));
   m.def("gated_backward", &gated_backward, py::arg("dy"), py::arg("weight"), py::arg("gu"), py::arg("act"), py::arg("want_db") = false);
   m.def("act_backward", &act_backward, py::arg("dy"), py::arg("saved"), py::arg("act"), py::arg("need_db") = false);
   m.def("colsum", &colsum);

@@ -160,6 +160,11 @@ def gated_mlp(x: torch.Tensor, w_fc: torch.Tensor, b_fc: Optional[torch.Tensor],
     code = _GATES.get(act)
     if code is None:
         raise ValueError(f"unknown gate activation {act!r} (silu | gelu | relu)")
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_fc, b_fc, w_proj, b_proj))
+    if x.is_cuda and not grad:
+        y = _ext.C().gated_mlp_forward(x, w_fc, b_fc, w_proj, b_proj, code)
+        if y is not None:
+            return y
     if w_fc.dim() != 2 or w_proj.dim() != 2 or w_fc.shape[0] % 2 or w_fc.shape[0] == 0 or w_proj.shape[1] * 2 != w_fc.shape[0]:
         raise ValueError(f"w_fc must be [2 * H, K] and w_proj [N, H], got {tuple(w_fc.shape)} and {tuple(w_proj.shape)}")
     if x.dim() < 1 or x.shape[-1] != w_fc.shape[1] or w_fc.shape[1] == 0 or w_proj.shape[0] == 0:
@@ -179,10 +184,8 @@ def gated_mlp(x: torch.Tensor, w_fc: torch.Tensor, b_fc: Optional[torch.Tensor],
         raise RuntimeError(f"gated_mlp: no native kernel for {x.dtype}")
     x2 = _aligned(x.reshape(-1, x.shape[-1]))
     tensors = [_aligned(t) for t in (w_fc, b_fc, w_proj, b_proj)]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, *tensors)):
+    if grad:
         y = _GatedMLP.apply(x2, *tensors, code)
     else:
-        C = _ext.C()
-        h, _ = C.gated_forward(x2, tensors[0], tensors[1], code, False)
-        y, _ = C.linear_forward(h, tensors[2], tensors[3], 0, False, True)
+        y = _ext.C().gated_mlp_forward(x2, *tensors, code)
     return y.reshape(*x.shape[:-1], w_proj.shape[0])

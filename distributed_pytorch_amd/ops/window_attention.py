@@ -49,13 +49,14 @@ def _native_layout(qkv: torch.Tensor) -> bool:
     return (T <= 1 or (qkv.stride(1) >= W and qkv.stride(1) % 8 == 0)) and (B <= 1 or (qkv.stride(0) >= 0 and qkv.stride(0) % 8 == 0))
 
 
-def native_window_attention_supported(qkv: torch.Tensor, n_head: int, n_kv_head: int) -> bool:
-    """True when the kernels take ``qkv`` (after a copy, where its rows are not contiguous and aligned)."""
+def native_window_attention_supported(qkv: torch.Tensor, n_head: int, n_kv_head: int, layout: Optional[bool] = None) -> bool:
+    """True when the kernels take ``qkv`` (after a copy, where its rows are not contiguous and aligned).  layout: ``_native_layout(qkv)``, where
+    it is known."""
     name = _NAMES.get(qkv.dtype)
     if name is None or not qkv.is_cuda or not _ext.have_C():
         return False
     B, T, W = qkv.shape
-    stride = qkv.stride(1) if _native_layout(qkv) and T > 1 else W
+    stride = qkv.stride(1) if T > 1 and (_native_layout(qkv) if layout is None else layout) else W
     return bool(_ext.C().window_attention_supported(B, T, n_head, n_kv_head, W // (n_head + 2 * n_kv_head), stride, name))
 
 
@@ -110,8 +111,9 @@ def window_attention_qkvpacked(qkv: torch.Tensor, n_head: int, window: int, sink
     if impl != "composed":
         if torch.is_autocast_enabled() and qkv.is_cuda and qkv.dtype not in _NAMES:
             qkv = qkv.to(torch.get_autocast_dtype("cuda"))
-        if native_window_attention_supported(qkv, n_head, n_kv):
-            if not _native_layout(qkv):
+        layout = _native_layout(qkv)
+        if native_window_attention_supported(qkv, n_head, n_kv, layout):
+            if not layout:
                 qkv = qkv.clone(memory_format=torch.contiguous_format)
             if lens is not None:
                 lens = (lens if lens.dtype == torch.int32 else lens.clamp(0, qkv.shape[1]).to(torch.int32)).contiguous()
