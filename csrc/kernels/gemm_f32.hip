@@ -46,7 +46,7 @@ __device__ __forceinline__ int kmajor_off(int row, int c) { return row * BK + ((
 //   !KMAJOR: tile is k [k0, k0+32) x rows [r0, r0+128) of a [K][ld] matrix (rows contiguous)
 // ALIGNED: base address, leading dimension and contiguous extent are multiples of 4 floats, so a 4-float piece is
 // one aligned 16-byte load or wholly outside the matrix.  Otherwise the piece is gathered float by float with a
-// bounds check each (the tail path for odd shapes).
+// bounds check each (the tail path for odd shapes, which only the last k-step of a row takes: see load_inner_tile).
 template <bool KMAJOR, bool ALIGNED>
 __device__ __forceinline__ void load_tile(const float* __restrict__ base, long long ld, long long r0, long long R, long long k0,
                                           long long K, f32x4 (&regs)[4]) {
@@ -77,6 +77,20 @@ __device__ __forceinline__ void load_tile(const float* __restrict__ base, long l
   }
 }
 
+// A tile of an odd shape that ends ahead of the contraction's last index (k0 + BK < K; ld >= 4): whole 16-byte loads from wherever they start and no
+// branches.  Rows beyond the matrix repeat its last one, a piece across the end of a row runs on into the next row, and both end up in
+// outputs that are not stored.  (464 x 2112 x 685, gathered float by float: 87 us, so: 67, with K = 684: 65.)
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+template <bool KMAJOR>
+__device__ __forceinline__ void load_inner_tile(const float* __restrict__ base, long long ld, long long r0, long long R, long long k0, f32x4 (&regs)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int id = threadIdx.x + i * kThreads;
+    const long long row = r0 + (KMAJOR ? id >> 3 : (id & 31) << 2), in = row < R ? row : R - 1;
+    regs[i] = *reinterpret_cast<const f32x4_any*>(KMAJOR ? base + in * ld + k0 + ((id & 7) << 2) : base + (k0 + (id >> 5)) * ld + in);
+  }
+}
+
 template <bool KMAJOR>
 __device__ __forceinline__ void store_tile(float* lds, const f32x4 (&regs)[4]) {
 #pragma unroll
@@ -101,7 +115,8 @@ __device__ __forceinline__ f32x4 read_frag(const float* lds, int tile_row0, int 
   }
 }
 
-template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED>
+// SPREAD: blockIdx.y takes its share of the contraction (p.split_k shares) and leaves raw sums in p.workspace[share][M][N].
+template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED, bool SPREAD = false>
 __global__ __launch_bounds__(kThreads, 2) void gemm_f32_kernel(GemmArgs p, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(16))) float smem[];
 
@@ -127,20 +142,27 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_f32_kernel(GemmArgs p, int t
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
   f32x4 ra[4], rb[4];
-  const long long nk = (p.K + BK - 1) / BK;
-  load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, 0, p.K, ra);
-  load_tile<B_KMAJOR, ALIGNED>(B, p.ldb, n0, p.N, 0, p.K, rb);
+  const long long nk_all = (p.K + BK - 1) / BK;
+  const long long kt0 = SPREAD ? nk_all * blockIdx.y / p.split_k : 0, nk = SPREAD ? nk_all * (blockIdx.y + 1) / p.split_k : nk_all;
+  const long long inner = !ALIGNED && p.lda >= 4 && p.ldb >= 4 ? (p.K - 1) / BK : 0;  // k-steps that load_inner_tile may load
+  auto load = [&](long long kt) __attribute__((always_inline)) {
+    if (!ALIGNED && kt < inner) {
+      load_inner_tile<A_KMAJOR>(A, p.lda, m0, p.M, kt * BK, ra);
+      load_inner_tile<B_KMAJOR>(B, p.ldb, n0, p.N, kt * BK, rb);
+    } else {
+      load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, kt * BK, p.K, ra);
+      load_tile<B_KMAJOR, ALIGNED>(B, p.ldb, n0, p.N, kt * BK, p.K, rb);
+    }
+  };
+  load(kt0);
   store_tile<A_KMAJOR>(smem, ra);
   store_tile<B_KMAJOR>(smem + kTileFloats, rb);
   __syncthreads();
 
   int cur = 0;
-  for (long long kt = 0; kt < nk; ++kt) {
+  for (long long kt = kt0; kt < nk; ++kt) {
     const bool more = kt + 1 < nk;
-    if (more) {
-      load_tile<A_KMAJOR, ALIGNED>(A, p.lda, m0, p.M, (kt + 1) * BK, p.K, ra);
-      load_tile<B_KMAJOR, ALIGNED>(B, p.ldb, n0, p.N, (kt + 1) * BK, p.K, rb);
-    }
+    if (more) load(kt + 1);
     const float* as = smem + cur * 2 * kTileFloats;
     const float* bs = as + kTileFloats;
 #pragma unroll
@@ -168,7 +190,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_f32_kernel(GemmArgs p, int t
   }
 
   // Epilogue.  Accumulator register e of lane l holds C[row = (e&3) + 8*(e>>2) + 4*(l>>5)][col = l&31].
-  float* C = static_cast<float*>(p.C);
+  float* C = SPREAD ? p.workspace + static_cast<long long>(blockIdx.y) * p.M * p.N : static_cast<float*>(p.C);
   float* P = static_cast<float*>(p.pre_act);
   const float* bias = static_cast<const float*>(p.bias);
   const int col_in = lane & 31, half = lane >> 5;
@@ -176,13 +198,17 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_f32_kernel(GemmArgs p, int t
   for (int j = 0; j < 2; ++j) {
     const long long col = n0 + wn + 32 * j + col_in;
     if (col >= p.N) continue;
-    const float bv = bias ? bias[col] : 0.f;
+    const float bv = !SPREAD && bias ? bias[col] : 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const long long row = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * half;
         if (row >= p.M) continue;
+        if (SPREAD) {
+          C[row * p.N + col] = acc[i][j][e];
+          continue;
+        }
         float v = p.alpha * acc[i][j][e] + bv;
         if (p.beta != 0.f) v += p.beta * C[row * p.ldc + col];
         if (P) P[row * p.ldc + col] = v;
@@ -190,6 +216,17 @@ __global__ __launch_bounds__(kThreads, 2) void gemm_f32_kernel(GemmArgs p, int t
       }
     }
   }
+}
+
+// Adds the shares of a spread product up in order, and the bias.
+__global__ __launch_bounds__(256) void spread_reduce_f32_kernel(GemmArgs p) {
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, plane = p.M * p.N;
+  if (i >= plane) return;
+  const long long row = i / p.N, col = i - row * p.N;
+  float v = p.workspace[i];
+#pragma unroll 4
+  for (int s = 1; s < p.split_k; ++s) v += p.workspace[i + s * plane];
+  static_cast<float*>(p.C)[row * p.ldc + col] = v + (p.bias ? static_cast<const float*>(p.bias)[col] : 0.f);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -229,6 +266,35 @@ void launch_gemm_f32(const GemmArgs& a, hipStream_t stream) {
   else if (a.a_kmajor && !a.b_kmajor) go(std::true_type{}, std::false_type{});
   else if (!a.a_kmajor && a.b_kmajor) go(std::false_type{}, std::true_type{});
   else go(std::false_type{}, std::false_type{});
+}
+
+// Shares of the contraction for a product with few tiles (see gemm_spread): a k-step is 1.7 us of matrix work here, one workgroup a compute unit keeps
+// it busy, and at least 8 steps have to be saved (464 x 2112 x 685: 67 -> 34 us, 64 x 2048 x 768: 68 -> 17, 512^3: 50 -> 19, 1024 x 768 x 384, 9
+// saved: 42 -> 23).
+int gemm_f32_spread(const GemmArgs& a, int compute_units) {
+  const long long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN), nk = (a.K + BK - 1) / BK;
+  if (2 * tiles > compute_units || nk < 12) return 1;
+  long long s = compute_units / tiles;
+  if (s > nk / 4) s = nk / 4;
+  const long long plane = a.M * a.N * 4;
+  if (s > (64ll << 20) / plane) s = (64ll << 20) / plane;
+  return s < 2 || nk - nk / s < 8 ? 1 : static_cast<int>(s);
+}
+
+void launch_gemm_f32_spread(const GemmArgs& a, hipStream_t stream) {
+  const int tiles_m = static_cast<int>((a.M + BM - 1) / BM), tiles_n = static_cast<int>((a.N + BN - 1) / BN);
+  const dim3 grid(static_cast<unsigned>(tiles_m) * static_cast<unsigned>(tiles_n), static_cast<unsigned>(a.split_k));
+  const size_t lds = 4 * kTileFloats * sizeof(float);
+  const bool vec = vector_aligned(a);
+  auto go = [&](auto ak, auto bk) {
+    constexpr bool AK = decltype(ak)::value, BKM = decltype(bk)::value;
+    if (vec) hipLaunchKernelGGL((gemm_f32_kernel<AK, BKM, true, true>), grid, dim3(kThreads), lds, stream, a, tiles_m, tiles_n);
+    else hipLaunchKernelGGL((gemm_f32_kernel<AK, BKM, false, true>), grid, dim3(kThreads), lds, stream, a, tiles_m, tiles_n);
+  };
+  if (a.a_kmajor && a.b_kmajor) go(std::true_type{}, std::true_type{});
+  else if (a.a_kmajor) go(std::true_type{}, std::false_type{});
+  else go(std::false_type{}, std::false_type{});  // (the three layouts of a linear layer)
+  hipLaunchKernelGGL(spread_reduce_f32_kernel, dim3(static_cast<unsigned>((a.M * a.N + 255) / 256)), dim3(256), 0, stream, a);
 }
 
 }  // namespace kernels

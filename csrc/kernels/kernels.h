@@ -211,6 +211,9 @@ void launch_gemm_f16(const GemmArgs& a, hipStream_t stream);
 // into gemm_spread() shares (a.split_k, a.workspace of split_k * M * (N rounded up to 4) floats) on the 128x128 kernel.
 int gemm_spread(const GemmArgs& a);
 void launch_gemm_spread(const GemmArgs& a, int dtype, hipStream_t stream);
+// The same in float32 (workspace of split_k * M * N floats).
+int gemm_f32_spread(const GemmArgs& a, int compute_units);
+void launch_gemm_f32_spread(const GemmArgs& a, hipStream_t stream);
 // At most kFewRows rows of A (bf16 / fp16, NT layout, plain with bias or gate 1): a kernel bound by reading B once.
 constexpr int kFewRows = 64;
 bool few_rows_supported(const GemmArgs& a, int dtype);

@@ -544,6 +544,17 @@ Tensor tile_counters_for(kernels::GemmArgs& a, const Tensor& like) {
   return t;
 }
 
+int compute_units_of(const Tensor& t) {
+  static std::atomic<int> known[64];
+  const int d = t.get_device();
+  int n = d < 64 ? known[d].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    TORCH_CHECK(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d) == hipSuccess && n > 0, "cannot read the device's compute units");
+    if (d < 64) known[d].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 // `like` supplies the device for the split-K workspace (fp32 partials, caching allocator).  spread: products of few rows take the kernel made
 // for them and products of few output tiles cut their contraction over the chip (another order of summation than without).
 void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& like, bool spread = false) {
@@ -566,7 +577,15 @@ void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& l
     }
   }
   if (dt == kernels::kF32) {
-    kernels::launch_gemm_f32(a, s);
+    kernels::GemmArgs b = a;
+    b.split_k = spread ? kernels::gemm_f32_spread(a, compute_units_of(like)) : 1;
+    if (b.split_k > 1) {
+      Tensor ws = at::empty({b.split_k * a.M * a.N}, like.options());
+      b.workspace = ws.data_ptr<float>();
+      kernels::launch_gemm_f32_spread(b, s);
+    } else {
+      kernels::launch_gemm_f32(a, s);
+    }
     return;
   }
   if (dt == kernels::kF16) {
@@ -663,7 +682,7 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_forward(Tensor x, Tensor w, c10:
   DevGuard guard(x);
   hipStream_t s = stream_of(x);
   if (dt == kernels::kF32) {
-    Tensor gu = std::get<0>(linear_forward(x, w, bias, kernels::kActNone, false, false));
+    Tensor gu = std::get<0>(linear_forward(x, w, bias, kernels::kActNone, false, true));
     Tensor h = at::empty({M, H}, x.options());
     kernels::launch_gate_fwd(gu.data_ptr(), h.data_ptr(), M, H, dt, static_cast<int>(act), s);
     return {h, save ? c10::optional<Tensor>(gu) : c10::nullopt};
@@ -747,7 +766,7 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_backward(Tensor dy, Tensor w, Te
     a.C = dh.data_ptr();
     a.ldc = H;
     TORCH_CHECK(gemm_path_ok(a, dt), "gated_backward: shape M=", M, " N=", N, " H=", H, " is not supported");
-    run_gemm(a, dt, s, dy);
+    run_gemm(a, dt, s, dy, true);
     kernels::launch_gate_bwd(dh.data_ptr(), gu.data_ptr(), dgu.data_ptr(), M, H, dt, static_cast<int>(act), s);
   } else {
     a.C = dgu.data_ptr();
@@ -1217,17 +1236,6 @@ std::tuple<Tensor, Tensor> attention_backward(Tensor d_o, Tensor qkv, Tensor o, 
 }
 
 // ------------------------------------------------------------------ attention with a sliding window and sinks
-int compute_units_of(const Tensor& t) {
-  static std::atomic<int> known[64];
-  const int d = t.get_device();
-  int n = d < 64 ? known[d].load(std::memory_order_relaxed) : 0;
-  if (n == 0) {
-    TORCH_CHECK(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d) == hipSuccess && n > 0, "cannot read the device's compute units");
-    if (d < 64) known[d].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 kernels::WindowAttnArgs window_args(const Tensor& qkv, int64_t n_head, int64_t n_kv_head, int64_t window, int64_t sinks, double scale,
                                     const c10::optional<Tensor>& lens, const char* who) {
   TORCH_CHECK(qkv.defined() && qkv.is_cuda() && qkv.dim() == 3, who, ": qkv must be a GPU tensor [B, T, (H + 2 KV) * D]");

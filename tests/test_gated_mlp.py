@@ -312,3 +312,23 @@ def test_bias_gradients_of_few_and_many_rows(M, N, dtype):
     bound = M * 2.0 ** -24 * g.double().abs().sum(0) + torch.finfo(dtype).eps / 2 * want.abs() + 1e-12
     assert db[N - 1] == float("inf")
     assert bool(((db.double() - want).abs() <= bound)[: N - 1].all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", [(200, 130, 1400), (129, 33, 1999), (5, 1000, 1283), (1031, 37, 40), (1400, 640, 520), (300, 300, 4096)])
+def test_products_whose_contraction_is_spread(M, N, K, dtype):
+    from distributed_pytorch_amd import _ext
+
+    C = _ext.C()
+    x, w, b = torch.randn(M, K, device=DEV).to(dtype), torch.randn(N, K, device=DEV).to(dtype), torch.randn(N, device=DEV).to(dtype)
+    g = torch.randn(M, N, device=DEV).to(dtype)
+    y = C.linear_forward(x, w, b, 0, False, True)[0]
+    dx, dw, db = C.linear_backward(g, x, w, True, True, None, True)
+    X, W, G = x.double(), w.double(), g.double()
+    half = torch.finfo(dtype).eps / 2
+    for got, want, size, n in ((y, X @ W.t() + b.double(), X.abs() @ W.abs().t() + b.double().abs(), K), (dx, G @ W, G.abs() @ W.abs(), N),
+                               (dw, G.t() @ X, G.abs().t() @ X.abs(), M), (db, G.sum(0), G.abs().sum(0), M)):
+        # n float32 products and additions, each off by 2^-24 of the sum of sizes at most; then one rounding to the type
+        bound = 2 * (n + 2) * 2.0 ** -24 * size + half * want.abs() + 1e-12
+        assert bool(((got.double() - want).abs() <= bound).all())
