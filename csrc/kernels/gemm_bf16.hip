@@ -6,8 +6,8 @@
 //   * 128x128 output tile per 256-thread workgroup, 4 waves as 2x2, each wave 64x64 =
 //     4x4 tiles of v_mfma_f32_16x16x32_bf16 (64 accumulator registers);
 //   * K is consumed 64 at a time through double-buffered LDS (2 x 32 KiB); the global loads
-//     of step k+1 are in flight during the MFMAs of step k and land in the other buffer
-//     after them, one barrier per step;
+//     of steps k+1 and k+2 are in flight during the MFMAs of step k, in two sets of registers,
+//     and those of k+1 land in the other buffer after them, one barrier per step;
 //   * an operand with the contraction index contiguous in memory is kept as [row][64 k]
 //     (128-byte rows, 16-byte chunks XOR-swizzled by (row>>1)&7): one ds_read_b128 is one
 //     whole MFMA fragment (8 consecutive k of one row);
