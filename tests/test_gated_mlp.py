@@ -332,3 +332,40 @@ def test_products_whose_contraction_is_spread(M, N, K, dtype):
         # n float32 products and additions, each off by 2^-24 of the sum of sizes at most; then one rounding to the type
         bound = 2 * (n + 2) * 2.0 ** -24 * size + half * want.abs() + 1e-12
         assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,K,H,N", [(1003, 520, 1386, 520), (64, 1472, 640, 200), (2300, 256, 256, 128)])
+def test_spread_products_captured_and_replayed(M, K, H, N, dtype):
+    t, dy = make(M, K, H, N, dtype)
+    leaf = {k: v.clone().requires_grad_() for k, v in t.items()}
+
+    def step():
+        y = gated_mlp(leaf["x"], leaf["w_fc"], leaf["b_fc"], leaf["w_proj"], leaf["b_proj"])
+        with torch.no_grad():
+            quiet = gated_mlp(leaf["x"], leaf["w_fc"], leaf["b_fc"], leaf["w_proj"], leaf["b_proj"])
+        return [y.detach(), quiet, *torch.autograd.grad(y, list(leaf.values()), dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):  # two graphs, replayed in turn
+        graphs.append((torch.cuda.CUDAGraph(), None))
+        with torch.cuda.graph(graphs[-1][0]):
+            out = step()
+        graphs[-1] = (graphs[-1][0], out)
+    for k in range(4):
+        with torch.no_grad():
+            leaf["x"].copy_(t["x"] * (1 + 0.1 * k))
+        want = step()
+        assert torch.equal(want[0], want[1])
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            for got, w in zip(out, want):
+                assert torch.equal(got, w)
