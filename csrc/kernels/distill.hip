@@ -18,8 +18,8 @@
 // branch) and a chained hash from vector to entries.  Entries of one class are summed beforehand in index order by the
 // first of them, which makes the result independent of the order in which the chains were built.
 // Bound by memory with one temperature: 8192 x 50304 bf16, 32 entries, forward and gradient in 340 us (4.85 TB/s, the rate of a copy); 2049 x 50257
-// fp32 with a second exponential 203 us (4.1 TB/s).  With both temperatures and powers 24576 x 50304 bf16 in place take 1.27 ms (3.9 TB/s):
-// by count 19 issue slots an element, 8 of them its two exponentials, which the two rows that fit a compute unit do not hide entirely.
+// fp32 with a second exponential 203 us (4.1 TB/s).  With both temperatures and powers 24576 x 50304 float32 logits and their
+// bf16 gradient take 2.23 ms (3.3 TB/s): a row of 200 KB fills most of a compute unit's registers, so that one is fetched, computed and stored at a time.
 // Everything is fp32 but the logits and their gradient; in fp16 the gradient is only ever rounded with the upstream gradient in it.
 // Rows need no alignment: element j of a row sits in vector (j + shift) / V of the 16-byte grid, the vectors at both ends are stored
 // element by element.
@@ -56,10 +56,12 @@ __device__ __forceinline__ float teacher_at(const DistillArgs& a, long long i) {
 
 // THREADS x KEEP 16-byte vectors are held in registers (KEEP = 0: none, every pass reads memory).  SECOND: how the exponentials at
 // temperature 1 come about when both temperatures are needed -- 0: they are not, 1: by an exponential of their own, 2 / 4: as the square /
-// fourth power of those at temperature 2 / 4.
-template <typename TR, int THREADS, int KEEP, int MODE, int SECOND, int WAVES_PER_SIMD>
+// fourth power of those at temperature 2 / 4.  TO: type of the gradient, TR's own or, of float32 logits on rows that start on 16-byte boundaries, a
+// 16-bit one.
+template <typename TR, typename TO, int THREADS, int KEEP, int MODE, int SECOND, int WAVES_PER_SIMD>
 __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(DistillArgs a) {
   using T = typename TR::T;
+  using O = typename TO::T;
   constexpr int V = TR::kVec, NW = THREADS / 64;
   constexpr bool GRAD = MODE != kForward;
   static_assert(KEEP == 0 || MODE != kBackward, "the backward reads every vector once");
@@ -76,24 +78,31 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
 
   const long long r = a.row0 + blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int C = static_cast<int>(a.C), ld = static_cast<int>(a.ld);
+  const int C = static_cast<int>(a.C), ld = static_cast<int>(a.out_ld);
   const T* row = static_cast<const T*>(a.logits) + r * a.ld;
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const char* grid_in = reinterpret_cast<const char*>(row) - shift * sizeof(T);                       // the row's first 16-byte vector
-  char* grid_out = GRAD ? reinterpret_cast<char*>(static_cast<T*>(a.dlogits) + r * a.ld - shift) : nullptr;  // same alignment (checked by the host)
+  char* grid_out = GRAD ? reinterpret_cast<char*>(static_cast<O*>(a.dlogits) + r * a.out_ld - shift) : nullptr;  // (its alignment: checked by the host)
   const int nvec = (shift + C + V - 1) / V, nvec_ld = (shift + ld + V - 1) / V;
   const long long target = a.targets ? a.targets[r] : -1;
   const bool ignored = a.targets && (target == a.ignore_index || target < 0 || target >= C);
 
   auto store_vec = [&](int k, const float (&d)[V]) __attribute__((always_inline)) {
     const int j0 = k * V - shift;
-    T* out = reinterpret_cast<T*>(grid_out + 16u * static_cast<unsigned>(k));
+    O* out = reinterpret_cast<O*>(grid_out + static_cast<unsigned>(V * sizeof(O)) * static_cast<unsigned>(k));
     if (j0 >= 0 && j0 + V <= ld) {
-      store_from_f32<TR, V, true>(out, d);
+      if constexpr (V == TO::kVec) {
+        store_from_f32<TO, V, true>(out, d);
+      } else {
+        u16x4 v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = TO::from_f32(d[j]);
+        __builtin_nontemporal_store(v, reinterpret_cast<u16x4_any*>(out));
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (j0 + j >= 0 && j0 + j < ld) out[j] = TR::from_f32(d[j]);
+        if (j0 + j >= 0 && j0 + j < ld) out[j] = TO::from_f32(d[j]);
     }
   };
   if (ignored) {
@@ -435,20 +444,26 @@ __global__ __launch_bounds__(256) void distill_apply_upstream_kernel(typename TR
 
 }  // namespace
 
+bool distill_types_supported(int dtype, int out_dtype, int mode) {
+  return dtype == out_dtype || mode == kForward || (dtype == kF32 && (out_dtype == kBF16 ? mode == kFused : mode == kBackward));
+}
+
 bool distill_supported(long long C, long long ld, long long K) {
   return C >= 1 && C <= ld && ld <= kDistillMaxWidth && K >= 1 && K <= kDistillMaxEntries;
 }
 
-void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t stream) {
+void launch_distill(const DistillArgs& args, int dtype, int out_dtype, int mode, hipStream_t stream) {
   if (args.N <= 0) return;
   DistillArgs a = args;
+  if (mode == kForward || dtype == out_dtype) a.out_ld = a.ld;
   const bool dual = a.tau != 1.f && a.soft_weight != 0.f && a.hard_weight != 0.f;
   // one exponential: at the temperature of the term that is there (tau = 1: of both)
   a.exp_scale = (a.soft_weight != 0.f ? a.inv_tau : 1.f) * kLog2e;
   a.hash = 64;
   while (a.hash <= a.K) a.hash *= 2;
-  dispatch_dtype(dtype, [&](auto tr) {
+  auto typed = [&](auto tr, auto to) {
     using TR = decltype(tr);
+    using TO = decltype(to);
     constexpr int V = TR::kVec;
     const long long nvec = (a.ld + 2 * V - 2) / V;  // worst alignment
     a.words = static_cast<int>((nvec + 63) / 64);
@@ -457,10 +472,10 @@ void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t st
       constexpr int THREADS = decltype(threads_c)::value, KEEP = decltype(keep_c)::value, MODE = decltype(mode_c)::value;
       constexpr int WAVES = decltype(waves_c)::value;
       const dim3 grid(static_cast<unsigned>(args.N - a.row0 < kRowsPerLaunch ? args.N - a.row0 : kRowsPerLaunch));
-      if (!dual) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 0, WAVES>), grid, dim3(THREADS), lds, stream, a);
-      else if (a.tau == 2.f) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 2, WAVES>), grid, dim3(THREADS), lds, stream, a);
-      else if (a.tau == 4.f) hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 4, WAVES>), grid, dim3(THREADS), lds, stream, a);
-      else hipLaunchKernelGGL((distill_kernel<TR, THREADS, KEEP, MODE, 1, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      if (!dual) hipLaunchKernelGGL((distill_kernel<TR, TO, THREADS, KEEP, MODE, 0, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else if (a.tau == 2.f) hipLaunchKernelGGL((distill_kernel<TR, TO, THREADS, KEEP, MODE, 2, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else if (a.tau == 4.f) hipLaunchKernelGGL((distill_kernel<TR, TO, THREADS, KEEP, MODE, 4, WAVES>), grid, dim3(THREADS), lds, stream, a);
+      else hipLaunchKernelGGL((distill_kernel<TR, TO, THREADS, KEEP, MODE, 1, WAVES>), grid, dim3(THREADS), lds, stream, a);
     };
     static_assert(((4 * (kDistillMaxEntries + 1) + 2 * kDistillMaxEntries + 2 * ((kDistillMaxWidth / 4 + 64) / 64)) * 4) <= 60 * 1024,
                   "a workgroup's tables fit the 64 KiB that a launch may have without asking");
@@ -487,12 +502,22 @@ void launch_distill(const DistillArgs& args, int dtype, int mode, hipStream_t st
       }
     };
     for (a.row0 = 0; a.row0 < args.N; a.row0 += kRowsPerLaunch) {
-      if (mode == kForward) by_size(integral_constant<int, kForward>{});
-      else if (mode == kBackward) by_size(integral_constant<int, kBackward>{});
-      else by_size(integral_constant<int, kFused>{});
+      if constexpr (std::is_same<TR, TO>::value) {
+        if (mode == kForward) by_size(integral_constant<int, kForward>{});
+        else if (mode == kBackward) by_size(integral_constant<int, kBackward>{});
+        else by_size(integral_constant<int, kFused>{});
+      } else if constexpr (std::is_same<TO, BF16>::value) {
+        by_size(integral_constant<int, kFused>{});  // (bf16 gradients of float32 logits are only asked for with the loss, ...
+      } else {
+        by_size(integral_constant<int, kBackward>{});  // ... fp16 ones only with the upstream gradient)
+      }
     }
-  });
+  };
+  if (mode == kForward || dtype == out_dtype) dispatch_dtype(dtype, [&](auto tr) { typed(tr, tr); });
+  else if (out_dtype == kBF16) typed(F32{}, BF16{});
+  else typed(F32{}, F16{});
 }
+
 
 void launch_distill_scale(const long long* targets, long long N, long long ignore_index, int mean, float* scale, hipStream_t stream) {
   hipLaunchKernelGGL(distill_scale_kernel, dim3(1), dim3(1024), 0, stream, targets, N, ignore_index, mean, scale);

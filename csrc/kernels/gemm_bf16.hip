@@ -287,7 +287,7 @@ __device__ __forceinline__ bf16x8 read_frag(const char* lds, int tile_row0, int 
 
 // TR = BF16 or F16: the two 16-bit types share everything but the MFMA opcode and the epilogue's conversions.
 // GATE / GACT: GemmArgs::gate with its activation.  SPREAD: blockIdx.y takes its share of the contraction (p.split_k shares) and leaves raw
-// fp32 sums in p.workspace[share][M][N rounded up to 4] for spread_reduce_kernel.
+// fp32 sums in p.workspace[share][M][N rounded up to 4] for spread_reduce_kernel (the one share of launch_gemm_to_f32 is the result).
 template <bool A_KMAJOR, bool B_KMAJOR, bool ALIGNED, typename TR, int GATE = 0, int GACT = kActNone, bool SPREAD = false>
 __global__ __launch_bounds__(kThreads, 2) void gemm_bf16_kernel(GemmArgs p, int tiles_m, int tiles_n) {
   static_assert(!SPREAD || GATE == 0, "plain products only");
@@ -733,12 +733,14 @@ constexpr int kStreamingMaxKSteps = 64;  // beyond K = 4096 a tile is long enoug
 // not carry its code and registers (as a run-time branch it cost the NT forward kernel 8 spilled registers).
 // GATE / GACT: GemmArgs::gate with its activation (1: interleaved B rows and a product epilogue, streaming like the plain kernel; 2: an
 // epilogue like the activation-backward one, with two tensors in and two out).
-template <bool A_KMAJOR, bool B_KMAJOR, bool SPLIT, int CONV = 0, bool ACTBWD = false, int GATE = 0, int GACT = kActNone>
+// OUT32: C is float32 (launch_gemm_to_f32).
+template <bool A_KMAJOR, bool B_KMAJOR, bool SPLIT, int CONV = 0, bool ACTBWD = false, int GATE = 0, int GACT = kActNone, bool OUT32 = false>
 __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p, int tiles_m, int tiles_n, int k_iters, unsigned* tile_counter) {
   static_assert(CONV == 0 || (CONV == 1 && A_KMAJOR && B_KMAJOR && !SPLIT) || (CONV == 2 && !A_KMAJOR && !B_KMAJOR && SPLIT),
                 "convolution views exist for the NT forward product and the split-K TN weight gradient");
   static_assert(!ACTBWD || (!SPLIT && CONV == 0), "the activation-backward epilogue belongs to the plain single-pass product");
   static_assert(GATE == 0 || (!SPLIT && CONV == 0 && !ACTBWD && A_KMAJOR && B_KMAJOR == (GATE == 1)), "gated pairs: NT forward, NN backward");
+  static_assert(!OUT32 || (!SPLIT && CONV == 0 && !ACTBWD && GATE == 0 && A_KMAJOR && B_KMAJOR), "float32 results: the plain NT product");
   extern __shared__ __attribute__((aligned(16))) char smem2[];  // [2 k-steps][B0 | A0 | B1 | A1][GELU table][staging][control]
   DPA_STAMP(0);
   DPA_STAMP_REAL(4);
@@ -1105,7 +1107,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
     // Full interior tiles of a plain product leave through the LDS-staged epilogue below (with the bias
     // already in the accumulators); everything else through the element-wise one.
     if (GATE == 2) whole_tile = m0 + BM2 <= p.M && n0 + BN2 <= p.N;
-    const bool staged = !SPLIT && p.beta == 0.f && p.alpha == 1.f && m0 + BM2 <= p.M && n0 + BN2 <= p.N && (p.ldc & 7) == 0 &&
+    const bool staged = !SPLIT && p.beta == 0.f && p.alpha == 1.f && m0 + BM2 <= p.M && n0 + BN2 <= p.N && (p.ldc & (OUT32 ? 3 : 7)) == 0 &&
                         ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(p.pre_act)) & 15) == 0;
     if (staged && p.bias != nullptr) {
       using lds_u16x4_cptr = const __attribute__((address_space(3))) u16x4*;
@@ -1278,7 +1280,52 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       }
       return;
     }
-    if constexpr (GATE == 1) {
+    if constexpr (OUT32) {
+      // The same strips, 16 rows x 32 columns a pass.  (24576 x 50304 x 768: 1.90 ms, 4.9 GB written; with a bf16 result 1.75 ms.)
+      if (!staged) {
+        ahead_stores = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const long long row = m0 + wm + 16 * i + (lane & 15), col = n0 + wn + 16 * j + 4 * (lane >> 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (row < p.M && col + e < p.N) static_cast<float*>(p.C)[row * p.ldc + col + e] = acc[i][j][e];
+          }
+      } else {
+        using lds_f32x4_ptr = __attribute__((address_space(3))) f32x4*;
+        using lds_f32x4_cptr = const __attribute__((address_space(3))) f32x4*;
+        const int l = fresh_lane();
+        const int r = l & 15, g = l >> 4;
+        const unsigned mine = lds_base + kStageOff + wid * 2048;
+        const unsigned wr_addr = mine + r * 128;
+        const unsigned rd_addr = mine + (l >> 3) * 128 + (l & 7) * 16;
+        float* const out = static_cast<float*>(p.C) + (m0 + wm + (l >> 3)) * p.ldc + n0 + wn + ((l & 7) ^ (l >> 3)) * 4;
+        auto write = [&](int q) __attribute__((always_inline)) {  // columns 32 (q & 1) .. of rows 16 (q >> 1) ..
+#pragma unroll
+          for (int jj = 0; jj < 2; ++jj) *(lds_f32x4_ptr)(wr_addr + (((4 * jj + g) ^ (r & 7)) << 4)) = acc[q >> 1][2 * (q & 1) + jj];
+        };
+        auto read_rows = [&](f32x4 (&v)[2]) __attribute__((always_inline)) {
+#pragma unroll
+          for (int it = 0; it < 2; ++it) v[it] = *(lds_f32x4_cptr)(rd_addr + it * 1024);
+        };
+        f32x4 v[2][2];
+        write(0);
+        read_rows(v[0]);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          if (q + 1 < 16) {
+            write(q + 1);
+            read_rows(v[(q + 1) & 1]);
+          }
+#pragma unroll
+          for (int it = 0; it < 2; ++it)
+            __builtin_nontemporal_store(v[q & 1][it], reinterpret_cast<f32x4*>(out + static_cast<long long>(16 * (q >> 1) + 8 * it) * p.ldc + 32 * (q & 1)));
+        }
+        ahead_stores = 32;
+      }
+    } else if constexpr (GATE == 1) {
       if (!staged) {
         ahead_stores = 0;
 #pragma unroll
@@ -1484,7 +1531,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       DPA_TILE_TIME(1);
       return;
     }
-    if (GATE == 0 && staged) {
+    if (GATE == 0 && !OUT32 && staged) {
       using lds_u16x4_ptr = __attribute__((address_space(3))) u16x4*;
       using lds_u32x4_ptr = const __attribute__((address_space(3))) u32x4*;
       const int l = fresh_lane();  // the epilogue's lane constants are derived here, not kept from the top of the kernel
@@ -1584,7 +1631,7 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
       else if (p.act == kActRelu) emit_all(std::integral_constant<int, kActRelu>{});
       else emit_all(std::integral_constant<int, kActNone>{});
       ahead_stores = p.pre_act ? 32 : 16;
-    } else if (GATE == 0) {
+    } else if (GATE == 0 && !OUT32) {
       ahead_stores = 0;  // ragged tile: an unknown number of stores, the next wait covers them all
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -1932,6 +1979,42 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream) {
   else if (a.a_kmajor && !a.b_kmajor) go(std::true_type{}, std::false_type{});
   else if (!a.a_kmajor && a.b_kmajor) go(std::false_type{}, std::true_type{});
   else go(std::false_type{}, std::false_type{});
+}
+
+bool gemm_to_f32_supported(const GemmArgs& a, int dtype) {
+  return (dtype == kBF16 || dtype == kF16) && a.a_kmajor && a.b_kmajor && gemm_bf16_supported(a) && a.ldc == ((a.N + 3) & ~3ll) && aligned16(a.C) &&
+         a.bias == nullptr && a.pre_act == nullptr && a.act == kActNone && a.beta == 0.f && a.alpha == 1.f;
+}
+
+void launch_gemm_to_f32(const GemmArgs& args, int dtype, hipStream_t stream) {
+  GemmArgs a = args;
+  if (dtype == kBF16 && use_large_tile(a)) {
+    const int tm = static_cast<int>((a.M + BM2 - 1) / BM2), tn = static_cast<int>((a.N + BN2 - 1) / BN2);
+    const long long tiles = static_cast<long long>(tm) * tn;
+    unsigned* counter = nullptr;
+    unsigned grid = static_cast<unsigned>(tiles);
+    if (a.tile_counters != nullptr && use_streaming(a, tiles, false)) {
+      counter = a.tile_counters;
+      hipLaunchKernelGGL(clear_tile_counters_kernel, dim3(1), dim3(64), 0, stream, counter);
+      grid = static_cast<unsigned>(compute_units()) & ~7u;
+    }
+    auto kernel = gemm_bf16_8ph_kernel<true, true, false, 0, false, 0, kActNone, true>;
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes2);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads2), kLdsBytes2, stream, a, tm, tn, static_cast<int>(a.K / BK2), counter);
+    return;
+  }
+  const int tiles_m = static_cast<int>((a.M + BM - 1) / BM), tiles_n = static_cast<int>((a.N + BN - 1) / BN);
+  const dim3 grid(static_cast<unsigned>(tiles_m) * static_cast<unsigned>(tiles_n));
+  const bool vec = gemm_bf16_vector_aligned(a);
+  a.workspace = static_cast<float*>(a.C);
+  a.split_k = 1;
+  auto typed = [&](auto tr) {
+    using TR = decltype(tr);
+    if (vec) hipLaunchKernelGGL((gemm_bf16_kernel<true, true, true, TR, 0, kActNone, true>), grid, dim3(kThreads), 4 * kTileBytes, stream, a, tiles_m, tiles_n);
+    else hipLaunchKernelGGL((gemm_bf16_kernel<true, true, false, TR, 0, kActNone, true>), grid, dim3(kThreads), 4 * kTileBytes, stream, a, tiles_m, tiles_n);
+  };
+  if (dtype == kF16) typed(F16{});
+  else typed(BF16{});
 }
 
 // Shares of the contraction that let a product with few 128x128 tiles fill the chip: two workgroups per compute unit, at least four k-steps a

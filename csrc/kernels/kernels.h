@@ -100,7 +100,8 @@ void launch_xent_fused(void* logits, int dtype, const long long* targets, long l
 // mode 0: row losses, correct flags, row_stats[3 r ..] = {max z, sum of exponentials, sum at temperature 1 where both are needed}
 // mode 1: dlogits from row_stats, scaled by scale[0] * grad_out[grad_out_rows ? r : 0]
 // mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits
-// dlogits [N, ld]: columns [C, ld) are written as zero; its address must equal that of logits modulo 16.
+// dlogits [N, out_ld]: columns [C, out_ld) are written as zero.  In the logits' type: out_ld is ld and the address equals that of logits modulo 16.
+// Float32 logits in rows of 16-byte vectors (ld a multiple of 4, an address of 16) may have a 16-bit gradient: bf16 in mode 2, fp16 in mode 1.
 constexpr int kDistillMaxEntries = 1024;
 constexpr long long kDistillCountRows = 512;
 constexpr long long kDistillMaxWidth = 1 << 20;  // of ld: one bit per 16 bytes of a row is kept in LDS
@@ -110,7 +111,7 @@ struct DistillArgs {
   const void* ids;
   const void* teacher;
   const long long* targets;
-  long long N, C, ld, ignore_index;
+  long long N, C, ld, out_ld, ignore_index;  // (out_ld: looked at where the gradient has another type)
   int K, ids_64, teacher_dtype;
   float tau, inv_tau, soft_weight, hard_weight;
   float* row_loss;
@@ -126,7 +127,8 @@ struct DistillArgs {
   long long row0;
 };
 bool distill_supported(long long C, long long ld, long long K);
-void launch_distill(const DistillArgs& a, int dtype, int mode, hipStream_t stream);
+bool distill_types_supported(int dtype, int out_dtype, int mode);
+void launch_distill(const DistillArgs& a, int dtype, int out_dtype, int mode, hipStream_t stream);
 // scale[0] = 1 / max(#targets != ignore_index, 1) for a mean (N rows without targets), 1 for a sum.
 void launch_distill_scale(const long long* targets, long long N, long long ignore_index, int mean, float* scale, hipStream_t stream);
 // metrics[0] = sum of row losses, [1] = correct rows, [2] = rows that count, [3] = mean; loss[0] = mean or sum.
@@ -207,6 +209,10 @@ void launch_gemm_bf16(const GemmArgs& a, hipStream_t stream);
 // fp16 storage (fp32 accumulate) on the 128x128 MFMA kernel; same argument conventions.
 bool gemm_f16_supported(const GemmArgs& a);
 void launch_gemm_f16(const GemmArgs& a, hipStream_t stream);
+// A product of 16-bit operands that is kept in float32: C [M, ldc] float32 with ldc = N rounded up to 4 and a 16-byte aligned base, NT layout, no bias /
+// act / pre_act / beta.  The columns behind N are left or hold anything.
+bool gemm_to_f32_supported(const GemmArgs& a, int dtype);
+void launch_gemm_to_f32(const GemmArgs& a, int dtype, hipStream_t stream);
 // Products with few output tiles (bf16 / fp16; the layouts NT, NN and TN of a linear layer; bias, no act / pre_act / beta): the contraction cut
 // into gemm_spread() shares (a.split_k, a.workspace of split_k * M * (N rounded up to 4) floats) on the 128x128 kernel.
 int gemm_spread(const GemmArgs& a);

@@ -360,14 +360,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> distill_forwa
     dlogits = gradient == "inplace" ? logits : at::empty_like(logits);
     a.dlogits = dlogits.data_ptr();
   }
-  kernels::launch_distill(a, kdtype(logits), gradient == "none" ? 0 : 2, s);
+  kernels::launch_distill(a, kdtype(logits), kdtype(logits), gradient == "none" ? 0 : 2, s);
   kernels::launch_distill_reduce(a.row_loss, a.correct, a.targets, a.N, ignore_index, mean ? 1 : 0, metrics.data_ptr<float>(), loss.data_ptr<float>(), s);
   return {loss, row_loss, correct, metrics, scale, stats, dlogits};
 }
 
-// dlogits from the statistics of a "none" forward.  grad_out: one value, or one per row.
+// dlogits from the statistics of a forward without them.  grad_out: one value, or one per row.  half_width: dlogits in fp16, so many columns of them
+// (of the float32 logits of projection_distill_forward, whose rows end in padding).
 Tensor distill_backward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets, Tensor row_stats, c10::optional<Tensor> scale,
-                        Tensor grad_out, int64_t n_classes, int64_t ignore_index, double temperature, double hard_weight, bool mean) {
+                        Tensor grad_out, int64_t n_classes, int64_t ignore_index, double temperature, double hard_weight, bool mean, int64_t half_width) {
   kernels::DistillArgs a = distill_args(logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, "distill_backward");
   check_gpu(row_stats, "row_stats");
   check_gpu(grad_out, "grad_out");
@@ -382,13 +383,16 @@ Tensor distill_backward(Tensor logits, Tensor ids, Tensor teacher, c10::optional
   }
   TORCH_CHECK(grad_out.scalar_type() == at::kFloat && (grad_out.dim() <= 1) && (grad_out.numel() == 1 || grad_out.numel() == a.N),
               "distill_backward: grad_out must be one float32 value or one per row");
+  TORCH_CHECK(half_width == 0 || (logits.scalar_type() == at::kFloat && a.ld % 4 == 0 && a.C <= half_width && half_width <= a.ld),
+              "distill_backward: an fp16 gradient needs float32 logits in rows of whole 16-byte vectors and ", a.C, " .. ", a.ld, " columns");
   DevGuard g(logits);
-  Tensor dlogits = at::empty_like(logits);
+  Tensor dlogits = half_width ? at::empty({a.N, half_width}, logits.options().dtype(at::kHalf)) : at::empty_like(logits);
   a.dlogits = dlogits.data_ptr();
+  a.out_ld = half_width;
   a.row_stats = row_stats.data_ptr<float>();
   a.grad_out = grad_out.data_ptr<float>();
   a.grad_out_rows = grad_out.dim() == 1 && grad_out.numel() == a.N ? 1 : 0;
-  kernels::launch_distill(a, kdtype(logits), 1, stream_of(logits));
+  kernels::launch_distill(a, kdtype(logits), kdtype(dlogits), 1, stream_of(logits));
   return dlogits;
 }
 
@@ -604,6 +608,77 @@ void run_gemm(const kernels::GemmArgs& a, int dt, hipStream_t s, const Tensor& l
   kernels::GemmArgs b = a;
   const Tensor counters = tile_counters_for(b, like);
   kernels::launch_gemm_bf16(b, s);
+}
+
+// The loss of the logits x W^T of bf16 or fp16 x [N, K] and W [V, K].  The logits are kept in float32, as a float32 loss wants them: rounded to 16
+// bits they move it by up to 1e-4 of its size, and turn over which of two close ones is the largest.  keep says what stays for a backward:
+//   "none"      nothing
+//   "gradient"  dlogits [N, V] in bf16 for a unit upstream gradient
+//   "logits"    the float32 logits [N, V rounded up to 4] and their row statistics, for distill_backward
+// Without the last, some rows at a time go through a buffer of at most workspace_bytes (or of 256 rows), so that the float32 logits never are
+// there all at once.  Returns (loss, correct, metrics, scale or undefined, row_stats or undefined, logits or undefined, dlogits or undefined).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> projection_distill_forward(Tensor x, Tensor w, Tensor ids, Tensor teacher,
+                                                                                              c10::optional<Tensor> targets, int64_t n_classes,
+                                                                                              int64_t ignore_index, double temperature,
+                                                                                              double hard_weight, bool mean, const std::string& keep,
+                                                                                              int64_t workspace_bytes) {
+  const char* who = "projection_distill_forward";
+  check_gpu(x, "x");
+  check_gpu(w, "weight");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.size(1) > 0, who, ": x [N, K] and weight [V, K] expected");
+  TORCH_CHECK(x.scalar_type() == w.scalar_type() && x.get_device() == w.get_device() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf),
+              who, ": x and weight must both be bf16 or both fp16, on one device");
+  TORCH_CHECK(keep == "none" || keep == "logits" || (keep == "gradient" && x.scalar_type() == at::kBFloat16), who,
+              ": keep must be none, logits or (in bf16) gradient");
+  const int64_t N = x.size(0), V = w.size(0), K = x.size(1), pitch = (V + 3) / 4 * 4;
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == N && teacher.sizes() == ids.sizes(), who, ": teacher_ids and teacher_logits must both be [N, K]");
+  const bool has_targets = targets.has_value() && targets->defined();
+  TORCH_CHECK(!has_targets || (targets->dim() == 1 && targets->size(0) == N), who, ": targets must be int64 [N]");
+  const int64_t C = n_classes > 0 ? n_classes : V;
+  TORCH_CHECK(C <= V, who, ": more classes than rows of the weight");
+  const int dt = kdtype(x);
+  DevGuard guard(x);
+  hipStream_t s = stream_of(x);
+  auto fopt = x.options().dtype(at::kFloat);
+  const bool whole = keep == "logits";
+  int64_t rows = whole ? N : std::min<int64_t>(N, std::max<int64_t>(workspace_bytes / (pitch * 4) / 256, 1) * 256);
+  rows = std::max<int64_t>(rows, 1);
+  Tensor loss = at::empty({}, fopt), row_loss = at::empty({N}, fopt), metrics = at::empty({4}, fopt), correct = at::empty({N}, x.options().dtype(at::kBool));
+  Tensor logits = at::empty({std::min(rows, N), pitch}, fopt), scale, stats, dlogits;
+  if (keep != "gradient") stats = at::empty({N, 3}, fopt);
+  if (keep == "gradient") dlogits = at::empty({N, V}, x.options());
+  // (checks of everything that is left, also where there are no rows)
+  (void)distill_args(logits.narrow(0, 0, 0), ids.narrow(0, 0, 0), teacher.narrow(0, 0, 0),
+                     has_targets ? c10::optional<Tensor>(targets->narrow(0, 0, 0)) : c10::nullopt, C, ignore_index, temperature, hard_weight, who);
+  const long long* const target = has_targets ? reinterpret_cast<const long long*>(targets->data_ptr<int64_t>()) : nullptr;
+  if (N > kernels::kDistillCountRows || rows < N) {
+    scale = at::empty({1}, fopt);
+    kernels::launch_distill_scale(target, N, ignore_index, mean ? 1 : 0, scale.data_ptr<float>(), s);
+  }
+  for (int64_t r0 = 0; r0 < N; r0 += rows) {
+    const int64_t n = std::min(rows, N - r0);
+    kernels::GemmArgs p{};
+    p.A = static_cast<const char*>(x.data_ptr()) + r0 * K * 2; p.B = w.data_ptr(); p.C = logits.data_ptr();
+    p.M = n; p.N = V; p.K = K; p.lda = K; p.ldb = K; p.ldc = pitch; p.a_kmajor = 1; p.b_kmajor = 1; p.alpha = 1.f;
+    TORCH_CHECK(kernels::gemm_to_f32_supported(p, dt), who, ": shape M=", n, " N=", V, " K=", K, " is not supported");
+    const Tensor counters = dt == kernels::kBF16 ? tile_counters_for(p, x) : Tensor();
+    kernels::launch_gemm_to_f32(p, dt, s);
+    const Tensor part = logits.narrow(0, 0, n);
+    kernels::DistillArgs a = distill_args(part, ids.narrow(0, r0, n), teacher.narrow(0, r0, n),
+                                          has_targets ? c10::optional<Tensor>(targets->narrow(0, r0, n)) : c10::nullopt, C, ignore_index, temperature,
+                                          hard_weight, who);
+    a.row_loss = row_loss.data_ptr<float>() + r0;
+    a.correct = reinterpret_cast<unsigned char*>(correct.data_ptr<bool>()) + r0;
+    a.mean = mean ? 1 : 0;
+    a.scale = scale.defined() ? scale.data_ptr<float>() : nullptr;
+    a.row_stats = stats.defined() ? stats.data_ptr<float>() + 3 * r0 : nullptr;
+    if (dlogits.defined()) a.dlogits = static_cast<char*>(dlogits.data_ptr()) + r0 * V * 2;
+    a.out_ld = V;
+    kernels::launch_distill(a, kernels::kF32, dlogits.defined() ? dt : kernels::kF32, dlogits.defined() ? 2 : 0, s);
+  }
+  kernels::launch_distill_reduce(row_loss.data_ptr<float>(), reinterpret_cast<unsigned char*>(correct.data_ptr<bool>()), target, N, ignore_index,
+                                 mean ? 1 : 0, metrics.data_ptr<float>(), loss.data_ptr<float>(), s);
+  return {loss, correct, metrics, scale, whole ? stats : Tensor(), whole ? logits : Tensor(), dlogits};
 }
 
 // Whether the MFMA GEMMs take C[M,N] = op(A) op(B)^T with contiguous operands in the given layouts.
@@ -1380,7 +1455,10 @@ void init_ops(py::module_& m) {
         py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"), py::arg("hard_weight"), py::arg("mean"), py::arg("gradient") = "none");
   m.def("distill_backward", &distill_backward, py::arg("logits"), py::arg("teacher_ids"), py::arg("teacher_logits"), py::arg("targets"),
         py::arg("row_stats"), py::arg("scale"), py::arg("grad_out"), py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"),
-        py::arg("hard_weight"), py::arg("mean") = true);
+        py::arg("hard_weight"), py::arg("mean") = true, py::arg("half_width") = 0);
+  m.def("projection_distill_forward", &projection_distill_forward, py::arg("x"), py::arg("weight"), py::arg("teacher_ids"), py::arg("teacher_logits"),
+        py::arg("targets"), py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"), py::arg("hard_weight"), py::arg("mean"), py::arg("keep"),
+        py::arg("workspace_bytes") = 8ll << 30);
   m.def("distill_apply_upstream", &distill_apply_upstream, py::arg("x"), py::arg("g"));
   m.attr("DISTILL_MAX_ENTRIES") = kernels::kDistillMaxEntries;
   m.def("dgrad_act_backward", &dgrad_act_backward, py::arg("dout"), py::arg("weight"), py::arg("aux"), py::arg("act"), py::arg("want_colsum"));

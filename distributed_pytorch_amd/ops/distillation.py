@@ -7,8 +7,8 @@ token is stored as its K largest logits with their classes; the student learns t
     loss_r = (1 - a) tau^2 sum_k p_k (log p_k - log q[id_k])  -  a log q1[target]        (a = hard_weight, tau = temperature)
 
 ``topk_distillation`` takes the student's logits, ``projection_topk_distillation`` the input and the weight of the
-vocabulary projection (the logits then exist only inside the op and become their own gradient in place, as in
-``projection_cross_entropy``).  On gfx950 the loss and the gradient of the logits come out of one kernel that reads each row
+vocabulary projection (the logits then exist only inside the op, in float32 whatever the tensors' type, so that the loss is as exact as that
+of float32 logits).  On gfx950 the loss and the gradient of the logits come out of one kernel that reads each row
 once.  An entry whose id is negative or not below ``n_classes``, or whose logit is ``-inf``, is absent; entries may come
 in any order, and entries of one class add up.  Rows whose target is ``ignore_index`` count for nothing and may hold
 anything; a row without entries keeps its hard term.
@@ -77,24 +77,29 @@ class _TopKDistillation(torch.autograd.Function):
 
 
 class _ProjectionTopKDistillation(torch.autograd.Function):
-    """Vocabulary projection and loss as one node: the logits are overwritten with their gradient by the kernel that
-    computes the loss, and the backward is two matrix products (see ``cross_entropy._ProjectionXent``).  In fp16 the logits stay and the
+    """Vocabulary projection and loss as one node, whose backward is two matrix products of the logits' gradient (see
+    ``cross_entropy._ProjectionXent``).  The logits are float32 whatever the tensors' type, as the loss is: in fp32 the kernel that computes the
+    loss overwrites them with their gradient, in bf16 it writes the gradient beside them and they go.  In fp16 they stay and the
     backward computes their gradient, for the reason given above."""
 
     @staticmethod
-    def forward(ctx, x2, weight, ids, teacher, targets, cfg, impl):
+    def forward(ctx, x2, weight, ids, teacher, targets, cfg, impl, grad):
         reduction, ignore_index, n_classes, temperature, hard_weight = cfg
         ctx.set_materialize_grads(False)
-        logits = gemm.nt(x2, weight, None, impl)
-        grad = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        inplace = grad and logits.dtype != torch.float16
-        loss, _, correct, metrics, scale, stats, _ = _ext.C().distill_forward(
-            logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, reduction == "mean", "inplace" if inplace else "none")
-        if inplace:
-            ctx.save_for_backward(x2, weight, logits)  # `logits` now holds d loss / d logits for a unit upstream gradient
-        elif grad:
+        C = _ext.C()
+        args = (ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, reduction == "mean")
+        half = x2.dtype == torch.float16
+        if impl == "native" and x2.dtype != torch.float32:
+            loss, correct, metrics, scale, stats, logits, dlogits = C.projection_distill_forward(
+                x2, weight, *args, "none" if not grad else "logits" if half else "gradient")
+        else:
+            logits = gemm.nt(x2, weight, None, impl)
+            loss, _, correct, metrics, scale, stats, dlogits = C.distill_forward(logits, *args, "inplace" if grad and not half else "none")
+        if grad and half:
             ctx.save_for_backward(x2, weight, logits, ids, teacher, targets, scale, stats)
-        ctx.impl, ctx.inplace, ctx.cfg = impl, inplace, cfg
+        elif grad:
+            ctx.save_for_backward(x2, weight, dlogits)  # for a unit upstream gradient
+        ctx.impl, ctx.half, ctx.cfg = impl, half, cfg
         ctx.mark_non_differentiable(correct, metrics)
         return loss, correct, metrics
 
@@ -102,25 +107,26 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss, _dcorrect, _dmetrics):
         if dloss is None:
-            return (None,) * 7
+            return (None,) * 8
         g = dloss.detach().to(torch.float32).reshape(())
         C = _ext.C()
-        if ctx.inplace:
-            x2, weight, dlogits = ctx.saved_tensors
-        else:
+        if ctx.half:
             x2, weight, logits, ids, teacher, targets, scale, stats = ctx.saved_tensors
             reduction, ignore_index, n_classes, temperature, hard_weight = ctx.cfg
-            dlogits = C.distill_backward(logits, ids, teacher, targets, stats, scale, g, n_classes, ignore_index, temperature, hard_weight, reduction == "mean")
+            dlogits = C.distill_backward(logits, ids, teacher, targets, stats, scale, g, n_classes, ignore_index, temperature, hard_weight,
+                                         reduction == "mean", weight.shape[0] if logits.dtype == torch.float32 else 0)
+        else:
+            x2, weight, dlogits = ctx.saved_tensors
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = gemm.nn(dlogits, weight, ctx.impl)
-            if ctx.inplace:
+            if not ctx.half:
                 C.distill_apply_upstream(dx, g)
         if ctx.needs_input_grad[1]:
             dw = gemm.weight_grad(dlogits, x2, weight, ctx.impl)
-            if ctx.inplace:
+            if not ctx.half:
                 C.distill_apply_upstream(dw, g)
-        return dx, dw, None, None, None, None, None
+        return dx, dw, None, None, None, None, None, None
 
 
 def _check(N: int, n_classes: int, width: int, ids, teacher, targets, temperature: float, hard_weight: float, reduction: str, allowed) -> None:
@@ -218,7 +224,12 @@ def projection_topk_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_
                                  reduction: str = "mean", ignore_index: int = -100, n_classes: Optional[int] = None, impl: str = "native",
                                  check_targets: Optional[bool] = None) -> DistillResult:
     """``topk_distillation`` of the logits ``x @ weight.T`` (``x``: [..., K_in], ``weight``: [C, K_in]; the teacher's tensors
-    are [..., K] and ``targets`` [...] over the same leading dimensions).  reduction: mean | sum."""
+    are [..., K] and ``targets`` [...] over the same leading dimensions).  reduction: mean | sum.
+
+    bf16 training keeps the logits' gradient (2 bytes each) until the backward, beside some rows of float32 logits in passing (8 GiB at
+    most); fp16 training keeps the float32 logits.  ``impl="library"`` takes the vendor's products, for comparisons: logits rounded to the tensors'
+    type, and the loss with them.
+    """
     x2 = x.reshape(-1, x.shape[-1])
     ids = teacher_ids.reshape(-1, teacher_ids.shape[-1])
     teacher = teacher_logits.reshape(-1, teacher_logits.shape[-1])
@@ -235,7 +246,8 @@ def projection_topk_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_
     teacher = teacher.detach()
     teacher = teacher if teacher.dtype in (torch.float32, torch.bfloat16, torch.float16) else teacher.float()
     loss, correct, metrics = _ProjectionTopKDistillation.apply(x2.contiguous(), weight.contiguous(), ids.contiguous(), teacher.contiguous(),
-                                                               None if t1 is None else t1.contiguous(), cfg, impl)
+                                                               None if t1 is None else t1.contiguous(), cfg, impl,
+                                                               torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad))
     return DistillResult(loss, correct, metrics)
 
 

@@ -520,3 +520,116 @@ def test_rows_are_counted_alike_by_few_and_many(N, dtype):
     assert n == N
     (g,) = torch.autograd.grad(r.loss, x)
     torch.testing.assert_close(g.double().cpu(), grad / n, rtol=torch.finfo(dtype).eps / 2 * 1.01, atol=near / n + (2.0 ** -25 if dtype == torch.float16 else 0))
+
+
+def projected(N, V, K_in, dtype, seed=0, K=11, C=None):
+    """Inputs of a vocabulary projection near its initialisation."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(N, K_in, generator=g).to(dtype).to(DEV)
+    w = (torch.randn(V, K_in, generator=g) * 0.02).to(dtype).to(DEV)
+    _, ids, teacher, targets = make(N, C or V, K, dtype, DEV, seed=seed, pad_rows=False)
+    return x, w, ids, teacher, targets
+
+
+# The loss is float32, so logits rounded to 16 bits (half a step of theirs is 2^-9 or 2^-12) are not good enough for it.  What float32 leaves, with
+# logits below 4 in size and sums of 768 products below 8: of a logit 96 roundings at most (a matrix instruction adds 8 products or more at once), half a step of
+# 2^-24 each, mostly of unlike sign, and some 30 more in exponents, sums of positive terms and logarithms: 2^-17 of a loss near 7 covers them, at any number of rows.
+@gpu
+@pytest.mark.parametrize("N", [1, 2, 4, 16, 64, 700])
+@pytest.mark.parametrize("V,K_in", [(1000, 768), (1003, 768), (5000, 250)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_projected_loss_is_as_exact_as_its_type(N, V, K_in, dtype):
+    for seed in range(3):
+        x, w, ids, teacher, targets = projected(N, V, K_in, dtype, seed)
+        z = x.double() @ w.double().t()
+        for tau, a in ((2.0, 0.5), (1.0, 0.0), (1.0, 1.0)):
+            rows, _, n = reference(z, ids, teacher, targets, tau, a)
+            for reduction, k in (("mean", n), ("sum", 1)):
+                r = projection_topk_distillation(x, w, ids, teacher, targets, tau, a, reduction)
+                assert abs(float(r.loss) - float(rows.sum()) / k) <= 2.0 ** -17 * max(1.0, tau ** 2) * n / k
+                assert abs(float(r.metrics[3]) - float(rows.sum()) / n) <= 2.0 ** -17 * max(1.0, tau ** 2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_projected_predictions_are_those_of_the_unrounded_logits(dtype):
+    x, w, ids, teacher, _ = projected(2048, 1000, 256, dtype)
+    z = x.double() @ w.double().t()
+    top = z.topk(2, 1)
+    clear = top.values[:, 0] - top.values[:, 1] > 1e-4
+    r = projection_topk_distillation(x, w, ids, teacher, top.indices[:, 0].contiguous(), 2.0, 0.5)
+    assert clear.float().mean() > 0.95 and bool(r.correct[clear].all())
+
+
+# both kernels of the float32 product: 128 x 128 tiles, 256 x 256 tiles one to a workgroup and several to a workgroup, with ragged edges
+@gpu
+@pytest.mark.parametrize("N,V,K_in", [(1, 17, 8), (130, 1003, 77), (2049, 4103, 64), (2048, 4096, 128), (4100, 12301, 192), (4096, 12544, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_projected_logits_and_parts_of_the_rows(N, V, K_in, dtype):
+    from distributed_pytorch_amd import _ext
+
+    x, w, ids, teacher, targets = projected(N, V, K_in, dtype, K=5)
+    targets[::7] = -100
+    args = (x, w, ids, teacher, targets, V, -100, 2.0, 0.5, True)
+    loss, correct, metrics, scale, stats, logits, _ = _ext.C().projection_distill_forward(*args, "logits")
+    assert logits.dtype == torch.float32 and logits.shape == (N, (V + 3) // 4 * 4)
+    z = x.float() @ w.float().t()  # (float64 does not fit the largest comfortably; the bound takes both sides' roundings)
+    bound = 2 * K_in * 2.0 ** -24 * (x.float().abs() @ w.float().abs().t()) + 1e-30
+    assert bool(((logits[:, :V] - z).abs() <= bound).all())
+    quiet = _ext.C().projection_distill_forward(*args, "none", workspace_bytes=1)  # 256 rows at a time
+    assert torch.equal(quiet[1], correct) and abs(float(quiet[0] - loss)) <= 2.0 ** -17
+    if dtype == torch.bfloat16:
+        d1 = _ext.C().projection_distill_forward(*args, "gradient")[6]
+        # the same arithmetic as the gradient of the float32 logits on their own, but rounded to bf16
+        whole = logits[:, :V].contiguous()
+        d2 = _ext.C().distill_forward(whole, ids, teacher, targets, V, -100, 2.0, 0.5, True, "new")[6]
+        if V % 4 == 0:
+            assert torch.equal(d1, d2.bfloat16())
+        else:  # rows that start elsewhere add up their exponentials in another order
+            torch.testing.assert_close(d1.float(), d2, rtol=2.0 ** -8 * 1.01, atol=4e-6 / N)
+        part = _ext.C().projection_distill_forward(*args, "gradient", workspace_bytes=1)
+        # (256 rows may run on the other kernel, whose products add up in another order)
+        torch.testing.assert_close(part[6].float(), d1.float(), rtol=2.0 ** -7, atol=2.0 ** -15 / N)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("N,V,K_in", [(65, 1003, 96), (2100, 4100, 64), (4096, 12301, 192)])
+def test_projected_pass_captured_and_replayed(N, V, K_in, dtype):
+    x, w, ids, teacher, targets = projected(N, V, K_in, dtype, K=5)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+
+    def step():
+        r = projection_topk_distillation(xs, ws, ids, teacher, targets, 2.0, 0.5)
+        return (r.loss, r.correct, *torch.autograd.grad(r.loss * 1024, (xs, ws)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            xs.copy_(x * (1 + 0.25 * k))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_projection_without_gradients_and_without_rows(dtype):
+    x, w, ids, teacher, targets = projected(50, 300, 64, dtype)
+    w.requires_grad_()
+    r = projection_topk_distillation(x, w, ids, teacher, targets, 2.0, 0.5)
+    with torch.no_grad():
+        s = projection_topk_distillation(x, w, ids, teacher, targets, 2.0, 0.5)
+    assert torch.equal(r.loss.detach(), s.loss) and torch.equal(r.metrics, s.metrics) and not s.loss.requires_grad
+    x0 = x[:0].requires_grad_()
+    r = projection_topk_distillation(x0, w, ids[:0], teacher[:0], targets[:0], 2.0, 0.5)
+    r.loss.backward()
+    assert float(r.loss) == 0.0 and x0.grad.shape == (0, 64) and torch.equal(w.grad, torch.zeros_like(w))
