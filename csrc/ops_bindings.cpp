@@ -1025,7 +1025,9 @@ Tensor colsum(Tensor dy) {
 // General matrix product on the MFMA kernels (used by tests and benchmarks):
 // C[M,N] = alpha * op(A) op(B)^T with the layout flags of kernels::GemmArgs.
 // out: write C into this [M, N] tensor (e.g. a gradient-bucket slice) instead of allocating it.
-Tensor gemm(Tensor A, Tensor B, bool a_kmajor, bool b_kmajor, c10::optional<Tensor> bias, int64_t act, c10::optional<Tensor> out) {
+// spread: see run_gemm (no activation).
+Tensor gemm(Tensor A, Tensor B, bool a_kmajor, bool b_kmajor, c10::optional<Tensor> bias, int64_t act, c10::optional<Tensor> out, bool spread) {
+  TORCH_CHECK(!spread || (act == kernels::kActNone && (a_kmajor || !b_kmajor)), "gemm: a spread product has no activation and one of a linear layer's layouts");
   check_gpu(A, "A");
   check_gpu(B, "B");
   TORCH_CHECK(A.dim() == 2 && B.dim() == 2 && A.scalar_type() == B.scalar_type(), "gemm: 2-D tensors of one dtype expected");
@@ -1056,7 +1058,7 @@ Tensor gemm(Tensor A, Tensor B, bool a_kmajor, bool b_kmajor, c10::optional<Tens
   const int dt = kdtype(A);
   TORCH_CHECK(gemm_path_ok(a, dt), "gemm: shape M=", M, " N=", N, " K=", K, " not supported for dtype ", A.scalar_type());
   DevGuard guard(A);
-  run_gemm(a, dt, stream_of(A), A);
+  run_gemm(a, dt, stream_of(A), A, spread);
   return C;
 }
 
@@ -1503,7 +1505,7 @@ void init_ops(py::module_& m) {
   m.def("conv3x3_forward", &conv3x3_forward, py::arg("xpad"), py::arg("weight"), py::arg("B"), py::arg("H"), py::arg("W"));
   m.def("conv3x3_wgrad", &conv3x3_wgrad, py::arg("dypad"), py::arg("xpad"), py::arg("B"), py::arg("H"), py::arg("W"));
   m.def("gemm", &gemm, py::arg("A"), py::arg("B"), py::arg("a_kmajor") = true, py::arg("b_kmajor") = true, py::arg("bias") = py::none(),
-        py::arg("act") = 0, py::arg("out") = py::none());
+        py::arg("act") = 0, py::arg("out") = py::none(), py::arg("spread") = false);
   m.def("batchnorm_supported", [](int64_t R, int64_t C, const std::string& dtype) {
     return kernels::batchnorm_supported(R, C, dtype == "float32" ? kernels::kF32 : (dtype == "bfloat16" ? kernels::kBF16 : kernels::kF16));
   });

@@ -89,7 +89,8 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
         C = _ext.C()
         args = (ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, reduction == "mean")
         half = x2.dtype == torch.float16
-        if impl == "native" and x2.dtype != torch.float32:
+        impl = "strict" if impl == "native" else impl
+        if impl == "strict" and x2.dtype != torch.float32:
             loss, correct, metrics, scale, stats, logits, dlogits = C.projection_distill_forward(
                 x2, weight, *args, "none" if not grad else "logits" if half else "gradient")
         else:

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 import torch.nn.functional as F
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from distributed_pytorch_amd.ops import TopKDistillation, projection_topk_distillation, topk_distillation
 
@@ -633,3 +634,55 @@ def test_projection_without_gradients_and_without_rows(dtype):
     r = projection_topk_distillation(x0, w, ids[:0], teacher[:0], targets[:0], 2.0, 0.5)
     r.loss.backward()
     assert float(r.loss) == 0.0 and x0.grad.shape == (0, 64) and torch.equal(w.grad, torch.zeros_like(w))
+
+
+class _Calls(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+    def products(self):
+        return [n for n in self.names if any(w in n for w in ("mm", "matmul", "linear", "dot", "mv"))]
+
+
+@gpu
+@pytest.mark.parametrize("N,V,K_in", [(50, 304, 64), (3, 16, 8), (33, 7, 96), (70, 1003, 77)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_projection_takes_no_library_product(N, V, K_in, dtype):
+    x, w, ids, teacher, targets = projected(N, V, K_in, dtype, K=5)
+    x.requires_grad_()
+    w.requires_grad_()
+    with _Calls() as seen:
+        r = projection_topk_distillation(x, w, ids, teacher, targets, 2.0, 0.5)
+        r.loss.backward()
+    assert seen.names and seen.products() == []
+    with _Calls() as seen:  # (the mode sees the products of a forward and of a backward)
+        F.linear(x, w).sum().backward()
+    assert len(seen.products()) >= 3
+
+
+@gpu
+@pytest.mark.parametrize("N,V,K_in", [(5, 7, 3), (33, 16, 96), (257, 5003, 64), (1000, 72, 333), (64, 20000, 520)])
+def test_half_precision_projection_against_float64(N, V, K_in):
+    x, w, ids, teacher, targets = projected(N, V, K_in, torch.float16, K=5)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    r = projection_topk_distillation(xs, ws, ids, teacher, targets, 2.0, 0.5)
+    up = 2.0 ** 12
+    (r.loss * up).backward()
+    z = x.double() @ w.double().t()
+    rows, grad, n = reference(z, ids, teacher, targets, 2.0, 0.5)
+    grad = grad.to(DEV) * up / n
+    assert abs(float(r.loss.detach()) - float(rows.sum()) / n) <= 2.0 ** -17 * 4
+    # dlogits: probabilities of float32 logits (2^-17 of their size), rounded to half a step of theirs or of the smallest; then one product
+    # of V or N terms in float32 and its rounding
+    half, tiny = 2.0 ** -11, 2.0 ** -25
+    q = grad.abs() + up / n * (torch.softmax(z / 2, 1) + 0.5 * torch.softmax(z, 1))
+    for got, want, bound, steps, terms in ((xs.grad, grad @ w.double(), q @ w.double().abs(), w.double().abs().sum(0), V),
+                                           (ws.grad, grad.t() @ x.double(), q.t() @ x.double().abs(), x.double().abs().sum(0), N)):
+        err = (got.double() - want).abs()
+        near = half + 2.0 ** -15 + terms * 2.0 ** -24
+        assert bool((err <= near * bound + half * want.abs() + tiny * (steps + 1)).all())
