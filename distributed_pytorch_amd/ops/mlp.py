@@ -37,6 +37,7 @@ from .. import _ext
 from . import gemm
 from .grad_sink import weight_grad_buffer
 from .linear import ACT_GELU, ACT_RELU, ACT_SILU, _act_code, _torch_act, linear_bias_act
+from .tangents import is_differentiated
 
 
 class _FusedMLP(torch.autograd.Function):
@@ -160,7 +161,7 @@ def gated_mlp(x: torch.Tensor, w_fc: torch.Tensor, b_fc: Optional[torch.Tensor],
     code = _GATES.get(act)
     if code is None:
         raise ValueError(f"unknown gate activation {act!r} (silu | gelu | relu)")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_fc, b_fc, w_proj, b_proj))
+    grad = is_differentiated(x, w_fc, b_fc, w_proj, b_proj)
     if x.is_cuda and not grad:
         y = _ext.C().gated_mlp_forward(x, w_fc, b_fc, w_proj, b_proj, code)
         if y is not None:

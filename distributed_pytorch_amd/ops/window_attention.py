@@ -20,6 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _ext
+from .tangents import is_differentiated
 
 _NAMES = {torch.bfloat16: "bfloat16", torch.float16: "float16"}
 
@@ -118,7 +119,7 @@ def window_attention_qkvpacked(qkv: torch.Tensor, n_head: int, window: int, sink
             if lens is not None:
                 lens = (lens if lens.dtype == torch.int32 else lens.clamp(0, qkv.shape[1]).to(torch.int32)).contiguous()
             cfg = (n_head, n_kv, int(window), int(sinks), scale)
-            if not (torch.is_grad_enabled() and qkv.requires_grad):
+            if not is_differentiated(qkv):
                 return _ext.C().window_attention_forward(qkv, *cfg, lens, False)[0]
             return _WindowAttention.apply(qkv, cfg, lens)
         if impl == "native":
