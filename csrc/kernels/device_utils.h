@@ -261,17 +261,18 @@ __device__ __forceinline__ float gelu_fwd(float x) {
 
 // act(g) and act'(g) of a gate, ACT = 1 relu, 2 gelu, 3 silu (kernels.h Act).
 //   silu: g t with t = 1 / (1 + exp(-g)); slope t (1 + g (1 - t))       gelu: g Phi(g); slope Phi(g) + g phi(g)
+// A NaN stays one in all of them, in the value and in the slope.
 template <int ACT>
 __device__ __forceinline__ float gate_value(float g) {
-  if constexpr (ACT == 1) return g > 0.f ? g : 0.f;
+  if constexpr (ACT == 1) return g < 0.f ? 0.f : g;
   else if constexpr (ACT == 2) return gelu_fwd(g);
   else return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
 }
 template <int ACT>
 __device__ __forceinline__ void gate_value_and_slope(float g, float& value, float& slope) {
   if constexpr (ACT == 1) {
-    value = g > 0.f ? g : 0.f;
-    slope = g > 0.f ? 1.f : 0.f;
+    value = g < 0.f ? 0.f : g;
+    slope = g > 0.f ? 1.f : g <= 0.f ? 0.f : g;
   } else if constexpr (ACT == 2) {
     const float cdf = normal_cdf(g);
     value = g * cdf;

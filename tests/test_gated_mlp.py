@@ -369,3 +369,29 @@ def test_spread_products_captured_and_replayed(M, K, H, N, dtype):
         for _, out in graphs:
             for got, w in zip(out, want):
                 assert torch.equal(got, w)
+
+
+# one size for each kernel: few rows, 128 x 128 and 256 x 256 tiles, fp32 products with the gate behind them
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("M,H,dtype", [(3, 40, torch.bfloat16), (150, 40, torch.float16), (4096, 2304, torch.bfloat16), (70, 40, torch.float32)])
+def test_a_gate_that_is_not_a_number_shows(M, H, dtype, act):
+    from distributed_pytorch_amd import _ext
+
+    C = _ext.C()
+    code = {"silu": C.ACT_SILU, "gelu": C.ACT_GELU, "relu": C.ACT_RELU}[act]
+    t, dy = make(M, 64, H, 64, dtype)
+    plain_h, plain_gu = C.gated_forward(t["x"], t["w_fc"], t["b_fc"], code, True)
+    plain_d = C.gated_backward(dy, t["w_proj"], plain_gu, code, True)
+    lost = H // 3
+    t["b_fc"][lost] = float("nan")       # the gate's half only: u stays finite
+    h, gu = C.gated_forward(t["x"], t["w_fc"], t["b_fc"], code, True)
+    quiet, _ = C.gated_forward(t["x"], t["w_fc"], t["b_fc"], code, False)
+    d, db = C.gated_backward(dy, t["w_proj"], gu, code, True)
+    assert torch.isnan(h[:, lost]).all() and torch.isnan(quiet[:, lost]).all() and torch.isnan(gu[:, lost]).all()
+    for got in (d, db):
+        assert torch.isnan(got[..., lost]).all() and torch.isnan(got[..., H + lost]).all()
+    rest = [i for i in range(2 * H) if i % H != lost]
+    for got, want in ((h, plain_h), (quiet, plain_h)):
+        assert torch.equal(got[:, rest[: H - 1]], want[:, rest[: H - 1]])
+    assert torch.equal(d[:, rest], plain_d[0][:, rest]) and torch.equal(db[rest], plain_d[1][rest])
