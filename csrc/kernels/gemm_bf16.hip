@@ -1216,10 +1216,11 @@ __global__ __launch_bounds__(kThreads2, 2) void gemm_bf16_8ph_kernel(GemmArgs p,
             for (int e = 0; e < 4; ++e) {
               float value, slope;
               gate_value_and_slope<GACT>(BF16::to_f32(gx[j][e]), value, slope);
-              dg[e] = BF16::from_f32(a[e] * BF16::to_f32(ux[j][e]) * slope);
-              du[e] = BF16::from_f32(a[e] * value);
-              cg[j][e] += BF16::to_f32(dg[e]);
-              cu[j][e] += BF16::to_f32(du[e]);
+              const float fg = a[e] * BF16::to_f32(ux[j][e]) * slope, fu = a[e] * value;
+              dg[e] = BF16::from_f32(fg);
+              du[e] = BF16::from_f32(fu);
+              cg[j][e] += fg;  // (the bias gradient's sums, ahead of the rounding)
+              cu[j][e] += fu;
             }
             *reinterpret_cast<u16x4*>(img_g + cell[j]) = dg;  // same lane, same cell
             *reinterpret_cast<u16x4*>(img_u + cell[j]) = du;

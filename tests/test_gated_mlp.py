@@ -395,3 +395,29 @@ def test_a_gate_that_is_not_a_number_shows(M, H, dtype, act):
     for got, want in ((h, plain_h), (quiet, plain_h)):
         assert torch.equal(got[:, rest[: H - 1]], want[:, rest[: H - 1]])
     assert torch.equal(d[:, rest], plain_d[0][:, rest]) and torch.equal(db[rest], plain_d[1][rest])
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+def test_bias_gradients_are_summed_ahead_of_the_rounding(act):
+    # Products of a contraction of 64 and g | u as stored are exact to float32 here; what is left is the additions and one rounding.  Summed after
+    # the rounding to bf16, 4096 terms of size d would leave 64 d 2^-10, which shows in the columns whose sum nearly cancels.
+    from distributed_pytorch_amd import _ext
+
+    C = _ext.C()
+    M, H, N = 4096, 2304, 64
+    g = torch.Generator().manual_seed(5)
+    dy = torch.randn(M, N, generator=g).bfloat16().to(DEV)
+    w = (torch.randn(N, H, generator=g) / 8).bfloat16().to(DEV)
+    gu = torch.randn(M, 2 * H, generator=g).bfloat16().to(DEV)
+    _, db = C.gated_backward(dy, w, gu, {"silu": C.ACT_SILU, "gelu": C.ACT_GELU, "relu": C.ACT_RELU}[act], True)
+    gate, u = gu.double().chunk(2, 1)
+    gate = gate.requires_grad_()
+    a = {"silu": F.silu, "gelu": F.gelu, "relu": F.relu}[act](gate)
+    (slope,) = torch.autograd.grad(a.sum(), gate)
+    dh = dy.double() @ w.double()
+    d = torch.cat([dh * u * slope, dh * a.detach()], 1)
+    want = d.sum(0)
+    # bf16's own rounding of the sum; of every term the activation's 2e-6 and of the sums 2^-24 an addition, of unlike sign: their root sum of squares, 6 of those
+    near = 2.0 ** -8 * want.abs() + 6 * (2e-6 + 64 * 2.0 ** -24) * d.square().sum(0).sqrt() + 6 * 2.0 ** -24 * 64 * d.square().sum(0).sqrt()
+    assert bool(((db.double() - want).abs() <= near).all())
