@@ -927,11 +927,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rank1_mlp_backward(Tensor dy, Tensor 
           grads.narrow(0, (NT + 2) * H, N)};
 }
 
-// Gradients of y = x W^T + b given g = dL/d(xW^T+b).  Returns (dx or None, dW, db or None).
+// Gradients of y = x W^T + b given g = dL/d(xW^T+b).  Returns (dx or None, dW or None, db or None).
 // dw_out: write the weight gradient into this tensor (a slice of a gradient bucket) instead of a fresh one.
 // spread: see run_gemm; the column sums of few rows are then taken in one launch.
-std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward(Tensor g, Tensor x, Tensor w, bool need_dx, bool need_db,
-                                                                                   c10::optional<Tensor> dw_out, bool spread) {
+// need_dw false (a frozen weight): the others come from the same kernels as with it.
+std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>> linear_backward(Tensor g, Tensor x, Tensor w, bool need_dx, bool need_db,
+                                                                                                c10::optional<Tensor> dw_out, bool spread, bool need_dw) {
   check_gpu(g, "grad");
   check_gpu(x, "x");
   check_gpu(w, "weight");
@@ -943,8 +944,12 @@ std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward
   const int dt = kdtype(x);
   DevGuard guard(x);
   hipStream_t s = stream_of(x);
+  // (the kernels of degenerate extents compute the weight and bias gradients in one pass)
+  const bool degenerate = K == 1 || N <= 16;
   Tensor dW;
-  if (dw_out.has_value() && dw_out->defined()) {
+  if (!need_dw && !(degenerate && need_db)) {
+    // nothing to write it to
+  } else if (need_dw && dw_out.has_value() && dw_out->defined()) {
     check_gpu(*dw_out, "dw_out");
     TORCH_CHECK(dw_out->sizes() == w.sizes() && dw_out->scalar_type() == w.scalar_type() && dw_out->is_contiguous() &&
                     dw_out->get_device() == w.get_device(), "linear_backward: dw_out must be a contiguous tensor like the weight");
@@ -957,24 +962,30 @@ std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward
   if (need_dx) dx = at::empty_like(x);
   auto fopt = x.options().dtype(at::kFloat);
   if (K == 1) {
-    Tensor ws = at::empty({kernels::colreduce_workspace(M, N)}, fopt);
-    Tensor db_tmp = need_db ? *db : at::empty({N}, w.options());
-    kernels::launch_outer_wgrad(g.data_ptr(), x.data_ptr(), dW.data_ptr(), db_tmp.data_ptr(), ws.data_ptr<float>(), M, N, dt, s);
+    if (need_dw || need_db) {
+      Tensor ws = at::empty({kernels::colreduce_workspace(M, N)}, fopt);
+      Tensor db_tmp = need_db ? *db : at::empty({N}, w.options());
+      kernels::launch_outer_wgrad(g.data_ptr(), x.data_ptr(), dW.data_ptr(), db_tmp.data_ptr(), ws.data_ptr<float>(), M, N, dt, s);
+    }
     if (need_dx) {
       // dx[m] = sum_n g[m,n] w[n]: a skinny product with a single output column.
       kernels::launch_skinny_n(g.data_ptr(), w.data_ptr(), nullptr, dx->data_ptr(), M, 1, N, dt, s);
     }
   } else if (N <= 16) {
-    Tensor ws = at::empty({kernels::skinny_wgrad_workspace(M, N, K)}, fopt);
-    kernels::launch_skinny_n_wgrad(g.data_ptr(), x.data_ptr(), dW.data_ptr(), need_db ? db->data_ptr() : nullptr, ws.data_ptr<float>(), M, N, K, dt, s);
+    if (need_dw || need_db) {
+      Tensor ws = at::empty({kernels::skinny_wgrad_workspace(M, N, K)}, fopt);
+      kernels::launch_skinny_n_wgrad(g.data_ptr(), x.data_ptr(), dW.data_ptr(), need_db ? db->data_ptr() : nullptr, ws.data_ptr<float>(), M, N, K, dt, s);
+    }
     if (need_dx) kernels::launch_skinny_n_dgrad(g.data_ptr(), w.data_ptr(), dx->data_ptr(), M, N, K, dt, s);
   } else {
-    // dW[N,K] = g^T x : contraction over M; both operands are stored with the contraction dim slowest.
-    kernels::GemmArgs a{};
-    a.A = g.data_ptr(); a.B = x.data_ptr(); a.C = dW.data_ptr();
-    a.M = N; a.N = K; a.K = M; a.lda = N; a.ldb = K; a.ldc = K; a.a_kmajor = 0; a.b_kmajor = 0; a.alpha = 1.f;
-    TORCH_CHECK(gemm_path_ok(a, dt), "linear_backward: weight-gradient shape not supported by the MFMA GEMM");
-    run_gemm(a, dt, s, g, spread);
+    if (need_dw) {
+      // dW[N,K] = g^T x : contraction over M; both operands are stored with the contraction dim slowest.
+      kernels::GemmArgs a{};
+      a.A = g.data_ptr(); a.B = x.data_ptr(); a.C = dW.data_ptr();
+      a.M = N; a.N = K; a.K = M; a.lda = N; a.ldb = K; a.ldc = K; a.a_kmajor = 0; a.b_kmajor = 0; a.alpha = 1.f;
+      TORCH_CHECK(gemm_path_ok(a, dt), "linear_backward: weight-gradient shape not supported by the MFMA GEMM");
+      run_gemm(a, dt, s, g, spread);
+    }
     if (need_dx) {
       // dx[M,K] = g W : contraction over N; A = g is contraction-contiguous, B = W is stored [N(contraction), K].
       kernels::GemmArgs b{};
@@ -990,7 +1001,7 @@ std::tuple<c10::optional<Tensor>, Tensor, c10::optional<Tensor>> linear_backward
       kernels::launch_colsum(g.data_ptr(), db->data_ptr(), ws.data_ptr<float>(), M, N, dt, s);
     }
   }
-  return {dx, dW, db};
+  return {dx, need_dw ? c10::optional<Tensor>(dW) : c10::nullopt, db};
 }
 
 // g = dy * act'(saved) and optionally db = colsum(g).  saved: output y for ReLU, pre-activation for GELU.
@@ -1493,7 +1504,7 @@ void init_ops(py::module_& m) {
   m.def("linear_forward", &linear_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act") = 0, py::arg("save_pre_act") = false,
         py::arg("spread") = false);
   m.def("linear_backward", &linear_backward, py::arg("grad"), py::arg("x"), py::arg("weight"), py::arg("need_dx") = true, py::arg("need_db") = true,
-        py::arg("dw_out") = py::none(), py::arg("spread") = false);
+        py::arg("dw_out") = py::none(), py::arg("spread") = false, py::arg("need_dw") = true);
   m.def("rank1_mlp_forward", &rank1_mlp_forward, py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("b2"), py::arg("act") = 0);
   m.def("rank1_mlp_backward", &rank1_mlp_backward, py::arg("dy"), py::arg("x"), py::arg("w1"), py::arg("b1"), py::arg("W2"), py::arg("act") = 0);
   m.def("gated_forward", &gated_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("save") = true);

@@ -125,16 +125,13 @@ class _GatedMLP(torch.autograd.Function):
         need = ctx.needs_input_grad
         has_fc, has_proj = ctx.biases
         dx = dw_fc = db_fc = dw_proj = db_proj = None
-        if need[3]:
-            _, dw_proj, db_proj = C.linear_backward(dy, h, w_proj, False, has_proj and need[4], _sink(w_proj), True)
-        elif has_proj and need[4]:
-            db_proj = C.colsum(dy)
+        # (a frozen weight changes nothing but its own gradient: the others come from the same kernels)
+        if need[3] or (has_proj and need[4]):
+            _, dw_proj, db_proj = C.linear_backward(dy, h, w_proj, False, has_proj and need[4], _sink(w_proj) if need[3] else None, True, need[3])
         if need[0] or need[1] or need[2]:
             dgu, db_fc = C.gated_backward(dy, w_proj, gu, ctx.act, has_fc and need[2])
-            if need[1]:
-                dx, dw_fc, _ = C.linear_backward(dgu, x2, w_fc, need[0], False, _sink(w_fc), True)
-            elif need[0]:
-                dx = C.gemm(dgu, w_fc, True, False)
+            if need[0] or need[1]:
+                dx, dw_fc, _ = C.linear_backward(dgu, x2, w_fc, need[0], False, _sink(w_fc) if need[1] else None, True, need[1])
         return dx, dw_fc, db_fc, dw_proj, db_proj, None
 
 

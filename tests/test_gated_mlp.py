@@ -421,3 +421,20 @@ def test_bias_gradients_are_summed_ahead_of_the_rounding(act):
     # bf16's own rounding of the sum; of every term the activation's 2e-6 and of the sums 2^-24 an addition, of unlike sign: their root sum of squares, 6 of those
     near = 2.0 ** -8 * want.abs() + 6 * (2e-6 + 64 * 2.0 ** -24) * d.square().sum(0).sqrt() + 6 * 2.0 ** -24 * 64 * d.square().sum(0).sqrt()
     assert bool(((db.double() - want).abs() <= near).all())
+
+
+# sizes whose products are spread, few rows, 256 x 256 tiles, degenerate extents
+@gpu
+@pytest.mark.parametrize("M,K,H,N,dtype", [(300, 96, 2048, 96, torch.float16), (464, 104, 1056, 40, torch.float32), (1003, 520, 1386, 520, torch.bfloat16),
+                                           (60, 72, 1040, 66, torch.float16), (4096, 256, 2304, 256, torch.bfloat16), (200, 1, 24, 7, torch.float32),
+                                           (200, 1, 24, 16, torch.bfloat16), (33, 5, 8, 1, torch.float16)])
+def test_frozen_tensors_leave_the_other_gradients_as_they_are(M, K, H, N, dtype):
+    t, dy = make(M, K, H, N, dtype)
+    want = run(t, dy, "silu")
+    every = list(t)
+    for frozen in (["w_fc"], ["w_proj"], ["w_fc", "w_proj"], ["x"], ["x", "w_fc"], ["b_fc"], ["b_proj"], ["x", "w_fc", "w_proj"], ["b_fc", "b_proj", "w_fc"]):
+        names = [n for n in every if n not in frozen]
+        leaf = {k: v.detach().requires_grad_(k in names) for k, v in t.items()}
+        y = gated_mlp(leaf["x"], leaf["w_fc"], leaf["b_fc"], leaf["w_proj"], leaf["b_proj"])
+        for n, g in zip(names, torch.autograd.grad(y, [leaf[n] for n in names], dy)):
+            assert torch.equal(g, want["d" + n]), (n, frozen)
