@@ -444,10 +444,6 @@ __global__ __launch_bounds__(256) void distill_apply_upstream_kernel(typename TR
 
 }  // namespace
 
-bool distill_types_supported(int dtype, int out_dtype, int mode) {
-  return dtype == out_dtype || mode == kForward || (dtype == kF32 && (out_dtype == kBF16 ? mode == kFused : mode == kBackward));
-}
-
 bool distill_supported(long long C, long long ld, long long K) {
   return C >= 1 && C <= ld && ld <= kDistillMaxWidth && K >= 1 && K <= kDistillMaxEntries;
 }
@@ -505,7 +501,7 @@ void launch_distill(const DistillArgs& args, int dtype, int out_dtype, int mode,
       if constexpr (std::is_same<TR, TO>::value) {
         if (mode == kForward) by_size(integral_constant<int, kForward>{});
         else if (mode == kBackward) by_size(integral_constant<int, kBackward>{});
-        else by_size(integral_constant<int, kFused>{});
+        else if constexpr (!std::is_same<TR, F16>::value) by_size(integral_constant<int, kFused>{});  // (fp16 gradients wait for the upstream one)
       } else if constexpr (std::is_same<TO, BF16>::value) {
         by_size(integral_constant<int, kFused>{});  // (bf16 gradients of float32 logits are only asked for with the loss, ...
       } else {

@@ -13,24 +13,24 @@ namespace kernels {
 namespace {
 
 // One thread per element; rows of H are short against the grid and every access of a wave is contiguous.
-template <typename TR, int ACT>
-__global__ __launch_bounds__(256) void gate_fwd_kernel(const typename TR::T* __restrict__ gu, typename TR::T* __restrict__ h, long long n, long long H) {
+template <int ACT>
+__global__ __launch_bounds__(256) void gate_fwd_kernel(const float* __restrict__ gu, float* __restrict__ h, long long n, long long H) {
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * 256) {
     const long long row = i / H, at = row * 2 * H + (i - row * H);
-    h[i] = TR::from_f32(gate_value<ACT>(TR::to_f32(gu[at])) * TR::to_f32(gu[at + H]));
+    h[i] = gate_value<ACT>(gu[at]) * gu[at + H];
   }
 }
 
-template <typename TR, int ACT>
-__global__ __launch_bounds__(256) void gate_bwd_kernel(const typename TR::T* __restrict__ dh, const typename TR::T* __restrict__ gu,
-                                                       typename TR::T* __restrict__ dgu, long long n, long long H) {
+template <int ACT>
+__global__ __launch_bounds__(256) void gate_bwd_kernel(const float* __restrict__ dh, const float* __restrict__ gu, float* __restrict__ dgu, long long n,
+                                                       long long H) {
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * 256) {
     const long long row = i / H, at = row * 2 * H + (i - row * H);
     float value, slope;
-    gate_value_and_slope<ACT>(TR::to_f32(gu[at]), value, slope);
-    const float d = TR::to_f32(dh[i]);
-    dgu[at] = TR::from_f32(d * TR::to_f32(gu[at + H]) * slope);
-    dgu[at + H] = TR::from_f32(d * value);
+    gate_value_and_slope<ACT>(gu[at], value, slope);
+    const float d = dh[i];
+    dgu[at] = d * gu[at + H] * slope;
+    dgu[at + H] = d * value;
   }
 }
 
@@ -48,28 +48,14 @@ unsigned blocks_for(long long n) {
 
 }  // namespace
 
-void launch_gate_fwd(const void* gu, void* h, long long M, long long H, int dtype, int act, hipStream_t stream) {
+void launch_gate_fwd(const float* gu, float* h, long long M, long long H, int act, hipStream_t stream) {
   if (M * H <= 0) return;
-  with_act(act, [&](auto act_c) {
-    dispatch_dtype(dtype, [&](auto tr) {
-      using TR = decltype(tr);
-      using T = typename TR::T;
-      hipLaunchKernelGGL((gate_fwd_kernel<TR, decltype(act_c)::value>), dim3(blocks_for(M * H)), dim3(256), 0, stream, static_cast<const T*>(gu),
-                         static_cast<T*>(h), M * H, H);
-    });
-  });
+  with_act(act, [&](auto act_c) { hipLaunchKernelGGL((gate_fwd_kernel<decltype(act_c)::value>), dim3(blocks_for(M * H)), dim3(256), 0, stream, gu, h, M * H, H); });
 }
 
-void launch_gate_bwd(const void* dh, const void* gu, void* dgu, long long M, long long H, int dtype, int act, hipStream_t stream) {
+void launch_gate_bwd(const float* dh, const float* gu, float* dgu, long long M, long long H, int act, hipStream_t stream) {
   if (M * H <= 0) return;
-  with_act(act, [&](auto act_c) {
-    dispatch_dtype(dtype, [&](auto tr) {
-      using TR = decltype(tr);
-      using T = typename TR::T;
-      hipLaunchKernelGGL((gate_bwd_kernel<TR, decltype(act_c)::value>), dim3(blocks_for(M * H)), dim3(256), 0, stream, static_cast<const T*>(dh),
-                         static_cast<const T*>(gu), static_cast<T*>(dgu), M * H, H);
-    });
-  });
+  with_act(act, [&](auto act_c) { hipLaunchKernelGGL((gate_bwd_kernel<decltype(act_c)::value>), dim3(blocks_for(M * H)), dim3(256), 0, stream, dh, gu, dgu, M * H, H); });
 }
 
 }  // namespace kernels

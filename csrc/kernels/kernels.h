@@ -99,7 +99,7 @@ void launch_xent_fused(void* logits, int dtype, const long long* targets, long l
 //   row loss = soft_weight tau^2 KL(p || softmax(z / tau)) + hard_weight CE(z, target), 0 for ignored rows
 // mode 0: row losses, correct flags, row_stats[3 r ..] = {max z, sum of exponentials, sum at temperature 1 where both are needed}
 // mode 1: dlogits from row_stats, scaled by scale[0] * grad_out[grad_out_rows ? r : 0]
-// mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits
+// mode 2: mode 0 without row_stats, and dlogits scaled by scale[0]; dlogits may alias logits; not in fp16
 // dlogits [N, out_ld]: columns [C, out_ld) are written as zero.  In the logits' type: out_ld is ld and the address equals that of logits modulo 16.
 // Float32 logits in rows of 16-byte vectors (ld a multiple of 4, an address of 16) may have a 16-bit gradient: bf16 in mode 2, fp16 in mode 1.
 constexpr int kDistillMaxEntries = 1024;
@@ -127,7 +127,6 @@ struct DistillArgs {
   long long row0;
 };
 bool distill_supported(long long C, long long ld, long long K);
-bool distill_types_supported(int dtype, int out_dtype, int mode);
 void launch_distill(const DistillArgs& a, int dtype, int out_dtype, int mode, hipStream_t stream);
 // scale[0] = 1 / max(#targets != ignore_index, 1) for a mean (N rows without targets), 1 for a sum.
 void launch_distill_scale(const long long* targets, long long N, long long ignore_index, int mean, float* scale, hipStream_t stream);
@@ -228,9 +227,9 @@ void launch_few_rows(const GemmArgs& a, int dtype, hipStream_t stream);
 bool gemm_gate_supported(const GemmArgs& a, int dtype);
 long long gemm_gate_colsum_rows(const GemmArgs& a, int dtype);  // 0: this launch takes no column sums
 void launch_gemm_gate(const GemmArgs& a, int dtype, hipStream_t stream);
-// The same on float32 (or any) products that exist already: h = act(g) * u; dgu = dh u act'(g) | dh act(g).
-void launch_gate_fwd(const void* gu, void* h, long long M, long long H, int dtype, int act, hipStream_t stream);
-void launch_gate_bwd(const void* dh, const void* gu, void* dgu, long long M, long long H, int dtype, int act, hipStream_t stream);
+// The same on float32 products that exist already: h = act(g) * u; dgu = dh u act'(g) | dh act(g).
+void launch_gate_fwd(const float* gu, float* h, long long M, long long H, int act, hipStream_t stream);
+void launch_gate_bwd(const float* dh, const float* gu, float* dgu, long long M, long long H, int act, hipStream_t stream);
 
 // dst [rows_total][C] (bf16, 16-byte aligned): row guard_front + q is haloed pixel q of x [B][H][W][C] -- zero on the
 // one-pixel frame of every image -- and every row outside [guard_front, guard_front + B*(H+2)*(W+2)) is zero.

@@ -338,7 +338,8 @@ kernels::DistillArgs distill_args(const Tensor& logits, const Tensor& ids, const
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> distill_forward(Tensor logits, Tensor ids, Tensor teacher, c10::optional<Tensor> targets,
                                                                                    int64_t n_classes, int64_t ignore_index, double temperature,
                                                                                    double hard_weight, bool mean, const std::string& gradient) {
-  TORCH_CHECK(gradient == "none" || gradient == "new" || gradient == "inplace", "distill_forward: gradient must be none, new or inplace");
+  TORCH_CHECK(gradient == "none" || ((gradient == "new" || gradient == "inplace") && logits.scalar_type() != at::kHalf),
+              "distill_forward: gradient must be none or, but for fp16, new or inplace");
   kernels::DistillArgs a = distill_args(logits, ids, teacher, targets, n_classes, ignore_index, temperature, hard_weight, "distill_forward");
   DevGuard g(logits);
   hipStream_t s = stream_of(logits);
@@ -759,7 +760,7 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_forward(Tensor x, Tensor w, c10:
   if (dt == kernels::kF32) {
     Tensor gu = std::get<0>(linear_forward(x, w, bias, kernels::kActNone, false, true));
     Tensor h = at::empty({M, H}, x.options());
-    kernels::launch_gate_fwd(gu.data_ptr(), h.data_ptr(), M, H, dt, static_cast<int>(act), s);
+    kernels::launch_gate_fwd(gu.data_ptr<float>(), h.data_ptr<float>(), M, H, static_cast<int>(act), s);
     return {h, save ? c10::optional<Tensor>(gu) : c10::nullopt};
   }
   kernels::GemmArgs a{};
@@ -842,7 +843,7 @@ std::tuple<Tensor, c10::optional<Tensor>> gated_backward(Tensor dy, Tensor w, Te
     a.ldc = H;
     TORCH_CHECK(gemm_path_ok(a, dt), "gated_backward: shape M=", M, " N=", N, " H=", H, " is not supported");
     run_gemm(a, dt, s, dy, true);
-    kernels::launch_gate_bwd(dh.data_ptr(), gu.data_ptr(), dgu.data_ptr(), M, H, dt, static_cast<int>(act), s);
+    kernels::launch_gate_bwd(dh.data_ptr<float>(), gu.data_ptr<float>(), dgu.data_ptr<float>(), M, H, static_cast<int>(act), s);
   } else {
     a.C = dgu.data_ptr();
     a.ldc = 2 * H;
@@ -1473,7 +1474,6 @@ void init_ops(py::module_& m) {
         py::arg("targets"), py::arg("n_classes"), py::arg("ignore_index"), py::arg("temperature"), py::arg("hard_weight"), py::arg("mean"), py::arg("keep"),
         py::arg("workspace_bytes") = 8ll << 30);
   m.def("distill_apply_upstream", &distill_apply_upstream, py::arg("x"), py::arg("g"));
-  m.attr("DISTILL_MAX_ENTRIES") = kernels::kDistillMaxEntries;
   m.def("dgrad_act_backward", &dgrad_act_backward, py::arg("dout"), py::arg("weight"), py::arg("aux"), py::arg("act"), py::arg("want_colsum"));
   m.def("dgrad_act_backward_supported", &dgrad_act_backward_supported);
   m.def("attention_supported", [](int64_t T, int64_t hd, int64_t rs) { return kernels::attention_supported(T, hd, rs); });
