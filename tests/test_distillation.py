@@ -686,3 +686,23 @@ def test_half_precision_projection_against_float64(N, V, K_in):
         err = (got.double() - want).abs()
         near = half + 2.0 ** -15 + terms * 2.0 ** -24
         assert bool((err <= near * bound + half * want.abs() + tiny * (steps + 1)).all())
+
+
+# Every kernel by width, rows that start on and off the 16-byte grid (a row's vectors at its ends are its neighbours' as well, which other workgroups
+# write over meanwhile), rows held in registers and rows read again from the memory that their gradient takes over.
+@gpu
+@pytest.mark.parametrize("width,C", [(70, 64), (1003, 1003), (1021, 900), (7171, 7171), (14343, 14340), (28672, 28000), (28673, 28673), (50257, 50257),
+                                     (57345, 57345), (65543, 65543), (131083, 131000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_over_the_logits_is_that_beside_them(width, C, dtype):
+    from distributed_pytorch_amd import _ext
+
+    logits, ids, teacher, targets = make(37, C, min(C, 30), dtype, DEV, width=width)
+    for tau, a in ((2.0, 0.5), (1.0, 0.0), (1.5, 0.5)):
+        args = (ids, teacher, targets, C, -100, tau, a, True)
+        want = _ext.C().distill_forward(logits, *args, "new")
+        over = logits.clone()
+        got = _ext.C().distill_forward(over, *args, "inplace")
+        assert got[6].data_ptr() == over.data_ptr()
+        for k in (0, 1, 2, 3, 6):
+            assert torch.equal(got[k], want[k]), k

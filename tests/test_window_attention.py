@@ -345,3 +345,23 @@ def test_many_short_sequences():
 
     assert not _ext.C().window_attention_supported(1 << 24, 1, 1, 1, 64, 192, "bfloat16")
     assert _ext.C().window_attention_supported((1 << 24) - 1, 1, 1, 1, 64, 192, "bfloat16")
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sinks", [1, 150])
+def test_padded_batches_whose_key_blocks_are_cut(sinks, D, dtype):
+    # a block with sinks meets 13 query tiles of three heads here, more than one piece of the dK / dV work holds: partial sums, with lengths that end the
+    # sequence inside, ahead of and at the end of what a piece walks
+    T = 777
+    lens = torch.tensor([0, 1, 64, 333, T - 1, T], device=DEV, dtype=torch.int32)
+    qkv, do = make(6, T, 12, 4, D, dtype, seed=sinks)
+    for b, n in enumerate(lens.tolist()):
+        qkv[b, n:] = float("nan")
+        do[b, n:] = float("nan")
+    o, g = check(qkv, do, 12, 4, 128, sinks, lens)
+    for b, n in enumerate(lens.tolist()):
+        assert torch.equal(o[b, n:], torch.zeros_like(o[b, n:])) and torch.equal(g[b, n:], torch.zeros_like(g[b, n:]))
+    again = run(qkv, do, 12, 4, 128, sinks, seq_lens=lens)
+    assert torch.equal(o, again[0]) and torch.equal(g, again[1])
