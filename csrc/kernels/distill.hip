@@ -164,7 +164,7 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     const long long at = r * a.K + k;
     const long long id = a.ids_64 ? static_cast<const long long*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
     const bool in = id >= 0 && id < C;
-    const float t = in ? teacher_at(a, at) * a.inv_tau : kNegInf;
+    const float t = in ? teacher_at(a, at) : kNegInf;  // (divided by tau as a difference to the largest: the type's lowest value is an entry too)
     const bool there = in && t != kNegInf && a.soft_weight != 0.f;  // without a soft term the teacher's values do not matter at all
     s_id[k] = there ? static_cast<int>(id) : -1;
     s_p[k] = t;
@@ -277,13 +277,13 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     }
     float z = 0.f;
     for (int k = lane; k < a.K; k += 64)
-      if (s_id[k] >= 0) z += __builtin_amdgcn_exp2f((s_p[k] - tm) * kLog2e);
+      if (s_id[k] >= 0) z += __builtin_amdgcn_exp2f((s_p[k] - tm) * a.inv_tau * kLog2e);
     z = wave_sum(z);
     const float log_z = logf(z), inv_z = 1.f / z;
     float b = 0.f;  // sum_k p_k (log p_k - log(exponential of x_k)); with log(sum) added it is the divergence
     for (int k = lane; k < a.K; k += 64) {
       if (s_id[k] < 0) continue;
-      const float t = s_p[k] - tm;
+      const float t = (s_p[k] - tm) * a.inv_tau;
       const float p = __builtin_amdgcn_exp2f(t * kLog2e) * inv_z;
       if (MODE != kBackward && !(p == 0.f)) b += p * ((t - log_z) - fmaf(s_x[k], c, -mc) * kLn2);
       s_p[k] = p * (a.soft_weight * a.tau);  // its share of the gradient

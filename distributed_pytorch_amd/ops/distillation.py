@@ -166,12 +166,15 @@ def _composed(logits, ids, teacher, targets, cfg) -> DistillResult:
     live = counted if targets is None else counted & (targets >= 0) & (targets < n_classes)
     z = torch.where(live.unsqueeze(1), z, z.new_zeros(()))  # an ignored row may hold anything
     row = z.new_zeros(N)
-    t = teacher.to(z.dtype) / temperature
+    t = teacher.to(z.dtype)
     there = (ids >= 0) & (ids < n_classes) & (t != float("-inf"))
     if hard_weight < 1:
         at = torch.where(there, ids, 0).long()
-        # a finite stand-in for "absent" keeps rows without entries out of inf - inf
-        log_p = torch.log_softmax(torch.where(there, t, t.new_full((), torch.finfo(t.dtype).min)), 1)
+        # Divided by the temperature as differences to the largest, which the type's lowest value survives; a finite stand-in for "absent" keeps
+        # rows without entries out of inf - inf.
+        top = torch.where(there, t, float("-inf")).amax(1, keepdim=True)
+        top = torch.where(there.any(1, keepdim=True), top, 0.0)
+        log_p = torch.log_softmax(torch.where(there, (t - top) / temperature, t.new_full((), torch.finfo(t.dtype).min)), 1)
         p = torch.where(there, log_p.exp(), 0.0)
         term = p * (log_p - torch.log_softmax(z / temperature, 1).gather(1, at))
         row = row + (1 - hard_weight) * temperature ** 2 * torch.where(p > 0, term, 0.0).sum(1)

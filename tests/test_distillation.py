@@ -706,3 +706,29 @@ def test_gradient_over_the_logits_is_that_beside_them(width, C, dtype):
         assert got[6].data_ptr() == over.data_ptr()
         for k in (0, 1, 2, 3, 6):
             assert torch.equal(got[k], want[k]), k
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("t_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tau", [0.25, 0.5, 1.0, 2.0])
+def test_entries_of_the_lowest_and_largest_values_are_entries(tau, t_dtype, device):
+    logits, ids, teacher, _ = make(5, 60, 6, torch.float32, device, pad_rows=False)
+    low, high = torch.finfo(t_dtype).min, torch.finfo(t_dtype).max
+    teacher = teacher.to(t_dtype)
+    teacher[0] = low                                      # all alike: one sixth each
+    teacher[1, :5] = low                                  # one entry takes it all
+    teacher[2] = high
+    teacher[3, ::2], teacher[3, 1::2] = high, low
+    teacher[4, 2] = NEG
+    x = logits.clone().requires_grad_()
+    r = topk_distillation(x, ids, teacher, None, tau, reduction="none")
+    (g,) = torch.autograd.grad(r.loss.sum(), x)
+    z = logits.double().cpu()
+    t = teacher.double().cpu()
+    p = torch.softmax((t - t.amax(1, keepdim=True)) / tau, 1)
+    log_q = torch.log_softmax(z / tau, 1).gather(1, ids.cpu())
+    want = tau ** 2 * (torch.special.xlogy(p, p) - torch.where(p > 0, p * log_q, 0.0)).sum(1)
+    grad = tau * torch.softmax(z / tau, 1).scatter_add(1, ids.cpu(), -p)
+    near = 64 * 2.0 ** -23 * max(1.0, 1 / tau)  # as in check(), of exponents up to 4 times as large
+    torch.testing.assert_close(r.loss.detach().double().cpu(), want, rtol=near, atol=near * max(1.0, tau ** 2))
+    torch.testing.assert_close(g.double().cpu(), grad, rtol=near, atol=near * max(tau, 1.0))
