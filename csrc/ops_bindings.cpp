@@ -309,7 +309,8 @@ kernels::DistillArgs distill_args(const Tensor& logits, const Tensor& ids, const
   TORCH_CHECK(kernels::distill_supported(C, ld, ids.size(1)), who, ": needs 1 <= n_classes <= width <= ", kernels::kDistillMaxWidth, " and 1 .. ",
               kernels::kDistillMaxEntries, " teacher entries (got ", C, ", ", ld, ", ", ids.size(1), ")");
   TORCH_CHECK(N < (1ll << 31), who, ": too many rows");
-  TORCH_CHECK(temperature > 0.0 && hard_weight >= 0.0 && hard_weight <= 1.0, who, ": needs temperature > 0 and 0 <= hard_weight <= 1");
+  TORCH_CHECK(temperature >= 1e-12 && temperature <= 1e12 && hard_weight >= 0.0 && hard_weight <= 1.0, who,
+              ": needs a temperature in 1e-12 .. 1e12 and 0 <= hard_weight <= 1");
   kernels::DistillArgs a{};
   if (targets.has_value() && targets->defined()) {
     check_gpu(*targets, "targets");

@@ -133,8 +133,8 @@ class _ProjectionTopKDistillation(torch.autograd.Function):
 def _check(N: int, n_classes: int, width: int, ids, teacher, targets, temperature: float, hard_weight: float, reduction: str, allowed) -> None:
     if reduction not in allowed:
         raise ValueError(f"reduction must be {' | '.join(allowed)}, got {reduction}")
-    if not temperature > 0 or temperature == float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-12 <= temperature <= 1e12:  # (float32 holds its reciprocal, and its square times any number of rows)
+        raise ValueError(f"temperature must lie in 1e-12 .. 1e12, got {temperature}")
     if not 0.0 <= hard_weight <= 1.0:
         raise ValueError(f"hard_weight must lie in [0, 1], got {hard_weight}")
     if hard_weight > 0 and targets is None:
@@ -201,7 +201,8 @@ def topk_distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
 
     ``targets[N]`` give the hard term (weight ``hard_weight``) and mark ignored rows; the mean is taken over rows whose
     target is not ``ignore_index`` (over all rows without targets).  ``n_classes`` < C marks trailing columns as padding:
-    they take no part and get zero gradient.  ``check_targets`` (or ``DIST_CHECK_TARGETS=1``) raises ``IndexError`` for
+    they take no part and get zero gradient.  ``temperature`` lies in 1e-12 .. 1e12, and logits divided by it are taken to stay below 2 ** 24
+    in size, beyond which float32 tells no neighbouring ones apart.  ``check_targets`` (or ``DIST_CHECK_TARGETS=1``) raises ``IndexError`` for
     a target or a teacher id beyond the classes, at the price of a host synchronisation.
     """
     if logits.dim() != 2:

@@ -732,3 +732,17 @@ def test_entries_of_the_lowest_and_largest_values_are_entries(tau, t_dtype, devi
     near = 64 * 2.0 ** -23 * max(1.0, 1 / tau)  # as in check(), of exponents up to 4 times as large
     torch.testing.assert_close(r.loss.detach().double().cpu(), want, rtol=near, atol=near * max(1.0, tau ** 2))
     torch.testing.assert_close(g.double().cpu(), grad, rtol=near, atol=near * max(tau, 1.0))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_temperatures_beyond_float32_are_refused(device):
+    logits, ids, teacher, targets = make(4, 11, 3, device=device)
+    for tau in (1e-50, 1e-30, 1e30, 1e50):
+        with pytest.raises(ValueError, match="temperature"):
+            topk_distillation(logits, ids, teacher, targets, tau, 0.5)
+        with pytest.raises(ValueError, match="temperature"):
+            projection_topk_distillation(logits, torch.randn(11, 11, device=device), ids, teacher, targets, tau, 0.5)
+    for tau in (1e-4, 1e4, 1e12):  # inside: finite, the soft term tau^2 log(C / K) of two flat distributions at last
+        r = topk_distillation(logits, ids, teacher, None, tau)
+        assert torch.isfinite(r.loss)
+    assert abs(float(r.loss) / 1e24 - math.log(11 / 3) * 3 / 4 - math.log(11 / 1) / 4) < 1e-5  # (one row keeps one entry)
