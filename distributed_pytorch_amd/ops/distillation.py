@@ -10,7 +10,7 @@ token is stored as its K largest logits with their classes; the student learns t
 vocabulary projection (the logits then exist only inside the op, in float32 whatever the tensors' type, so that the loss is as exact as that
 of float32 logits).  On gfx950 the loss and the gradient of the logits come out of one kernel that reads each row
 once.  An entry whose id is negative or not below ``n_classes``, or whose logit is ``-inf``, is absent; entries may come
-in any order, and entries of one class add up.  Rows whose target is ``ignore_index`` count for nothing and may hold
+in any order, and entries of one class add up.  No gradient reaches the teacher.  Rows whose target is ``ignore_index`` count for nothing and may hold
 anything; a row without entries keeps its hard term.
 """
 from __future__ import annotations
@@ -166,7 +166,7 @@ def _composed(logits, ids, teacher, targets, cfg) -> DistillResult:
     live = counted if targets is None else counted & (targets >= 0) & (targets < n_classes)
     z = torch.where(live.unsqueeze(1), z, z.new_zeros(()))  # an ignored row may hold anything
     row = z.new_zeros(N)
-    t = teacher.to(z.dtype)
+    t = teacher.detach().to(z.dtype)
     there = (ids >= 0) & (ids < n_classes) & (t != float("-inf"))
     if hard_weight < 1:
         at = torch.where(there, ids, 0).long()

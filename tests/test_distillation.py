@@ -746,3 +746,13 @@ def test_temperatures_beyond_float32_are_refused(device):
         r = topk_distillation(logits, ids, teacher, None, tau)
         assert torch.isfinite(r.loss)
     assert abs(float(r.loss) / 1e24 - math.log(11 / 3) * 3 / 4 - math.log(11 / 1) / 4) < 1e-5  # (one row keeps one entry)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_no_gradient_reaches_the_teacher(device):
+    logits, ids, teacher, targets = make(4, 11, 3, device=device)
+    x, t = logits.requires_grad_(), teacher.requires_grad_()
+    r = topk_distillation(x, ids, t, targets, 2.0, 0.5)
+    gx, gt = torch.autograd.grad(r.loss, (x, t), allow_unused=True)
+    assert gx is not None and gt is None
+    assert not topk_distillation(x.detach(), ids, t, targets, 2.0, 0.5).loss.requires_grad
