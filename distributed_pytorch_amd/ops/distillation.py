@@ -229,12 +229,15 @@ def projection_topk_distillation(x: torch.Tensor, weight: torch.Tensor, teacher_
                                  reduction: str = "mean", ignore_index: int = -100, n_classes: Optional[int] = None, impl: str = "native",
                                  check_targets: Optional[bool] = None) -> DistillResult:
     """``topk_distillation`` of the logits ``x @ weight.T`` (``x``: [..., K_in], ``weight``: [C, K_in]; the teacher's tensors
-    are [..., K] and ``targets`` [...] over the same leading dimensions).  reduction: mean | sum.
+    are [..., K] and ``targets`` [...] over the same leading dimensions).  reduction: mean | sum.  Ignored rows of ``x`` may hold anything
+    finite (the weight's gradient is a product with all of ``x``).
 
     bf16 training keeps the logits' gradient (2 bytes each) until the backward, beside some rows of float32 logits in passing (8 GiB at
     most); fp16 training keeps the float32 logits.  ``impl="library"`` takes the vendor's products, for comparisons: logits rounded to the tensors'
     type, and the loss with them.
     """
+    if impl not in ("native", "library"):
+        raise ValueError(f"impl must be native | library, got {impl}")
     x2 = x.reshape(-1, x.shape[-1])
     ids = teacher_ids.reshape(-1, teacher_ids.shape[-1])
     teacher = teacher_logits.reshape(-1, teacher_logits.shape[-1])

@@ -756,3 +756,60 @@ def test_no_gradient_reaches_the_teacher(device):
     gx, gt = torch.autograd.grad(r.loss, (x, t), allow_unused=True)
     assert gx is not None and gt is None
     assert not topk_distillation(x.detach(), ids, t, targets, 2.0, 0.5).loss.requires_grad
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_an_unknown_product_is_refused(device):
+    _, ids, teacher, targets = make(4, 11, 3, device=device)
+    with pytest.raises(ValueError, match="impl"):
+        projection_topk_distillation(torch.randn(4, 8, device=device), torch.randn(11, 8, device=device), ids, teacher, impl="stock")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_projection_of_views_and_single_gradients(dtype):
+    x, w, ids, teacher, targets = projected(120, 1003, 96, dtype)
+    up = 256.0
+
+    def run(a, b, names="xw", **kw):
+        a, b = a.detach().requires_grad_("x" in names), b.detach().requires_grad_("w" in names)
+        r = projection_topk_distillation(a, b, ids, teacher, targets, 2.0, 0.5, **kw)
+        return r.loss.detach(), dict(zip(names, torch.autograd.grad(r.loss * up, [a if n == "x" else b for n in names])))
+
+    loss, want = run(x, w)
+    for names in ("x", "w"):
+        one, got = run(x, w, names)
+        assert torch.equal(one, loss) and torch.equal(got[names], want[names])
+    off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)  # noqa: E731  one element off a 16-byte boundary
+    turned = lambda t: t.t().contiguous().t()  # noqa: E731
+    for view in (off, turned):
+        same, got = run(view(x), view(w))
+        assert torch.equal(same, loss) and torch.equal(got["x"], want["x"]) and torch.equal(got["w"], want["w"])
+    # the vendor's products: logits rounded to the type, half a step of about 2 at most; gradients of those
+    other, got = run(x, w, impl="library")
+    half = torch.finfo(dtype).eps / 2
+    assert abs(float(other) - float(loss)) <= 4 * half * 2 + 2e-5
+    for n in "xw":
+        assert float((got[n].float() - want[n].float()).norm()) <= (8 * half + 2e-5) * float(want[n].float().norm())
+
+
+@gpu
+def test_projections_on_two_streams():
+    a, b = projected(2100, 4100, 64, torch.bfloat16, 1), projected(2100, 4100, 64, torch.bfloat16, 2)
+
+    def grads(t):
+        x, w = t[0].detach().requires_grad_(), t[1].detach().requires_grad_()
+        r = projection_topk_distillation(x, w, *t[2:], 2.0, 0.5)
+        return (r.loss.detach(), *torch.autograd.grad(r.loss, (x, w)))
+
+    want = [grads(a), grads(b)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            ga = grads(a)
+        with torch.cuda.stream(s2):
+            gb = grads(b)
+        torch.cuda.synchronize()
+        for got, w in ((ga, want[0]), (gb, want[1])):
+            assert all(torch.equal(p, q) for p, q in zip(got, w))

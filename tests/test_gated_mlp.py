@@ -438,3 +438,16 @@ def test_frozen_tensors_leave_the_other_gradients_as_they_are(M, K, H, N, dtype)
         y = gated_mlp(leaf["x"], leaf["w_fc"], leaf["b_fc"], leaf["w_proj"], leaf["b_proj"])
         for n, g in zip(names, torch.autograd.grad(y, [leaf[n] for n in names], dy)):
             assert torch.equal(g, want["d" + n]), (n, frozen)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,K,H,N", [(50, 72, 130, 67), (300, 64, 256, 129), (2100, 40, 96, 33), (150, 1, 24, 7)])
+def test_an_upstream_gradient_that_starts_anywhere(M, K, H, N, dtype):
+    t, dy = make(M, K, H, N, dtype)
+    want = run(t, dy, "silu")
+    off = torch.cat([dy.new_zeros(1), dy.reshape(-1)])[1:].view(M, N)
+    got = run(t, off, "silu")
+    assert off.is_contiguous() and off.data_ptr() % 16 and set(got) == set(want)
+    for k in want:  # (other loads, the same sums)
+        assert torch.equal(got[k], want[k]), k
