@@ -269,7 +269,7 @@ void launch_gemm_f32(const GemmArgs& a, hipStream_t stream) {
 }
 
 // Shares of the contraction for a product with few tiles (see gemm_spread): a k-step is 1.7 us of matrix work here, one workgroup a compute unit keeps
-// it busy, and at least 8 steps have to be saved (464 x 2112 x 685: 67 -> 34 us, 64 x 2048 x 768: 68 -> 17, 512^3: 50 -> 19, 1024 x 768 x 384, 9
+// it busy, and at least 8 steps have to be saved (464 x 2112 x 685: 67 -> 34 us, 64 x 2048 x 768: 68 -> 17, 512^3: 50 -> 19, 1024 x 768 x 384, 8
 // saved: 42 -> 23).
 int gemm_f32_spread(const GemmArgs& a, int compute_units) {
   const long long tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN), nk = (a.K + BK - 1) / BK;

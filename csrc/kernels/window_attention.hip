@@ -14,7 +14,7 @@
 // products run transposed (S^T = K Q^T), so a query's softmax statistics are scalars of its lane and the probabilities leave the
 // accumulators as the operand of the next product without changing lanes; the other operand of that product comes
 // from the row-major tile through the transposing LDS read.  Probabilities and score gradients are rounded to the 16-bit type there, as operands
-// of a matrix instruction have to be; scores, statistics, delta and all sums are fp32, and the row sums add up the rounded probabilities, so that
+// of a matrix instruction have to be; scores, statistics, delta (of the output as it is stored) and all sums are fp32, and the row sums add up the rounded probabilities, so that
 // a row's weights sum to 1.  Tiles travel global -> LDS by DMA, requested one tile (two in the dK/dV kernel at head size 128) ahead.  The tile image is one for both kinds of reads: 16-byte chunk c of row r sits at chunk c ^ swz(r).  The 16 lanes that a row-wise
 // read serves at once (rows 0-3 and 12-15 at one chunk, rows 4-11 at the next) then fall on 16 different 16-byte bank groups, and the 8
 // rows of a transposing read on 8 different 32-byte groups.
@@ -27,9 +27,12 @@
 // sums, which a last kernel adds up in order: no atomics, the same result every time.
 //
 // Measured (bf16), window 256 / sinks 4 over 64 x 1024 positions, 12 heads of 64: forward 128 us (3.1 TB/s of its inputs and outputs), dQ 174 us
-// (3.5 TB/s), dK/dV 222 us (2.7 TB/s): between the memory's rate and the vector work per score (an exponential, a product and half a
-// conversion beside 2 to 4 x 64 multiply-adds).  Window 1024 / sinks 4 over 16384 positions, 8 heads of 128 on 2: forward 105 us (636 TFLOP/s of
-// the visible pairs), dQ 127 us (784), dK/dV 257 us (520; one workgroup a compute unit, its accumulators and K / V rows fill the registers), join 17 us.
+// (3.5 TB/s), dK/dV 215 us (2.8 TB/s).  Neither memory nor the matrix pipes (21 - 35 % busy) are what bounds them: by the counters a square of 32 x 32 scores
+// takes 160 vector and 106 scalar instructions in the forward (166 and 103 in dQ, 174 and 126 in dK/dV) beside its 18 to 32 products -- 10 vector
+// instructions a score, of which the softmax needs about 4; the others are the mask's comparisons, addresses, and prologues and epilogues over the fewer than
+// nine squares that a wave has here -- and the waves wait for the rest (the forward at head size 64 spills 2 registers, dK/dV 9).  Window 1024 / sinks 4 over 16384 positions, 8 heads of 128 on 2: forward 105 us (636 TFLOP/s of
+// the visible pairs), dQ 127 us (784), dK/dV 257 us (520; one workgroup a compute unit: its stages and strips are 131 of 160 KiB
+// of LDS, and a wave a SIMD, at 304 of 512 registers, has nothing to run while it waits, 48 % of its cycles), join 17 us.
 #include <type_traits>
 
 #include "device_utils.h"
@@ -772,7 +775,7 @@ struct Part {
   }
 };
 
-// A piece is walked as one stream: the requests run two units ahead of the products, across the end of a block into the next one, and the
+// A piece is walked as one stream: the requests run one unit (two at head size 128) ahead of the products, across the end of a block into the next one, and the
 // next block's K and V rows are fetched while the finished one is stored (18 KiB of LDS of its own for that), so only a piece's first
 // block waits for memory.  (Starting every block by itself -- unit arithmetic with 64-bit divisions, requests, K / V, two trips to memory --
 // cost about as much as 4 of its 6 units at a window of 256.)
