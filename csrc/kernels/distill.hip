@@ -10,16 +10,16 @@
 //
 // One workgroup per row.  The row is read once: every thread keeps its 16-byte vectors packed in registers through the
 // maximum, the two sums of exponentials and the gradient, so a fused call moves exactly one read and one write of the
-// logits (rows too wide for the registers are read again, out of L2 / Infinity Cache).  With one temperature in play (tau = 1, a = 0
-// or a = 1) there is one exponential per element and pass; otherwise the one at temperature 1 is a power of the other where tau is 2 or 4,
+// logits.  Rows too wide for the registers are read twice, the second time out of the 256 MB cache: maximum and sums are then taken in one pass.
+// With one temperature in play (tau = 1, a = 0 or a = 1) there is one exponential per element and pass; otherwise the one at temperature 1 is a power of the other where tau is 2 or 4,
 // and a second exponential for other tau (an exponential takes four issue slots, a power one or two).
 // The K teacher entries (and the label, as one more) are a scatter into the row.  A vector that is about to be stored has to know its entries: LDS
 // holds one bit per vector (a wave's 64 vectors are one 64-bit word, so most waves skip the look-up on a scalar
 // branch) and a chained hash from vector to entries.  Entries of one class are summed beforehand in index order by the
 // first of them, which makes the result independent of the order in which the chains were built.
-// Bound by memory with one temperature: 8192 x 50304 bf16, 32 entries, forward and gradient in 340 us (4.85 TB/s, the rate of a copy); 2049 x 50257
-// fp32 with a second exponential 203 us (4.1 TB/s).  With both temperatures and powers 24576 x 50304 float32 logits and their
-// bf16 gradient take 2.23 ms (3.3 TB/s): a row of 200 KB fills most of a compute unit's registers, so that one is fetched, computed and stored at a time.
+// Bound by memory with one temperature: 8192 x 50304 bf16, 32 entries, every row counted, forward and gradient in 345 us (4.8 TB/s, the rate of a
+// copy); 2049 x 50257 fp32 with a second exponential 228 us (3.6 TB/s).  With both temperatures and powers 24576 x 50304 float32 logits and their
+// bf16 gradient take 1.75 ms (4.2 TB/s of one reading and the gradient).
 // Everything is fp32 but the logits and their gradient; in fp16 the gradient is only ever rounded with the upstream gradient in it.
 // Rows need no alignment: element j of a row sits in vector (j + shift) / V of the 16-byte grid, the vectors at both ends are stored
 // element by element.
@@ -36,6 +36,7 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kNone = 0x7fffffff;
+constexpr float kLowest = -3.4028234663852886e38f;  // an exponent below every other: nothing has been added up yet
 constexpr long long kRowsPerLaunch = 1 << 21;  // a launch counts its threads (1024 a row at most) in 32 bits
 enum Mode : int { kForward = 0, kBackward = 1, kFused = 2 };
 
@@ -146,9 +147,17 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
 #pragma unroll
       for (int q = 0; q < KEEP; ++q) keep_packed(kept[q]);
     } else {
-      for (int k = tid; k < nvec; k += THREADS) {
-        raw16 v = *reinterpret_cast<const raw16*>(grid_in + 16u * static_cast<unsigned>(k));
-        one(k, v);
+      constexpr int AHEAD = 4;  // vectors on their way at a time
+      for (int k0 = tid; k0 < nvec; k0 += AHEAD * THREADS) {
+        raw16 v[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+          if (k0 + q * THREADS < nvec) v[q] = *reinterpret_cast<const raw16*>(grid_in + 16u * static_cast<unsigned>(k0 + q * THREADS));
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+          if (k0 + q * THREADS < nvec) one(k0 + q * THREADS, v[q]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   };
@@ -185,9 +194,15 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     }
   }
 
+  auto power = [](float e) __attribute__((always_inline)) {  // of an exponential at temperature 2 / 4, the one at temperature 1
+    const float e2 = e * e;
+    return SECOND == 2 ? e2 : e2 * e2;
+  };
+
   // ---- row maximum: of whole vectors, three values an instruction; which element it is, only its owners look up
   const float c = a.exp_scale;  // log2(e) / temperature of the first exponential
   float m, mt = kNegInf, S = 0.f, S1 = 0.f;
+  float s = 0.f, s1 = 0.f, at = kLowest, at1 = kLowest;  // (rows read again: sums so far, relative to this thread's largest exponents so far)
   int best = kNone;
   if (MODE == kBackward) {
     m = a.row_stats[3 * r];
@@ -201,6 +216,27 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
 #pragma unroll
       for (int j = 0; j < V; ++j) vm = fmaxf(vm, decltype(whole)::value || !outside(k, j) ? x[j] : kNegInf);
       if (vm > mt) { mt = vm; best = k; }
+      if constexpr (KEEP == 0) {
+        // A row that is not kept would have to be read once more for the sums: they are taken along, and follow the maximum.
+        const float to = fmaxf(at, vm * c), f = __builtin_amdgcn_exp2f(at - to);
+        at = to;
+        s *= f;
+        if (SECOND == 1) {
+          const float to1 = fmaxf(at1, vm * kLog2e);
+          s1 *= __builtin_amdgcn_exp2f(at1 - to1);
+          at1 = to1;
+        } else if (SECOND) {
+          s1 *= power(f);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (!decltype(whole)::value && outside(k, j)) x[j] = kNegInf;
+          const float e = __builtin_amdgcn_exp2f(fmaf(x[j], c, -at));
+          s += e;
+          if (SECOND == 1) s1 += __builtin_amdgcn_exp2f(fmaf(x[j], kLog2e, -at1));
+          else if (SECOND) s1 += power(e);
+        }
+      }
     });
     m = mt;
 #pragma unroll
@@ -215,8 +251,7 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
   const float mc = m * c, mc1 = m * kLog2e;
   auto second = [&](float x, float e) __attribute__((always_inline)) {
     if (SECOND == 1) return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -mc1));
-    const float e2 = e * e;
-    return SECOND == 2 ? e2 : e2 * e2;
+    return power(e);
   };
   if (MODE != kBackward) {
     int arg = kNone;
@@ -245,8 +280,13 @@ __global__ __launch_bounds__(THREADS, WAVES_PER_SIMD) void distill_kernel(Distil
     if (lane == 0) s_arg[wid] = arg;
 
     // ---- sums of exponentials at both temperatures
-    float s = 0.f, s1 = 0.f;
-    each_vec([&](int k, const raw16& v, auto whole) __attribute__((always_inline)) {
+    if constexpr (KEEP == 0) {
+      const float f = __builtin_amdgcn_exp2f(at - mc);
+      s *= f;
+      if (SECOND == 1) s1 *= __builtin_amdgcn_exp2f(at1 - mc1);
+      else if (SECOND) s1 *= power(f);
+    }
+    else each_vec([&](int k, const raw16& v, auto whole) __attribute__((always_inline)) {
       float x[V];
       raw_to_f32<TR, V>(v, x);
 #pragma unroll
@@ -483,6 +523,7 @@ void launch_distill(const DistillArgs& args, int dtype, int out_dtype, int mode,
       constexpr integral_constant<int, 8> w8{};
       constexpr integral_constant<int, 64> t64{};
       constexpr integral_constant<int, 256> t256{};
+      [[maybe_unused]] constexpr integral_constant<int, 512> t512{};
       constexpr integral_constant<int, 1024> t1024{};
       constexpr integral_constant<int, 0> none{};
       if constexpr (MODE == kBackward) {
@@ -493,8 +534,15 @@ void launch_distill(const DistillArgs& args, int dtype, int out_dtype, int mode,
         if (nvec <= 64 * 4) go(t64, integral_constant<int, 4>{}, m, w4);
         else if (nvec <= 256 * 7) go(t256, integral_constant<int, 7>{}, m, w4);
         else if (nvec <= 1024 * 7) go(t1024, integral_constant<int, 7>{}, m, w8);
-        else if (nvec <= 1024 * 16) go(t1024, integral_constant<int, 16>{}, m, w4);
-        else go(t1024, none, m, w8);
+        else if constexpr (std::is_same<TR, TO>::value) {
+          if (nvec <= 1024 * 16) go(t1024, integral_constant<int, 16>{}, m, w4);
+          else go(t1024, none, m, w8);
+        } else {
+          // Float32 logits of a projection, twice the bytes of their gradient: held, a row takes a whole compute unit's registers and is fetched, computed
+          // and stored by itself (24576 x 50304: 2.25 ms); read twice, four rows share one and the second reading comes out of the 256 MB cache (1.75 ms;
+          // with two rows of 1024 threads 1.91, with eight of 256, whose 400 MB do not stay there, 2.24).
+          go(t512, none, m, w8);
+        }
       }
     };
     for (a.row0 = 0; a.row0 < args.N; a.row0 += kRowsPerLaunch) {

@@ -813,3 +813,27 @@ def test_projections_on_two_streams():
         torch.cuda.synchronize()
         for got, w in ((ga, want[0]), (gb, want[1])):
             assert all(torch.equal(p, q) for p, q in zip(got, w))
+
+
+# rows of float32 logits that are read twice, with the sums taken along with the maximum: one vector a thread, several, and a ragged last one
+@gpu
+@pytest.mark.parametrize("N,V,C", [(7, 28676, 28676), (5, 30011, 29000), (40, 50304, 50257), (3, 131083, 131083)])
+@pytest.mark.parametrize("tau,a", [(1.0, 0.0), (2.0, 0.5), (4.0, 0.25), (3.0, 0.5), (2.0, 1.0)])
+def test_wide_projected_rows(N, V, C, tau, a):
+    from distributed_pytorch_amd import _ext
+
+    x, w, ids, teacher, targets = projected(N, V, 64, torch.bfloat16, K=9, C=C)
+    x = x * 12                                       # logits of about 2, with a long tail
+    x[1] = 0                                         # all alike
+    targets[2] = -100
+    r = _ext.C().projection_distill_forward(x, w, ids, teacher, targets, C, -100, tau, a, True, "gradient")
+    z = x.double() @ w.double().t()
+    rows, grad, n = reference(z, ids, teacher, targets, tau, a, C)
+    near = 64 * 2.0 ** -23                           # as in check()
+    size = max(1.0, tau ** 2) * (1 + float(rows.abs().max()) / max(1.0, tau ** 2))
+    assert abs(float(r[0]) - float(rows.sum()) / n) <= near * size
+    torch.testing.assert_close(r[6].double().cpu(), grad / n, rtol=2.0 ** -9 * 2.02, atol=near * max(tau, 1.0) / n)
+    best = z[:, :C].argmax(1).cpu()
+    top = z[:, :C].topk(2, 1).values.cpu()
+    sure = (top[:, 0] - top[:, 1] > 1e-4) & (targets.cpu() != -100)
+    assert torch.equal(r[1].cpu()[sure], (best == targets.cpu())[sure])
