@@ -36,7 +36,9 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kNone = 0x7fffffff;
-constexpr float kLowest = -3.4028234663852886e38f;  // an exponent below every other: nothing has been added up yet
+// An exponent below those of all logits that count (2^24 in size after the division by tau), where nothing has been added up yet.  Not lower: relative to itself
+// a logit of -1e30 or the type's lowest value, as masks have, would be off by the rounding of its exponent, which is then beyond any float's.
+constexpr float kLowest = -1e8f;
 constexpr long long kRowsPerLaunch = 1 << 21;  // a launch counts its threads (1024 a row at most) in 32 bits
 enum Mode : int { kForward = 0, kBackward = 1, kFused = 2 };
 

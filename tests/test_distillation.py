@@ -837,3 +837,32 @@ def test_wide_projected_rows(N, V, C, tau, a):
     top = z[:, :C].topk(2, 1).values.cpu()
     sure = (top[:, 0] - top[:, 1] > 1e-4) & (targets.cpu() != -100)
     assert torch.equal(r[1].cpu()[sure], (best == targets.cpu())[sure])
+
+
+# classes hidden by a large negative logit: whole threads see nothing else at first, on rows that are held, read twice, and read again in the backward
+@gpu
+@pytest.mark.parametrize("hide", [-1e9, -1e30, "lowest", NEG])
+@pytest.mark.parametrize("C,dtype", [(900, torch.float32), (20011, torch.bfloat16), (70001, torch.float32), (140003, torch.bfloat16), (140003, torch.float16)])
+def test_hidden_classes(C, dtype, hide):
+    if dtype == torch.float16 and hide in (-1e9, -1e30):
+        hide = "lowest"
+    value = torch.finfo(dtype).min if hide == "lowest" else hide
+    logits, ids, teacher, targets = make(4, C, 6, dtype, DEV, pad_rows=False)
+    logits = logits + 20
+    g = torch.Generator().manual_seed(C)
+    open_ = [torch.arange(C - 50, C), torch.arange(0, 50), torch.randperm(C, generator=g)[:50], torch.arange(C)]
+    for r, keep in enumerate(open_):
+        row = torch.full((C,), value, dtype=dtype, device=DEV)
+        row[keep.to(DEV)] = logits[r, keep.to(DEV)]
+        logits[r] = row
+        ids[r] = keep[torch.randperm(len(keep), generator=g)[:6]].to(DEV)
+        targets[r] = int(keep[7])
+    for tau, a in ((1.0, 0.0), (2.0, 0.5), (4.0, 0.25), (3.0, 0.5)):
+        check(logits, ids, teacher, targets, tau, a)
+        x = logits.clone().requires_grad_()
+        r = topk_distillation(x, ids, teacher, targets, tau, a, reduction="none")
+        rows, grad, _ = reference(logits, ids, teacher, targets, tau, a)
+        near = 64 * 2.0 ** -23 * max(1.0, tau ** 2)
+        torch.testing.assert_close(r.loss.detach().double().cpu(), rows, rtol=near, atol=near)
+        (d,) = torch.autograd.grad(r.loss.sum(), x)
+        torch.testing.assert_close(d.double().cpu(), grad, rtol=torch.finfo(dtype).eps / 2 * 1.01, atol=near + (2.0 ** -25 if dtype == torch.float16 else 0.0))
